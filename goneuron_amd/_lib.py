@@ -49,6 +49,13 @@ class KernelStat(C.Structure):
                 ("units", C.c_double)]
 
 
+class KVCache(C.Structure):
+    """gn_kv_cache: device pointers and sizes of a paged 8-bit cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("table", C.c_void_p), ("pages", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("max_pages", C.c_int32)]
+
+
 class Info(C.Structure):
     _fields_ = [("arch", C.c_char * 64), ("cu_count", C.c_int32), ("hbm_bytes", C.c_int64),
                 ("peak_fp32_mfma_tflops", C.c_double), ("peak_hbm_gbps", C.c_double)]
@@ -154,6 +161,19 @@ SIGNATURES = {
     "gn_moe_workspace": (C.c_int, [C.c_int32] * 5 + [C.POINTER(C.c_int64)]),
     "gn_moe_forward": (C.c_int, [vp] + [vp] * 4 + [C.c_int32] * 6 + [C.POINTER(C.c_uint64)]),
     "gn_moe_backward": (C.c_int, [vp] + [vp] * 6 + [C.c_int32] * 6 + [C.c_float]),
+    "gn_kv_cache_bytes": (C.c_int, [C.c_int32] * 4 + [C.POINTER(C.c_int64), i32p]),
+    "gn_rope_tables": (C.c_int, [vp, vp, vp, C.c_int32, C.c_int32]),
+    "gn_kv_append": (C.c_int, [vp, C.POINTER(KVCache), vp, vp, vp, vp] + [C.c_int64] * 4 + [vp, vp, C.c_int32, vp, vp]
+                     + [C.c_int32] * 5 + [vp]),
+    "gn_kv_attention_workspace": (C.c_int, [C.c_int32] * 6 + [C.POINTER(C.c_int64)]),
+    "gn_kv_attention": (C.c_int, [vp, C.POINTER(KVCache), vp, vp, C.c_int64, C.c_int64, vp, vp] + [C.c_int32] * 5
+                        + [C.c_float, C.c_int32, C.c_int32, vp, vp]),
+    "gn_mha_cached_workspace": (C.c_int, [C.c_int32] * 6 + [C.POINTER(C.c_int64)]),
+    "gn_mha_cached_forward": (C.c_int, [vp, C.POINTER(KVCache)] + [vp] * 5 + [C.c_int32, vp, vp] + [C.c_int32] * 5
+                              + [vp, vp]),
+    "gn_sample_workspace": (C.c_int, [C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
+    "gn_sample": (C.c_int, [vp, vp, C.c_int64, C.c_int32] + [vp] * 6 + [C.c_int32, C.c_int32, vp]),
+    "gn_model_sample": (C.c_int, [vp, vp, C.c_int32] + [vp] * 6),
     "gn_gemm": (C.c_int, [vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_float, vp,
                           C.c_int32, vp, C.c_int32, vp, C.c_int32]),
     "gn_adam_step": (C.c_int, [vp, vp, vp, vp, vp, C.c_int64, C.c_float, C.c_float, C.c_float,

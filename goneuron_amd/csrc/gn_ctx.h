@@ -193,7 +193,8 @@ struct MhaBufs {
   float *Q, *K, *V, *O, *GO, *GQ, *GK, *GV, *S, *S3, *rcos, *rsin, *SC;
   int64_t s3_stride;
 };
-void rope_tables(int T, int hd, std::vector<float> &cs, std::vector<float> &sn);
+// angles of positions p0 .. p0 + T - 1
+void rope_tables(int T, int hd, std::vector<float> &cs, std::vector<float> &sn, int p0 = 0);
 int mha_forward_impl(gn_ctx *c, const float *x, const float *params, float *out, const MhaBufs &m,
                      int B, int T, int D, int NH, int causal, int rope);
 int mha_backward_impl(gn_ctx *c, const float *x, const float *params, const float *gout, float *grads,

@@ -270,14 +270,14 @@ int mha_check(gn_ctx *c, int B, int T, int D, int NH) {
 }  // namespace
 
 // applyRoPE's angles (transformer.go:215-221) in float32, as the reference
-void rope_tables(int T, int hd, std::vector<float> &cs, std::vector<float> &sn) {
+void rope_tables(int T, int hd, std::vector<float> &cs, std::vector<float> &sn, int p0) {
   const int half = hd / 2;
   cs.assign((size_t)T * std::max(half, 1), 0.f);
   sn.assign(cs.size(), 0.f);
   for (int t = 0; t < T; ++t)
     for (int k = 0; k < half; ++k) {
       const float theta = (float)pow(10000.0, -(double)(2 * k) / (double)hd);
-      const float mt = (float)t * theta;
+      const float mt = (float)(p0 + t) * theta;
       cs[(size_t)t * half + k] = (float)cos((double)mt);
       sn[(size_t)t * half + k] = (float)sin((double)mt);
     }

@@ -22,6 +22,7 @@
 
 #include "gn_common.h"
 #include "gn_ctx.h"
+#include "gn_serve.h"
 
 using namespace gn;
 
@@ -3276,6 +3277,49 @@ extern "C" int gn_model_predict_device(gn_model *M, const float *x, int32_t B, f
   LayerRT &O = M->L.back();
   HIP_OK(c, hipMemcpyAsync(out, O.out, (size_t)B * O.out_len * sizeof(float),
                            hipMemcpyDeviceToDevice, c->stream));
+  return GN_OK;
+}
+
+// One prediction and a draw from every sample's outputs, in the context's scratch
+// (as many rows at a time as it holds).
+extern "C" int gn_model_sample(gn_model *M, const float *x, int32_t B, const float *temperature,
+                               const int32_t *top_k, const float *top_p, const float *min_p, const float *u,
+                               int32_t *ids) {
+  if (!M) return GN_ERR_INVALID;
+  gn_ctx *c = M->ctx;
+  ENTRY(c);
+  if (B <= 0 || B > M->maxB || !x || !u || !ids) return set_err(c, GN_ERR_INVALID, "bad sample args");
+  LayerRT &O = M->L.back();
+  if (O.d.kind == GN_LAYER_DENSE && O.d.act == GN_ACT_SOFTMAX && O.d.act_is_ptr)
+    return set_err(c, GN_ERR_UNSUPPORTED, "sample: the last layer gives probabilities, not logits");
+  if (O.out_len > SAMPLE_MAX_V)
+    return set_err(c, GN_ERR_UNSUPPORTED, "sample: %lld outputs, more than %d", (long long)O.out_len, SAMPLE_MAX_V);
+  for (LayerRT &R : M->L) R.train = 0;
+  int rc = pass_flags(M, B, false);
+  if (rc) return rc;
+  M->last_predict = true;
+  rc = model_forward(M, x, B, false);
+  if (rc) return rc;
+  M->last_B = B;
+  const int V = (int)O.out_len;
+  int rows = std::min(B, 65535);
+  while (rows > 1 && sample_work_floats(rows, V) > (int64_t)c->scratch_floats) rows = (rows + 1) / 2;
+  for (int b = 0; b < B; b += rows) {
+    SampleArgs a{};
+    a.z = O.out + (int64_t)b * V;
+    a.stride = V;
+    a.temperature = temperature ? temperature + b : nullptr;
+    a.top_k = top_k ? top_k + b : nullptr;
+    a.top_p = top_p ? top_p + b : nullptr;
+    a.min_p = min_p ? min_p + b : nullptr;
+    a.u = u + b;
+    a.ids = ids + b;
+    a.B = std::min(rows, B - b);
+    a.V = V;
+    a.work = c->scratch;
+    KTimer kt(c, GN_KCLASS_OTHER, "sample", f4((double)a.B * V));
+    HIP_OK(c, launch_sample(a, GN_DTYPE_F32, c->stream));
+  }
   return GN_OK;
 }
 

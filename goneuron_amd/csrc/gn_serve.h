@@ -1,0 +1,65 @@
+// Library-private: the operators that answer token by token (paged 8-bit
+// cache, attention over it, sampling), kernels in k_kv.hip and k_sample.hip,
+// entry points in gn_serve.hip.
+#pragma once
+#include "gn_common.h"
+
+namespace gn {
+
+constexpr int KV_MAX_HEAD = 256;
+constexpr int KV_MAX_SCALE_EXP = -100;  // smallest block scale: 2^-100
+// the padded row of a head: what the kernels are built for
+inline int kv_row(int hd) {
+  return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : hd <= 192 ? 192 : 256;
+}
+
+// one call's view of the cache and of the packed sequences
+struct KvArgs {
+  uint8_t *k, *v;
+  float *ks, *vs;
+  const int32_t *table, *starts, *lens;
+  int32_t *bad;
+  int pages, P, lgP, KVH, hd, R, max_pages;
+  int B, N, max_new, max_len;
+};
+
+struct KvAppendArgs {
+  KvArgs c;
+  const void *q, *x[2];  // queries, (keys, values)
+  void *qo;
+  int64_t qs, xs[2], qos;
+  const float *cs, *sn;  // null: no rotation
+  int rope_len, H;
+  int touch;             // pages a sequence's new tokens can lie in
+  int qtok, qtiles;      // tokens of one rotation block, blocks a sequence
+  int vec;               // rows, tables and halves allow 4-value accesses
+};
+hipError_t launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s);
+
+struct KvAttnArgs {
+  KvArgs c;
+  const void *q;
+  void *out;
+  int64_t qs, os;
+  int H, G;  // query heads, query heads a key head
+  float scale;
+  int causal;
+  float *work;
+};
+int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd);
+hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, hipStream_t s);
+
+struct SampleArgs {
+  const void *z;
+  int64_t stride;
+  const float *temperature, *top_p, *min_p, *u;
+  const int32_t *top_k;
+  int32_t *ids;
+  int B, V;
+  float *work;
+};
+constexpr int SAMPLE_MAX_V = 1 << 20;
+int64_t sample_work_floats(int B, int V);
+hipError_t launch_sample(const SampleArgs &a, int dtype, hipStream_t s);
+
+}  // namespace gn

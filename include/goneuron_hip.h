@@ -237,6 +237,12 @@ int gn_model_predict(gn_model *m, const float *x, int32_t B, float *out);
 /* The same with HBM-resident x (B x in_size) and output (B x out_size); no
  * host synchronisation (the device-side ForwardBatch of sequential.go:145-160). */
 int gn_model_predict_device(gn_model *m, const float *x_dev, int32_t B, float *out_dev);
+/* gn_model_predict_device and a draw from each sample's outputs as logits (gn_sample's settings;
+ * device pointers, ids: B int32).  No counterpart in the reference.  The last
+ * layer must give logits or log-probabilities: a Dense Softmax pointer is
+ * GN_ERR_UNSUPPORTED. */
+int gn_model_sample(gn_model *m, const float *x_dev, int32_t B, const float *temperature, const int32_t *top_k,
+                    const float *top_p, const float *min_p, const float *u, int32_t *ids);
 /* Network.SetTraining (net.go:187-193): sets the flag of every layer.  Layers
  * start as the reference constructs them (Dropout and BatchNorm2D in training
  * mode, MoE not: dropout.go:56, batchnorm2d.go:88, moe.go:46-90); Predict
@@ -516,6 +522,120 @@ int gn_moe_forward(gn_ctx *ctx, const float *x, const float *params, float *out,
 int gn_moe_backward(gn_ctx *ctx, const float *x, const float *params, const float *gout, float *grads,
                     float *gin, float *work, int32_t B, int32_t I, int32_t O, int32_t E, int32_t K,
                     int32_t training, float scale);
+
+/* ---- answering token by token ---------------------------------------------
+ * No counterpart in the reference, whose Predict runs the whole window for
+ * every token.  A paged cache of rotated keys and values in 8 bits, the
+ * attention that reads it, and the draw of the next token.  Device pointers;
+ * calls queue work on the context's stream, allocate nothing, do not
+ * synchronise (but gn_rope_tables) and can be captured into a graph, which
+ * then reads starts, lens, the page table and every row's settings anew at
+ * each replay.  Calls that may run at the same time (two contexts, two graphs)
+ * need a `work` each.
+ *
+ * Tokens are packed: sequence b's new tokens are the rows starts[b] ..
+ * starts[b + 1] - 1 (starts: B + 1 int32) of the inputs and outputs, at the
+ * positions lens[b], lens[b] + 1, ... (lens: B int32, the tokens cached before
+ * the call; the caller advances it after the step).  A sequence may have no
+ * new token; rows outside every sequence are neither read nor written. */
+#define GN_DTYPE_F32 0
+#define GN_DTYPE_BF16 1
+
+/* The cache's memory, all of it the caller's.  Pages of page_size tokens (16,
+ * 32, 64 or 128), head_dim 1 to 256.  Bytes are E4M3 (sign, 4 exponent, 3
+ * mantissa bits; 0x7f NaN); a byte stands for its value times the power of two
+ * in the scale of its page and head.  Position p of sequence b is token p %
+ * page_size of page table[b * max_pages + p / page_size].  Zero a new cache's
+ * k and v once (gn_memset_zero); scales need no start.  While a call
+ * appends to a page, that page belongs to one sequence; full pages may stand
+ * in several sequences' tables. */
+typedef struct gn_kv_cache {
+  void *k;              /* pages x kv_heads x page_size x row */
+  void *v;              /* pages x kv_heads x row x page_size (transposed) */
+  float *k_scale;       /* pages x kv_heads */
+  float *v_scale;       /* pages x kv_heads */
+  const int32_t *table; /* B x max_pages */
+  int32_t pages, page_size, kv_heads, head_dim, max_pages;
+} gn_kv_cache;
+/* bytes of k (and of v) and the padded row: head_dim rounded up to 32, 64, 96,
+ * 128, 192 or 256. */
+int gn_kv_cache_bytes(int32_t pages, int32_t page_size, int32_t kv_heads, int32_t head_dim, int64_t *bytes,
+                      int32_t *row);
+/* applyRoPE's angles (transformer.go:212-236) of positions 0 .. positions - 1
+ * for heads of head_dim, the same numbers as gn_mha_forward uses: cos and sin
+ * are positions x (head_dim / 2) floats.  Synchronises. */
+int gn_rope_tables(gn_ctx *ctx, float *cos, float *sin, int32_t positions, int32_t head_dim);
+/* Rotates new queries and keys by their positions and appends keys and values
+ * to the cache, one launch.  q: rows of heads x head_dim, k and v: rows of
+ * kv_heads x head_dim, in dtype; strides in elements from one token's row to
+ * the next (queries, keys and values may lie side by side in one matrix).  The
+ * pair (x_i, x_{i + head_dim/2}) turns by (cos, sin)[position][i]; cos and sin
+ * null: nothing turns.  q_out (may be q itself, with its stride) receives the
+ * queries in dtype; q and q_out null: keys and values only.  N: rows of the
+ * inputs; max_new: the largest number of new tokens of a sequence; rope_len:
+ * positions in cos and sin.
+ * The scale of a block (one page, one head, K or V apart) is the smallest power
+ * of two, 2^-100 at least, that brings its finite values within 448, or the
+ * block's scale so far if that is larger and the block holds tokens already;
+ * where it grows, the tokens already there are scaled to it (exact but for what
+ * falls below the smallest E4M3 step).  A rotated value is rounded to float32
+ * and then to the nearest E4M3 value, ties to even; a value that is not finite
+ * is kept as NaN.
+ * bad (may be null; B int32, cleared by the caller): set to 1 for a sequence
+ * that is skipped whole because its starts or lens lie outside [0, N] or the
+ * table, it has more than max_new tokens or positions beyond rope_len, and for
+ * one with a page outside [0, pages), whose tokens are not stored. */
+int gn_kv_append(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, const void *k, const void *v, void *q_out,
+                 int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos,
+                 const float *sin, int32_t rope_len, const int32_t *starts, const int32_t *lens, int32_t B, int32_t N,
+                 int32_t max_new, int32_t heads, int32_t dtype, int32_t *bad);
+/* out = softmax(scale q K^T) V over each sequence's cache, after its new
+ * tokens were appended: a query at position p sees positions 0 .. p (causal) or
+ * all of lens[b] + new tokens.  heads must be a multiple of kv_heads (query head
+ * h reads key head h / (heads / kv_heads)).  q, out: N rows of heads x head_dim
+ * in dtype.  max_len: an upper bound of lens[b] + new tokens, from which (with
+ * max_new) the work is split; a sequence beyond it is skipped.  Sums and
+ * maxima are float32; the products of float32 queries have float32's precision,
+ * bfloat16 ones round the weights to bfloat16.  Tokens in pages outside [0,
+ * pages) are left out; a query that sees none gives 0.  bad as above.  work:
+ * gn_kv_attention_workspace floats for the same sizes (may be 0: then work may
+ * be null). */
+int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max_len, int32_t heads, int32_t kv_heads,
+                              int32_t head_dim, int64_t *floats);
+int gn_kv_attention(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,
+                    int64_t out_stride, const int32_t *starts, const int32_t *lens, int32_t B, int32_t N,
+                    int32_t max_new, int32_t max_len, int32_t heads, float scale, int32_t causal, int32_t dtype,
+                    float *work, int32_t *bad);
+/* MultiHeadAttention (transformer.go:405-529) for new tokens of B sequences
+ * over such a cache: x and out are N rows of D floats, params as
+ * gn_mha_forward's; Q, K, V of the new tokens, rotated where cos and sin are
+ * given (gn_rope_tables), K and V appended, causal attention over the cache, wOut.
+ * kv->kv_heads x kv->head_dim must be D.  With all tokens at once and empty sequences it
+ * computes gn_mha_forward's causal layer, keys and values rounded to 8 bits. */
+int gn_mha_cached_workspace(int32_t B, int32_t N, int32_t max_new, int32_t max_len, int32_t D, int32_t heads,
+                            int64_t *floats);
+int gn_mha_cached_forward(gn_ctx *ctx, const gn_kv_cache *kv, const float *x, const float *params, float *out,
+                          const float *cos, const float *sin, int32_t rope_len, const int32_t *starts,
+                          const int32_t *lens, int32_t B, int32_t N, int32_t max_new, int32_t max_len, int32_t D,
+                          float *work, int32_t *bad);
+/* Draws one index of each of B rows of V logits (row stride in elements, dtype)
+ * with the given random number u[b] in [0, 1).  With m the row's largest logit,
+ * w_i = exp((z_i - m) / temperature[b]); NaN and -inf logits are left out.  Kept
+ * are the top_k[b] largest logits (<= 0: all), of those the shortest run in
+ * falling order whose weights reach top_p[b] of their sum (>= 1: all, <= 0: the
+ * first), of those the ones with w_i >= min_p[b]; the largest always stays, and
+ * equal logits go by the lowest index.  ids[b] is the first index, in rising
+ * order, at which the kept weights' running sum exceeds u[b] times their sum; -1
+ * for a row without a logit to choose.  A temperature that is not above 0 takes
+ * the largest logit.  All settings are device arrays of B; temperature (1),
+ * top_k, top_p and min_p may be null.  Weights are float64 exponentials rounded
+ * to whole multiples of 2^-43 and summed as integers, so a result does not
+ * depend on any order of sums.  V <= 2^20.  work: gn_sample_workspace floats,
+ * 8-byte aligned. */
+int gn_sample_workspace(int32_t B, int32_t V, int64_t *floats);
+int gn_sample(gn_ctx *ctx, const void *logits, int64_t stride, int32_t dtype, const float *temperature,
+              const int32_t *top_k, const float *top_p, const float *min_p, const float *u, int32_t *ids, int32_t B,
+              int32_t V, float *work);
 
 /* Generic fp32 GEMM: C[M,N] = alpha * op(A) op(B); trans flags as BLAS
  * (A is M x K row-major when transA == 0, K x M when 1; B is K x N when
