@@ -46,8 +46,16 @@ struct KvAttnArgs {
   int causal;
   float *work;
 };
+// how a call's work is split
+struct KvPlan {
+  int chunk, splits;  // keys of a split, splits of the longest sequence
+  int rt, rows_wg;    // 16-row tiles of a wave, rows of a workgroup
+  bool by_rows;       // the workgroup's waves take rows of their own (else keys)
+  int tiles;
+};
 int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd);
 hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, hipStream_t s);
+hipError_t launch_kv_attn_bf16(const KvAttnArgs &a, const KvPlan &p, hipStream_t s);
 
 struct SampleArgs {
   const void *z;

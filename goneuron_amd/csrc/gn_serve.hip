@@ -23,7 +23,7 @@ int cache_check(gn_ctx *c, const gn_kv_cache *kv, KvArgs &a) {
   if (kv->head_dim < 1 || kv->head_dim > KV_MAX_HEAD)
     return set_err(c, GN_ERR_UNSUPPORTED, "kv cache: head size %d is not 1 to %d", kv->head_dim, KV_MAX_HEAD);
   if (kv->pages < 1 || kv->kv_heads < 1 || kv->max_pages < 1 ||
-      (int64_t)kv->max_pages * kv->page_size > 0x7fffffff - 256)
+      (int64_t)kv->max_pages * kv->page_size > 0x7fffffff - 4096)
     return set_err(c, GN_ERR_INVALID, "kv cache: %d pages, %d heads, %d pages a sequence", kv->pages, kv->kv_heads,
                    kv->max_pages);
   if (((uintptr_t)kv->k | (uintptr_t)kv->v) & 15)
@@ -50,13 +50,13 @@ int batch_check(gn_ctx *c, KvArgs &a, const int32_t *starts, const int32_t *lens
   if (B < 0 || N < 0 || max_new < 0 || max_len < 0 || heads < 1 || heads % a.KVH)
     return set_err(c, GN_ERR_INVALID, "B %d, N %d, max_new %d, max_len %d, %d heads over %d", B, N, max_new, max_len,
                    heads, a.KVH);
-  if (B > 65535 || N > kMaxRows || heads > 65535)
-    return set_err(c, GN_ERR_UNSUPPORTED, "B %d, N %d or %d heads beyond the launch limits", B, N, heads);
+  if (B > 65535 || N > kMaxRows || heads > 65535 || (int64_t)B * max_new > kMaxRows)
+    return set_err(c, GN_ERR_UNSUPPORTED, "B %d, N %d, max_new %d or %d heads beyond the launch limits", B, N, max_new, heads);
   a.starts = starts;
   a.lens = lens;
   a.B = B;
   a.N = N;
-  a.max_new = std::min(max_new, N);
+  a.max_new = max_new;
   a.max_len = max_len;
   a.bad = bad;
   return GN_OK;
@@ -80,6 +80,7 @@ int append_impl(gn_ctx *c, const KvArgs &kv, const void *q, const void *k, const
                 int heads, int dtype) {
   KvAppendArgs a{};
   a.c = kv;
+  a.c.max_new = std::min(kv.max_new, kv.N);  // no sequence has more, whatever the bound
   a.q = q;
   a.x[0] = k;
   a.x[1] = v;
@@ -169,7 +170,7 @@ extern "C" int gn_kv_append(gn_ctx *c, const gn_kv_cache *kv, const void *q, con
   if (rc) return rc;
   if (!cos != !sin || (cos && rope_len < 0)) return set_err(c, GN_ERR_INVALID, "cos and sin come together");
   if (!q != !q_out) return set_err(c, GN_ERR_INVALID, "q and q_out come together");
-  if (B == 0 || a.max_new == 0) return GN_OK;
+  if (B == 0 || N == 0 || max_new == 0) return GN_OK;
   const int64_t kw = (int64_t)a.KVH * a.hd, qw = (int64_t)heads * a.hd;
   if ((rc = row_check(c, "k", k, k_stride, kw, dtype)) || (rc = row_check(c, "v", v, v_stride, kw, dtype))) return rc;
   if (q && ((rc = row_check(c, "q", q, q_stride, qw, dtype)) || (rc = row_check(c, "q_out", q_out, q_out_stride, qw, dtype))))
@@ -199,10 +200,10 @@ extern "C" int gn_kv_attention(gn_ctx *c, const gn_kv_cache *kv, const void *q, 
   rc = batch_check(c, a, starts, lens, B, N, max_new, max_len, heads, dtype, bad);
   if (rc) return rc;
   if (!isfinite(scale)) return set_err(c, GN_ERR_INVALID, "scale is not finite");
-  if (B == 0 || a.max_new == 0) return GN_OK;
+  if (B == 0 || N == 0 || max_new == 0) return GN_OK;
   const int64_t w = (int64_t)heads * a.hd;
   if ((rc = row_check(c, "q", q, q_stride, w, dtype)) || (rc = row_check(c, "out", out, out_stride, w, dtype))) return rc;
-  if (!work && kv_attn_work_floats(B, a.max_new, max_len, heads, a.KVH, a.hd) > 0)
+  if (!work && kv_attn_work_floats(B, max_new, max_len, heads, a.KVH, a.hd) > 0)
     return set_err(c, GN_ERR_INVALID, "kv_attention needs its workspace");
   return attn_impl(c, a, q, out, q_stride, out_stride, heads, scale, causal, dtype, work);
 }
@@ -218,7 +219,7 @@ extern "C" int gn_mha_cached_workspace(int32_t B, int32_t N, int32_t max_new, in
       D / heads > KV_MAX_HEAD)
     return GN_ERR_INVALID;
   *floats = 4 * (((int64_t)N * D + 63) / 64 * 64) +
-            kv_attn_work_floats(B, std::min(max_new, N), max_len, heads, heads, D / heads);
+            kv_attn_work_floats(B, max_new, max_len, heads, heads, D / heads);
   return GN_OK;
 }
 
@@ -234,7 +235,7 @@ extern "C" int gn_mha_cached_forward(gn_ctx *c, const gn_kv_cache *kv, const flo
   if (rc) return rc;
   if ((int64_t)a.KVH * a.hd != D) return set_err(c, GN_ERR_SHAPE, "%d heads of %d are not D = %d", a.KVH, a.hd, D);
   if (!cos != !sin || (cos && rope_len < 0)) return set_err(c, GN_ERR_INVALID, "cos and sin come together");
-  if (B == 0 || a.max_new == 0) return GN_OK;
+  if (B == 0 || N == 0 || max_new == 0) return GN_OK;
   if (!x || !params || !out || !work) return set_err(c, GN_ERR_INVALID, "null pointer");
   const int64_t nd = (int64_t)D * D + D, rows = ((int64_t)N * D + 63) / 64 * 64;
   float *qkv = work, *o = work + 3 * rows;

@@ -1,71 +1,14 @@
-// The paged 8-bit cache of rotated keys and values: appending to it and
-// attention over it.
+// The paged 8-bit cache of rotated keys and values: appending to it.
 //
 // Layout: K pages [page][kv head][token][R], V pages [page][kv head][R][token]
 // in E4M3 with a power-of-two scale per (page, kv head) for each.  V lies
 // transposed so that attention's two products read both caches as their matrix
 // operands lie in registers, 16 bytes a lane, with no pass through LDS; the
 // writer owns a whole block anyway (its scale covers the block).
-#include "gn_serve.h"
+#include "gn_kv.h"
 
 namespace gn {
 namespace {
-
-__device__ __forceinline__ float bf16_f32(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
-// round to nearest even; NaN stays NaN
-__device__ __forceinline__ uint16_t f32_bf16(float f) {
-  const uint32_t u = __float_as_uint(f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
-}
-template <typename T>
-struct Elem;
-template <>
-struct Elem<float> {
-  static __device__ __forceinline__ float get(const float *p) { return *p; }
-  static __device__ __forceinline__ void put(float *p, float v) { *p = v; }
-  static __device__ __forceinline__ void get4(const float *p, float (&v)[4]) {
-    const float4 x = *reinterpret_cast<const float4 *>(p);
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-  }
-  static __device__ __forceinline__ void put4(float *p, const float (&v)[4]) {
-    *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  }
-};
-template <>
-struct Elem<uint16_t> {
-  static __device__ __forceinline__ float get(const uint16_t *p) { return bf16_f32(*p); }
-  static __device__ __forceinline__ void put(uint16_t *p, float v) { *p = f32_bf16(v); }
-  static __device__ __forceinline__ void get4(const uint16_t *p, float (&v)[4]) {
-    const uint2 x = *reinterpret_cast<const uint2 *>(p);
-    v[0] = bf16_f32((uint16_t)x.x); v[1] = bf16_f32((uint16_t)(x.x >> 16));
-    v[2] = bf16_f32((uint16_t)x.y); v[3] = bf16_f32((uint16_t)(x.y >> 16));
-  }
-  static __device__ __forceinline__ void put4(uint16_t *p, const float (&v)[4]) {
-    uint2 x;
-    x.x = f32_bf16(v[0]) | ((uint32_t)f32_bf16(v[1]) << 16);
-    x.y = f32_bf16(v[2]) | ((uint32_t)f32_bf16(v[3]) << 16);
-    *reinterpret_cast<uint2 *>(p) = x;
-  }
-};
-
-// A sequence as the call's arrays describe it; n = 0 where there is nothing to
-// do.  bad: its bounds lie outside the inputs or the table, or it is larger
-// than the sizes the launch was made for.
-struct Seq {
-  int start, n, len;
-  bool bad;
-};
-__device__ __forceinline__ Seq kv_seq(const KvArgs &c, int b, int limit) {
-  Seq s;
-  s.start = c.starts[b];
-  const int end = c.starts[b + 1];
-  s.len = c.lens[b];
-  s.bad = s.start < 0 || end < s.start || end > c.N || end - s.start > c.max_new || s.len < 0 ||
-          (int64_t)s.len + (end - s.start) > limit;
-  s.n = s.bad ? 0 : end - s.start;
-  return s;
-}
 
 // ---------------------------------------------------------------- append
 // x * 2^-e rounded to E4M3 (|x| <= 448 2^e by the choice of e); what is not
@@ -302,70 +245,6 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   }
 }
 
-// ---------------------------------------------------------------- attention
-// One wave per (row, query head): 64 keys at a time, a lane each, and the
-// weights against V with a lane per column.
-template <typename T>
-__global__ __launch_bounds__(64) void kv_attn_kernel(KvAttnArgs a) {
-  __shared__ float qs[KV_MAX_HEAD];
-  __shared__ float ps[64];
-  const KvArgs &c = a.c;
-  const int lane = threadIdx.x, h = blockIdx.y, b = blockIdx.z, t = blockIdx.x;
-  const Seq s = kv_seq(c, b, min(c.max_len, c.max_pages * c.P));
-  if (s.bad && c.bad && lane == 0) c.bad[b] = 1;
-  if (t >= s.n) return;
-  const int kvh = h / a.G, len = a.causal ? s.len + t + 1 : s.len + s.n;
-  const T *q = (const T *)a.q + (int64_t)(s.start + t) * a.qs + (int64_t)h * c.hd;
-  for (int d = lane; d < c.hd; d += 64) qs[d] = Elem<T>::get(q + d);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  bool any = false;
-  for (int j0 = 0; j0 < len; j0 += 64) {
-    const int j = j0 + lane;
-    int page = -1;
-    if (j < len) page = c.table[(int64_t)b * c.max_pages + (j >> c.lgP)];
-    const bool on = j < len && page >= 0 && page < c.pages;
-    if (j < len && !on && c.bad) c.bad[b] = 1;
-    const int64_t blk = on ? (int64_t)page * c.KVH + kvh : 0;
-    float x = -INFINITY;
-    if (on) {
-      const uint8_t *k = c.k + (blk * c.P + (j & (c.P - 1))) * c.R;
-      x = 0.f;
-      for (int d = 0; d < c.hd; ++d) x += qs[d] * __builtin_amdgcn_cvt_f32_fp8((int)k[d], 0);
-      x *= c.ks[blk] * a.scale;
-    }
-    float mm = x;
-    for (int off = 32; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor(mm, off, 64));
-    any = any || __any(on);
-    const float mn = fmaxf(m, mm), safe = mn == -INFINITY ? 0.f : mn;
-    const float f = __expf(m - safe), p = on ? __expf(x - safe) : 0.f;
-    float sum = p;
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    l = l * f + sum;
-    m = mn;
-    __syncthreads();
-    ps[lane] = on ? p * c.vs[blk] : 0.f;
-    __syncthreads();
-    for (int u = 0; u < 4; ++u) o[u] *= f;
-    for (int jj = 0; jj < 64; ++jj) {
-      const int on2 = __shfl((int)on, jj, 64);
-      if (!on2) continue;
-      const int64_t blk2 = __shfl(page, jj, 64) * (int64_t)c.KVH + kvh;
-      const uint8_t *v = c.v + blk2 * c.P * c.R + ((j0 + jj) & (c.P - 1));
-      const float w = ps[jj];
-      for (int u = 0; u < 4; ++u) {
-        const int d = lane + 64 * u;
-        if (d < c.hd) o[u] += w * __builtin_amdgcn_cvt_f32_fp8((int)v[(int64_t)d * c.P], 0);
-      }
-    }
-  }
-  T *out = (T *)a.out + (int64_t)(s.start + t) * a.os + (int64_t)h * c.hd;
-  for (int u = 0; u < 4; ++u) {
-    const int d = lane + 64 * u;
-    if (d < c.hd) Elem<T>::put(out + d, any ? o[u] / l : 0.f);
-  }
-}
-
 }  // namespace
 
 hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
@@ -387,17 +266,6 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
     hipLaunchKernelGGL(kv_append_kernel<float>, dim3((unsigned)blocks), dim3(nt), sh, s, a);
   else
     hipLaunchKernelGGL(kv_append_kernel<uint16_t>, dim3((unsigned)blocks), dim3(nt), sh, s, a);
-  return hipGetLastError();
-}
-
-int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd) { return 0; }
-
-hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, hipStream_t s) {
-  const dim3 grid(a.c.max_new, a.H, a.c.B);
-  if (dtype == GN_DTYPE_F32)
-    hipLaunchKernelGGL(kv_attn_kernel<float>, grid, dim3(64), 0, s, a);
-  else
-    hipLaunchKernelGGL(kv_attn_kernel<uint16_t>, grid, dim3(64), 0, s, a);
   return hipGetLastError();
 }
 

@@ -1,0 +1,37 @@
+// Attention over the paged 8-bit cache: the split of the work, and the kernels for
+// float32 queries.
+#include "k_kv_attn.h"
+
+namespace gn {
+
+static KvPlan kv_plan(int B, int max_new, int max_len, int H, int KVH, int R) {
+  KvPlan p{};
+  const int64_t rows = (int64_t)max_new * (H / KVH);
+  p.rt = rows <= 16 ? 1 : 2;
+  p.by_rows = rows > 64;
+  p.rows_wg = 16 * p.rt * (p.by_rows ? 4 : 1);
+  p.tiles = (int)((rows + p.rows_wg - 1) / p.rows_wg);
+  // splits of the keys until some 1024 workgroups have work, 512 keys at least
+  const int64_t items = (int64_t)B * KVH * p.tiles;
+  int64_t chunk = (items * max_len / 1024 + 255) / 256 * 256;
+  chunk = chunk < 512 ? 512 : chunk;
+  if (items >= 1024 || chunk >= max_len) chunk = ((int64_t)max_len + 255) / 256 * 256;
+  p.chunk = (int)(chunk < 256 ? 256 : chunk);
+  p.splits = max_len > p.chunk ? (max_len + p.chunk - 1) / p.chunk : 1;
+  return p;
+}
+
+int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd) {
+  if (B == 0 || max_new == 0 || max_len == 0) return 0;
+  const int R = kv_row(hd);
+  const KvPlan p = kv_plan(B, max_new, max_len, H, KVH, R);
+  return p.splits == 1 ? 0 : (int64_t)p.splits * B * max_new * H * (R + 2);
+}
+
+hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, hipStream_t s) {
+  const KvArgs &c = a.c;
+  const KvPlan p = kv_plan(c.B, c.max_new, c.max_len, a.H, c.KVH, c.R);
+  return dtype == GN_DTYPE_F32 ? kv_attn_typed<float>(a, p, s) : launch_kv_attn_bf16(a, p, s);
+}
+
+}  // namespace gn
