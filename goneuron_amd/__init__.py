@@ -519,6 +519,32 @@ class Sequential:
         """Sequential.Predict (sequential.go:118-122): inference mode."""
         return self.PredictBatch(_f32(x).reshape(1, -1))[0]
 
+    def Sample(self, x, u, temperature=None, top_k=None, top_p=None, min_p=None):
+        """A prediction of every row of x and a draw from its outputs as logits
+        (gn_model_sample; no counterpart in the reference): int32 indices.  u:
+        a random number in [0, 1) for each row; each setting a number for all
+        rows or one for each."""
+        x = _f32(x)
+        B = x.shape[0]
+        if B == 0:
+            return np.empty(0, np.int32)
+        self._reserve(B)
+        if u is None:
+            raise GNError(-1, "Sample needs a random number for each row")
+
+        def rows(a, t, ptr):
+            if a is None:
+                return None, None
+            a = np.ascontiguousarray(np.broadcast_to(np.asarray(a, t), (B,)))
+            return a, a.ctypes.data_as(ptr)
+
+        (t, tp), (k, kp), (p, pp), (m, mp), (r, rp) = (
+            rows(temperature, np.float32, _lib.f32p), rows(top_k, np.int32, _lib.i32p), rows(top_p, np.float32, _lib.f32p),
+            rows(min_p, np.float32, _lib.f32p), rows(u, np.float32, _lib.f32p))
+        ids = np.empty(B, np.int32)
+        self._ck(lib().gn_model_sample(self.h, _fp(x), B, tp, kp, pp, mp, rp, ids.ctypes.data_as(_lib.i32p)))
+        return ids
+
     # flat arena views (net.go:787-846)
     def Params(self):
         out = np.empty(self.nparams, np.float32)

@@ -173,7 +173,7 @@ SIGNATURES = {
                               + [vp, vp]),
     "gn_sample_workspace": (C.c_int, [C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
     "gn_sample": (C.c_int, [vp, vp, C.c_int64, C.c_int32] + [vp] * 6 + [C.c_int32, C.c_int32, vp]),
-    "gn_model_sample": (C.c_int, [vp, vp, C.c_int32] + [vp] * 6),
+    "gn_model_sample": (C.c_int, [vp, f32p, C.c_int32, f32p, i32p, f32p, f32p, f32p, i32p]),
     "gn_gemm": (C.c_int, [vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_float, vp,
                           C.c_int32, vp, C.c_int32, vp, C.c_int32]),
     "gn_adam_step": (C.c_int, [vp, vp, vp, vp, vp, C.c_int64, C.c_float, C.c_float, C.c_float,

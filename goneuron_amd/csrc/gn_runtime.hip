@@ -3280,8 +3280,9 @@ extern "C" int gn_model_predict_device(gn_model *M, const float *x, int32_t B, f
   return GN_OK;
 }
 
-// One prediction and a draw from every sample's outputs, in the context's scratch
-// (as many rows at a time as it holds).
+// One prediction and a draw from every sample's outputs.  Settings, indices and the
+// draw's workspace lie in the context's scratch (as many rows at a time as it
+// holds), which the forward pass is done with by then.
 extern "C" int gn_model_sample(gn_model *M, const float *x, int32_t B, const float *temperature,
                                const int32_t *top_k, const float *top_p, const float *min_p, const float *u,
                                int32_t *ids) {
@@ -3290,37 +3291,48 @@ extern "C" int gn_model_sample(gn_model *M, const float *x, int32_t B, const flo
   ENTRY(c);
   if (B <= 0 || B > M->maxB || !x || !u || !ids) return set_err(c, GN_ERR_INVALID, "bad sample args");
   LayerRT &O = M->L.back();
+  const int V = O.out_len;
   if (O.d.kind == GN_LAYER_DENSE && O.d.act == GN_ACT_SOFTMAX && O.d.act_is_ptr)
     return set_err(c, GN_ERR_UNSUPPORTED, "sample: the last layer gives probabilities, not logits");
-  if (O.out_len > SAMPLE_MAX_V)
-    return set_err(c, GN_ERR_UNSUPPORTED, "sample: %lld outputs, more than %d", (long long)O.out_len, SAMPLE_MAX_V);
+  if (V > SAMPLE_MAX_V)
+    return set_err(c, GN_ERR_UNSUPPORTED, "sample: %d outputs, more than %d", V, SAMPLE_MAX_V);
+  const size_t part = ((size_t)B + 63) / 64 * 64, used = 6 * part;
+  int rows = std::min(B, 65535);
+  while (rows > 1 && used + sample_work_floats(rows, V) > c->scratch_floats) rows = (rows + 1) / 2;
+  if (used + sample_work_floats(rows, V) > c->scratch_floats)
+    return set_err(c, GN_ERR_UNSUPPORTED, "sample: %d rows of %d exceed the scratch", B, V);
   for (LayerRT &R : M->L) R.train = 0;
   int rc = pass_flags(M, B, false);
   if (rc) return rc;
+  HIP_OK(c, hipMemcpyAsync(M->xin, x, (size_t)B * M->L[0].in_len * sizeof(float), hipMemcpyHostToDevice, c->stream));
   M->last_predict = true;
-  rc = model_forward(M, x, B, false);
+  rc = model_forward(M, M->xin, B, false);
   if (rc) return rc;
   M->last_B = B;
-  const int V = (int)O.out_len;
-  int rows = std::min(B, 65535);
-  while (rows > 1 && sample_work_floats(rows, V) > (int64_t)c->scratch_floats) rows = (rows + 1) / 2;
+  const void *host[5] = {temperature, top_k, top_p, min_p, u};
+  for (int i = 0; i < 5; ++i)
+    if (host[i])
+      HIP_OK(c, hipMemcpyAsync(c->scratch + i * part, host[i], (size_t)B * 4, hipMemcpyHostToDevice, c->stream));
+  int32_t *out = reinterpret_cast<int32_t *>(c->scratch + 5 * part);
   for (int b = 0; b < B; b += rows) {
     SampleArgs a{};
     a.z = O.out + (int64_t)b * V;
     a.stride = V;
-    a.temperature = temperature ? temperature + b : nullptr;
-    a.top_k = top_k ? top_k + b : nullptr;
-    a.top_p = top_p ? top_p + b : nullptr;
-    a.min_p = min_p ? min_p + b : nullptr;
-    a.u = u + b;
-    a.ids = ids + b;
+    a.temperature = temperature ? c->scratch + b : nullptr;
+    a.top_k = top_k ? reinterpret_cast<const int32_t *>(c->scratch + part) + b : nullptr;
+    a.top_p = top_p ? c->scratch + 2 * part + b : nullptr;
+    a.min_p = min_p ? c->scratch + 3 * part + b : nullptr;
+    a.u = c->scratch + 4 * part + b;
+    a.ids = out + b;
     a.B = std::min(rows, B - b);
     a.V = V;
-    a.work = c->scratch;
+    a.work = c->scratch + used;
     KTimer kt(c, GN_KCLASS_OTHER, "sample", f4((double)a.B * V));
     HIP_OK(c, launch_sample(a, GN_DTYPE_F32, c->stream));
   }
-  return GN_OK;
+  HIP_OK(c, hipMemcpyAsync(ids, out, (size_t)B * sizeof(int32_t), hipMemcpyDeviceToHost, c->stream));
+  HIP_OK(c, hipStreamSynchronize(c->stream));
+  return check_flags(M);
 }
 
 extern "C" int gn_model_layer_output(gn_model *M, int32_t layer, float *dst, int64_t n) {

@@ -237,11 +237,11 @@ int gn_model_predict(gn_model *m, const float *x, int32_t B, float *out);
 /* The same with HBM-resident x (B x in_size) and output (B x out_size); no
  * host synchronisation (the device-side ForwardBatch of sequential.go:145-160). */
 int gn_model_predict_device(gn_model *m, const float *x_dev, int32_t B, float *out_dev);
-/* gn_model_predict_device and a draw from each sample's outputs as logits (gn_sample's settings;
- * device pointers, ids: B int32).  No counterpart in the reference.  The last
- * layer must give logits or log-probabilities: a Dense Softmax pointer is
- * GN_ERR_UNSUPPORTED. */
-int gn_model_sample(gn_model *m, const float *x_dev, int32_t B, const float *temperature, const int32_t *top_k,
+/* gn_model_predict and a draw from each sample's outputs as logits, with
+ * gn_sample's settings as host arrays of B (each but u may be NULL); ids: B
+ * indices.  No counterpart in the reference.  The last layer must give logits or
+ * log-probabilities: a Dense Softmax pointer is GN_ERR_UNSUPPORTED. */
+int gn_model_sample(gn_model *m, const float *x, int32_t B, const float *temperature, const int32_t *top_k,
                     const float *top_p, const float *min_p, const float *u, int32_t *ids);
 /* Network.SetTraining (net.go:187-193): sets the flag of every layer.  Layers
  * start as the reference constructs them (Dropout and BatchNorm2D in training
@@ -527,11 +527,10 @@ int gn_moe_backward(gn_ctx *ctx, const float *x, const float *params, const floa
  * No counterpart in the reference, whose Predict runs the whole window for
  * every token.  A paged cache of rotated keys and values in 8 bits, the
  * attention that reads it, and the draw of the next token.  Device pointers;
- * calls queue work on the context's stream, allocate nothing, do not
- * synchronise (but gn_rope_tables) and can be captured into a graph, which
- * then reads starts, lens, the page table and every row's settings anew at
- * each replay.  Calls that may run at the same time (two contexts, two graphs)
- * need a `work` each.
+ * calls queue work on the context's stream, allocate nothing and do not
+ * synchronise (but gn_rope_tables); what lies in device memory (starts, lens,
+ * the page table, settings) is read when the work runs.  Calls that may run at
+ * the same time (two contexts) need a `work` each.
  *
  * Tokens are packed: sequence b's new tokens are the rows starts[b] ..
  * starts[b + 1] - 1 (starts: B + 1 int32) of the inputs and outputs, at the
