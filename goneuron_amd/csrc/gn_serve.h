@@ -44,6 +44,7 @@ struct KvAttnArgs {
   int H, G;  // query heads, query heads a key head
   float scale;
   int causal;
+  int vec;  // queries and outputs allow 4-value accesses, heads are whole eights
   float *work;
 };
 // how a call's work is split
@@ -53,6 +54,10 @@ struct KvPlan {
   bool by_rows;       // the workgroup's waves take rows of their own (else keys)
   int tiles;
 };
+// padded heads up to this size leave registers for two 16-row tiles a wave
+constexpr int kv_two_tiles(int bytes) { return bytes == 4 ? 64 : 128; }
+// the workspace: (maximum, sum) of every split's rows, then their outputs
+__host__ __device__ inline int64_t kv_part_at(int splits, int64_t slots) { return (splits * slots * 2 + 3) / 4 * 4; }
 int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd);
 hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, hipStream_t s);
 hipError_t launch_kv_attn_bf16(const KvAttnArgs &a, const KvPlan &p, hipStream_t s);

@@ -114,6 +114,7 @@ int attn_impl(gn_ctx *c, const KvArgs &kv, const void *q, void *out, int64_t qs,
   a.G = heads / kv.KVH;
   a.scale = scale;
   a.causal = causal != 0;
+  a.vec = kv.hd % 8 == 0 && aligned4(q, qs, dtype) && aligned4(out, os, dtype);
   a.work = work;
   // the cache's lengths are on the device: the bound stands for them
   KTimer kt(c, GN_KCLASS_OTHER, "kv_attention", 2.0 * kv.B * kv.max_len * (double)kv.KVH * kv.hd);
@@ -205,6 +206,7 @@ extern "C" int gn_kv_attention(gn_ctx *c, const gn_kv_cache *kv, const void *q, 
   if ((rc = row_check(c, "q", q, q_stride, w, dtype)) || (rc = row_check(c, "out", out, out_stride, w, dtype))) return rc;
   if (!work && kv_attn_work_floats(B, max_new, max_len, heads, a.KVH, a.hd) > 0)
     return set_err(c, GN_ERR_INVALID, "kv_attention needs its workspace");
+  if ((uintptr_t)work & 15) return set_err(c, GN_ERR_INVALID, "kv_attention: work must be 16-byte aligned");
   return attn_impl(c, a, q, out, q_stride, out_stride, heads, scale, causal, dtype, work);
 }
 
@@ -237,6 +239,7 @@ extern "C" int gn_mha_cached_forward(gn_ctx *c, const gn_kv_cache *kv, const flo
   if (!cos != !sin || (cos && rope_len < 0)) return set_err(c, GN_ERR_INVALID, "cos and sin come together");
   if (B == 0 || N == 0 || max_new == 0) return GN_OK;
   if (!x || !params || !out || !work) return set_err(c, GN_ERR_INVALID, "null pointer");
+  if ((uintptr_t)work & 15) return set_err(c, GN_ERR_INVALID, "mha_cached: work must be 16-byte aligned");
   const int64_t nd = (int64_t)D * D + D, rows = ((int64_t)N * D + 63) / 64 * 64;
   float *qkv = work, *o = work + 3 * rows;
   {

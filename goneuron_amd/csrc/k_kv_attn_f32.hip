@@ -1,14 +1,16 @@
 // Attention over the paged 8-bit cache: the split of the work, and the kernels for
 // float32 queries.
+#include <algorithm>
+
 #include "k_kv_attn.h"
 
 namespace gn {
 
-static KvPlan kv_plan(int B, int max_new, int max_len, int H, int KVH, int R) {
+static KvPlan kv_plan(int B, int max_new, int max_len, int H, int KVH, int R, int bytes) {
   KvPlan p{};
   const int64_t rows = (int64_t)max_new * (H / KVH);
-  p.rt = rows <= 16 ? 1 : 2;
-  p.by_rows = rows > 64;
+  p.by_rows = rows > 16;
+  p.rt = rows > 64 && R <= kv_two_tiles(bytes) ? 2 : 1;
   p.rows_wg = 16 * p.rt * (p.by_rows ? 4 : 1);
   p.tiles = (int)((rows + p.rows_wg - 1) / p.rows_wg);
   // splits of the keys until some 1024 workgroups have work, 512 keys at least
@@ -24,13 +26,18 @@ static KvPlan kv_plan(int B, int max_new, int max_len, int H, int KVH, int R) {
 int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd) {
   if (B == 0 || max_new == 0 || max_len == 0) return 0;
   const int R = kv_row(hd);
-  const KvPlan p = kv_plan(B, max_new, max_len, H, KVH, R);
-  return p.splits == 1 ? 0 : (int64_t)p.splits * B * max_new * H * (R + 2);
+  const int64_t slots = (int64_t)B * max_new * H;
+  int64_t most = 0;
+  for (int bytes = 2; bytes <= 4; bytes += 2) {  // whichever type the queries have
+    const KvPlan p = kv_plan(B, max_new, max_len, H, KVH, R, bytes);
+    if (p.splits > 1) most = std::max(most, kv_part_at(p.splits, slots) + p.splits * slots * R);
+  }
+  return most;
 }
 
 hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, hipStream_t s) {
   const KvArgs &c = a.c;
-  const KvPlan p = kv_plan(c.B, c.max_new, c.max_len, a.H, c.KVH, c.R);
+  const KvPlan p = kv_plan(c.B, c.max_new, c.max_len, a.H, c.KVH, c.R, dtype == GN_DTYPE_F32 ? 4 : 2);
   return dtype == GN_DTYPE_F32 ? kv_attn_typed<float>(a, p, s) : launch_kv_attn_bf16(a, p, s);
 }
 

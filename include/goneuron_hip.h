@@ -597,8 +597,8 @@ int gn_kv_append(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, const void *
  * maxima are float32; the products of float32 queries have float32's precision,
  * bfloat16 ones round the weights to bfloat16.  Tokens in pages outside [0,
  * pages) are left out; a query that sees none gives 0.  bad as above.  work:
- * gn_kv_attention_workspace floats for the same sizes (may be 0: then work may
- * be null). */
+ * gn_kv_attention_workspace floats for the same sizes, 16-byte aligned (may be
+ * 0: then work may be null). */
 int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max_len, int32_t heads, int32_t kv_heads,
                               int32_t head_dim, int64_t *floats);
 int gn_kv_attention(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,
