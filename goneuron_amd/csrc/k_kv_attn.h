@@ -685,16 +685,17 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
   if (w == 0) A.store(a, pl, x, x.row0, n, g);
 }
 
-// Joins a row's splits: a workgroup per (row, head), its waves every 16th split
-// with a few loads in flight each (one wave alone waits for a load per split: 150
-// us at 128 splits, 6 us this way).
-template <typename T>
-__global__ __launch_bounds__(1024) void kv_join_kernel(KvAttnArgs a, KvPlan pl) {
+// Joins a row's splits.  WAVES waves per (row, head): 1 where the rows fill the card, 4
+// where few rows have few splits (2048 rows of 8: 7 us, 12 with one), 16 where they
+// have many (32 rows of 64: 8 us; one wave alone waits for a load per split, 150 us
+// at 128).
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void kv_join_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int U = KV_MAX_HEAD / 64;
-  __shared__ float sl[16], so[16][KV_MAX_HEAD];
   const KvArgs &c = a.c;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  const int64_t slots = (int64_t)c.B * c.max_new * a.H, slot = blockIdx.x;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t slots = (int64_t)c.B * c.max_new * a.H, slot = WAVES == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x;
+  if (slot >= slots) return;
   const int h = (int)(slot % a.H), t = (int)(slot / a.H % c.max_new), b = (int)(slot / a.H / c.max_new);
   const Seq s = kv_seq(c, b, min(c.max_len, c.max_pages * c.P));
   if (t >= s.n) return;
@@ -718,7 +719,7 @@ __global__ __launch_bounds__(1024) void kv_join_kernel(KvAttnArgs a, KvPlan pl) 
   const float *part = a.work + kv_part_at(pl.splits, slots) + slot * c.R;
   float acc[U] = {}, l = 0.f;
 #pragma unroll 4
-  for (int i = w; i < n; i += nw) {
+  for (int i = WAVES == 1 ? 0 : w; i < n; i += WAVES) {
     const float2 v = *reinterpret_cast<const float2 *>(ml + i * slots * 2);
     const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - M);
     l += v.x == -INFINITY ? 0.f : v.y * f;
@@ -726,18 +727,27 @@ __global__ __launch_bounds__(1024) void kv_join_kernel(KvAttnArgs a, KvPlan pl) 
     for (int u = 0; u < U; ++u)
       if (lane + 64 * u < c.hd) acc[u] += part[i * slots * c.R + lane + 64 * u] * f;
   }
-#pragma unroll
-  for (int u = 0; u < U; ++u) so[w][lane + 64 * u] = acc[u];
-  if (lane == 0) sl[w] = l;
-  __syncthreads();
   T *out = (T *)a.out + (int64_t)(s.start + t) * a.os + (int64_t)h * c.hd;
-  for (int d = threadIdx.x; d < c.hd; d += blockDim.x) {
-    float o = 0.f, sum = 0.f;
-    for (int i = 0; i < nw; ++i) {
-      o += so[i][d];
-      sum += sl[i];
+  const float nothing = none ? __uint_as_float(0x7fc00000u) : 0.f;
+  if constexpr (WAVES == 1) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (lane + 64 * u < c.hd) Elem<T>::put(out + lane + 64 * u, M != -INFINITY ? acc[u] / l : nothing);
+  } else {
+    __shared__ float sl[WAVES], so[WAVES][KV_MAX_HEAD];
+#pragma unroll
+    for (int u = 0; u < U; ++u) so[w][lane + 64 * u] = acc[u];
+    if (lane == 0) sl[w] = l;
+    __syncthreads();
+    for (int d = threadIdx.x; d < c.hd; d += 64 * WAVES) {
+      float o = 0.f, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) {
+        o += so[i][d];
+        sum += sl[i];
+      }
+      Elem<T>::put(out + d, M != -INFINITY ? o / sum : nothing);
     }
-    Elem<T>::put(out + d, M != -INFINITY ? o / sum : none ? __uint_as_float(0x7fc00000u) : 0.f);
   }
 }
 
@@ -776,8 +786,12 @@ hipError_t kv_attn_typed(const KvAttnArgs &a, const KvPlan &p, hipStream_t s) {
   }
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t slots = (int64_t)c.B * c.max_new * a.H;
-  const int waves = p.splits >= 32 ? 16 : 4;  // a few splits a wave
-  hipLaunchKernelGGL(kv_join_kernel<T>, dim3((unsigned)slots), dim3(64 * waves), 0, s, a, p);
+  if (slots >= 16384)
+    hipLaunchKernelGGL((kv_join_kernel<T, 1>), dim3((unsigned)((slots + 3) / 4)), dim3(256), 0, s, a, p);
+  else if (p.splits <= 16)
+    hipLaunchKernelGGL((kv_join_kernel<T, 4>), dim3((unsigned)slots), dim3(256), 0, s, a, p);
+  else
+    hipLaunchKernelGGL((kv_join_kernel<T, 16>), dim3((unsigned)slots), dim3(1024), 0, s, a, p);
   return hipGetLastError();
 }
 

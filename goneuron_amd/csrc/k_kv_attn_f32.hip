@@ -13,13 +13,17 @@ static KvPlan kv_plan(int B, int max_new, int max_len, int H, int KVH, int R, in
   p.rt = rows > 64 && R <= kv_two_tiles(bytes) ? 2 : 1;
   p.rows_wg = 16 * p.rt * (p.by_rows ? 4 : 1);
   p.tiles = (int)((rows + p.rows_wg - 1) / p.rows_wg);
-  // splits of the keys until some 1024 workgroups have work, 512 keys at least
-  const int64_t items = (int64_t)B * KVH * p.tiles;
-  int64_t chunk = (items * max_len / 1024 + 255) / 256 * 256;
-  chunk = chunk < 512 ? 512 : chunk;
-  if (items >= 1024 || chunk >= max_len) chunk = ((int64_t)max_len + 255) / 256 * 256;
-  p.chunk = (int)(chunk < 256 ? 256 : chunk);
-  p.splits = max_len > p.chunk ? (max_len + p.chunk - 1) / p.chunk : 1;
+  // Keys are split until every CU has work to change over to.  Single tokens: 4096
+  // workgroups (eight rounds of two a CU, for sequences of unlike length), 64 splits
+  // at most (the join reads them all).  Prompts: 512 workgroups, 128 keys a split at
+  // least.
+  const int64_t items = (int64_t)B * KVH * p.tiles, unit = p.by_rows ? 64 : 256;
+  int64_t splits = p.by_rows ? 512 / items : std::min<int64_t>(4096 / items, 64);
+  splits = std::min(splits, max_len / (p.by_rows ? 128 : 512) + 0l);
+  splits = std::max<int64_t>(splits, 1);
+  const int64_t chunk = (std::max(max_len, 1) + splits - 1) / splits;
+  p.chunk = (int)((chunk + unit - 1) / unit * unit);
+  p.splits = (std::max(max_len, 1) + p.chunk - 1) / p.chunk;
   return p;
 }
 

@@ -6,11 +6,13 @@
 // over atomics and over prefixes are then the same number whatever their order,
 // and a comparison with a border (top-p's share, the draw) can be made anywhere.
 //
-// Rows are cut into chunks, a workgroup each.  The logits are read by four passes
-// (maximum, histogram, candidates, kept weights), all but the first out of cache:
-// the histogram's 1024 bins of 1/32 in the exponent fix the bins in which top-k and
-// top-p cut, only their elements are then selected among exactly, by
-// radix over (logit, falling index), so that equal logits go by the lowest index.
+// A histogram of 1024 bins of 1/32 in the exponent fixes the bins in which top-k
+// and top-p cut; only their elements are then ranked exactly, by (logit, falling
+// index), so that equal logits go by the lowest index.  A row of up to 16384 logits
+// is one workgroup's, its logits in LDS from the first pass to the draw.  Longer
+// rows are cut into chunks, a workgroup each, and read by three passes (maximum,
+// histogram, candidates) and, where too many logits are kept to go into the list of
+// candidates, a fourth, all but the first out of cache.
 #include "gn_serve.h"
 
 namespace gn {
@@ -19,8 +21,31 @@ namespace {
 constexpr int SM_BINS = 1024;
 constexpr int SM_PER = 32;        // bins per unit of the exponent
 constexpr int SM_CAP = 4096;      // candidates of a row kept in a list
+constexpr int SM_RANK = 256;      // candidates ranked against each other; more: radix
 constexpr int SM_MASS_BITS = 43;
-constexpr int SM_MAX_CHUNKS = 256;
+constexpr int SM_WAVE = 1024;     // logits of a wave, 16 a lane
+constexpr int SM_ONE = 16384;     // rows up to this size: one workgroup
+
+// 2^43 exp(-b / 32), from exp(-1/32) and its powers by their series
+struct ExpTable {
+  double v[SM_BINS];
+  static constexpr double series(double x) {  // exp(x), |x| <= 1
+    double term = 1.0, sum = 1.0;
+    for (int i = 1; i < 30; ++i) {
+      term *= x / i;
+      sum += term;
+    }
+    return sum;
+  }
+  constexpr ExpTable() : v() {
+    double whole = 8796093022208.0;  // 2^43 exp(-(b / 32))
+    for (int b = 0; b < SM_BINS; ++b) {
+      if (b && b % SM_PER == 0) whole *= series(-1.0);
+      v[b] = whole * series(-(double)(b % SM_PER) / SM_PER);
+    }
+  }
+};
+__device__ const ExpTable exp_table = ExpTable();
 
 struct RowState {
   uint64_t tau;        // kept: elements whose key is at least this
@@ -30,42 +55,41 @@ struct RowState {
   uint32_t r;          // rank of the last kept element inside kbin
   uint32_t nlist;      // candidates found (the list holds the first SM_CAP)
   int32_t kbin, plo, phi;  // -1: top-k / top-p does not cut
+  int32_t last;            // the list holds all of bins 0 .. last (-1: the cuts' bins)
+  int32_t done;            // the draw is made
   int32_t pad;
 };
 
 struct SampleWs {
-  uint64_t *mass, *csum, *list;
+  uint64_t *mass, *wsum, *list;
   RowState *st;
   uint32_t *count;
   float *cmax;
-  int chunk, C;
+  int C, waves;  // chunks of a row, waves of a chunk
 };
 
-__host__ __device__ inline size_t up64(size_t n) { return (n + 63) / 64 * 64; }
+inline size_t up64(size_t n) { return (n + 63) / 64 * 64; }
 
-// the cut of a row into chunks: enough workgroups to fill the card, chunks long
-// enough that the histogram's flush (1024 bins) stays small beside them
-inline int sample_chunk(int B, int V) {
-  int chunk = 4096;
-  while (chunk < 16384 && (int64_t)B * ((V + chunk - 1) / chunk) > 2048) chunk *= 2;
-  return chunk;
-}
 size_t sample_carve(char *base, int B, int V, SampleWs *w) {
   SampleWs t{};
-  t.chunk = sample_chunk(B, V);
-  t.C = (V + t.chunk - 1) / t.chunk;
+  // chunks of 4096, or of 16384 where those fill the card: a quarter of the
+  // histograms to join and to search
+  t.waves = (int64_t)B * ((V + 4 * SM_WAVE - 1) / (4 * SM_WAVE)) > 2048 ? 16 : 4;
+  t.C = (V + t.waves * SM_WAVE - 1) / (t.waves * SM_WAVE);
   size_t off = 0;
   const auto take = [&](size_t bytes) {
     char *p = base ? base + off : nullptr;
     off += up64(bytes);
     return p;
   };
-  t.mass = (uint64_t *)take((size_t)B * SM_BINS * 8);
-  t.csum = (uint64_t *)take((size_t)B * t.C * 8);
-  t.list = (uint64_t *)take((size_t)B * SM_CAP * 8);
-  t.st = (RowState *)take((size_t)B * sizeof(RowState));
-  t.count = (uint32_t *)take((size_t)B * SM_BINS * 4);
-  t.cmax = (float *)take((size_t)B * t.C * 4);
+  if (V > SM_ONE) {
+    t.mass = (uint64_t *)take((size_t)B * SM_BINS * 8);
+    t.wsum = (uint64_t *)take((size_t)B * t.C * t.waves * 8);
+    t.list = (uint64_t *)take((size_t)B * SM_CAP * 8);
+    t.st = (RowState *)take((size_t)B * sizeof(RowState));
+    t.count = (uint32_t *)take((size_t)B * SM_BINS * 4);
+    t.cmax = (float *)take((size_t)B * t.C * 4);
+  }
   if (w) *w = t;
   return off;
 }
@@ -77,23 +101,40 @@ __device__ __forceinline__ float logit<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ float logit<uint16_t>(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
 
-// f(i, z) over [lo, hi), the elements dealt to the workgroup's threads, 16 bytes
-// at a time where rows allow it (lo is a multiple of the chunk)
-template <typename T, typename F>
-__device__ __forceinline__ void each(const T *row, int lo, int hi, int vec, F f) {
-  constexpr int N = 16 / sizeof(T);
-  if (vec) {
-    const int full = lo + (hi - lo) / N * N;
-    for (int i = lo + threadIdx.x * N; i < full; i += blockDim.x * N) {
-      const uint4 q = *reinterpret_cast<const uint4 *>(row + i);
-      const T *e = reinterpret_cast<const T *>(&q);
+// A lane's 16 of a wave's 1024 logits from `base` on: 16 bytes at a time, group q's
+// element k being base + at<T>(q, lane) + k, so that (q, lane, k) rises with the
+// index.  Behind the row: NaN, which nothing counts.
+template <typename T>
+struct Lane {
+  static constexpr int N = 16 / sizeof(T), Q = 16 / N;
+  static __device__ __forceinline__ int at(int q, int lane) { return q * 64 * N + lane * N; }
+  float z[16];
+  int base, lane;
+  __device__ __forceinline__ int index(int e) const { return base + at(e / N, lane) + e % N; }
+  __device__ __forceinline__ void load(const T *row, int base_, int V, int vec) {
+    base = base_;
+    lane = threadIdx.x & 63;
 #pragma unroll
-      for (int j = 0; j < N; ++j) f(i + j, logit<T>(e[j]));
+    for (int q = 0; q < Q; ++q) {
+      const int i = base + at(q, lane);
+      if (vec && i + N <= V) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(row + i);
+        const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int k = 0; k < N; ++k) z[q * N + k] = logit<T>(e[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) z[q * N + k] = i + k < V ? logit<T>(row[i + k]) : __uint_as_float(0x7fc00000u);
+      }
     }
-    lo = full;
   }
-  for (int i = lo + threadIdx.x; i < hi; i += blockDim.x) f(i, logit<T>(row[i]));
-}
+  __device__ __forceinline__ float max() const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, z[e]);  // passes NaN by
+    return m;
+  }
+};
 
 __device__ __forceinline__ bool usable(float z) { return z > -INFINITY; }  // neither NaN nor -inf
 // rising with the logit, then with the falling index; -0 is 0
@@ -115,17 +156,26 @@ __device__ __forceinline__ int bin_of(double t) {
   const double x = t * -(double)SM_PER;
   return x < (double)(SM_BINS - 1) ? (int)x : SM_BINS - 1;
 }
-__device__ __forceinline__ double weight_scaled(double t, int up) {  // 2^up exp(t); 0 far below
-  if (!(t > -40.0)) return 0.0;
-  double n;
-  const double r = exp_r10(t, n);
-  return __builtin_ldexp(__builtin_fma(expm1_poly(r), r, 1.0), (int)n + up);
+// 2^43 exp(t) for t <= 0 of bin `bin`: the table's value times the series of the
+// rest, 1/32 at most (its first omitted term is below 6e-15 of the value); 0 in the
+// last bin, where a weight is below 2^-46
+__device__ __forceinline__ double weight_of(double t, int bin, const double *tab) {
+  if (bin >= SM_BINS - 1) return 0.0;
+  const double y = __builtin_fma((double)bin, 1.0 / SM_PER, t);
+  double p = 1.0 / 720.0;
+  p = __builtin_fma(p, y, 1.0 / 120.0);
+  p = __builtin_fma(p, y, 1.0 / 24.0);
+  p = __builtin_fma(p, y, 1.0 / 6.0);
+  p = __builtin_fma(p, y, 0.5);
+  p = __builtin_fma(p, y, 1.0);
+  p = __builtin_fma(p, y, 1.0);
+  return p * tab[bin];
 }
 // a number of [0, 2^43] to the nearest whole one
 __device__ __forceinline__ uint64_t whole(double w) {
   return (uint64_t)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
 }
-__device__ __forceinline__ uint64_t mass_of(double t) { return whole(weight_scaled(t, SM_MASS_BITS)); }
+__device__ __forceinline__ uint64_t mass_of(double t, int bin, const double *tab) { return whole(weight_of(t, bin, tab)); }
 
 struct RowSet {
   bool greedy, k_on, p_on;
@@ -172,75 +222,29 @@ struct Add {
 struct Or {
   __device__ uint64_t operator()(uint64_t a, uint64_t b) const { return a | b; }
 };
-// running sum over the workgroup's threads, this one's value included
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *sh) {  // sh: 16 values
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+  const int lane = threadIdx.x & 63;
   for (int o = 1; o < 64; o <<= 1) {
     const uint64_t x = __shfl_up(v, o, 64);
     if (lane >= o) v += x;
   }
+  return v;
+}
+// running sum over the workgroup's threads, this one's value included
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *sh) {  // sh: 16 values
+  const int w = threadIdx.x >> 6;
+  v = wave_scan(v);
   __syncthreads();
-  if (lane == 63) sh[w] = v;
+  if ((threadIdx.x & 63) == 63) sh[w] = v;
   __syncthreads();
   for (int i = 0; i < w; ++i) v += sh[i];
   return v;
 }
-__device__ __forceinline__ float row_max(const SampleWs &w, int b, float *sh) {
+// each wave for itself, without a barrier
+__device__ __forceinline__ float row_max(const SampleWs &w, int b) {
   float m = -INFINITY;
-  for (int i = threadIdx.x; i < w.C; i += blockDim.x) m = fmaxf(m, w.cmax[(int64_t)b * w.C + i]);
-  return block_reduce(m, sh, Max());
-}
-
-// the chunk's largest logit; clears what the later passes add to
-template <typename T>
-__global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a, SampleWs w, int vec) {
-  __shared__ float sh[16];
-  const int c = blockIdx.x, b = blockIdx.y;
-  const T *row = (const T *)a.z + (int64_t)b * a.stride;
-  for (int i = c * 256 + threadIdx.x; i < SM_BINS; i += w.C * 256) {
-    w.mass[(int64_t)b * SM_BINS + i] = 0;
-    w.count[(int64_t)b * SM_BINS + i] = 0;
-  }
-  if (c == 0 && threadIdx.x == 0) {
-    w.st[b].tau = 0;
-    w.st[b].nlist = 0;
-  }
-  float m = -INFINITY;
-  each<T>(row, c * w.chunk, min(a.V, (c + 1) * w.chunk), vec, [&](int, float z) { m = fmaxf(m, z); });  // passes NaN by
-  m = block_reduce(m, sh, Max());
-  if (threadIdx.x == 0) w.cmax[(int64_t)b * w.C + c] = m;
-}
-
-// counts and weights by distance from the maximum
-template <typename T>
-__global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs a, SampleWs w, int vec) {
-  __shared__ unsigned long long hm[SM_BINS];
-  __shared__ uint32_t hc[SM_BINS];
-  __shared__ float sh[16];
-  const int c = blockIdx.x, b = blockIdx.y;
-  const RowSet s = row_set(a, b);
-  if (!cuts(s)) return;
-  const float m = row_max(w, b, sh);
-  for (int i = threadIdx.x; i < SM_BINS; i += 256) {
-    hm[i] = 0;
-    hc[i] = 0;
-  }
-  __syncthreads();
-  const T *row = (const T *)a.z + (int64_t)b * a.stride;
-  each<T>(row, c * w.chunk, min(a.V, (c + 1) * w.chunk), vec, [&](int, float z) {
-    if (!usable(z)) return;
-    const double t = scaled(z, m, s.invT);
-    const int bin = bin_of(t);
-    atomicAdd(&hc[bin], 1u);
-    const uint64_t q = mass_of(t);
-    if (q) atomicAdd(&hm[bin], (unsigned long long)q);
-  });
-  __syncthreads();
-  for (int i = threadIdx.x; i < SM_BINS; i += 256)
-    if (hc[i]) {
-      atomicAdd(&w.count[(int64_t)b * SM_BINS + i], hc[i]);
-      if (hm[i]) atomicAdd((unsigned long long *)&w.mass[(int64_t)b * SM_BINS + i], hm[i]);
-    }
+  for (int i = threadIdx.x & 63; i < w.C; i += 64) m = fmaxf(m, w.cmax[(int64_t)b * w.C + i]);
+  return wave_reduce(m, Max());
 }
 
 // whole multiples that reach the share p of a sum (at least one)
@@ -249,129 +253,155 @@ __device__ __forceinline__ uint64_t share(float p, uint64_t sum) {
   return t < 1.0 ? 1 : (uint64_t)t;
 }
 
-// The bins in which top-k and top-p cut, and their elements into the row's list.
-// Every chunk finds the same bins from the histogram.
-template <typename T>
-__global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a, SampleWs w, int vec) {
-  __shared__ uint64_t cm[SM_BINS];  // running mass, bin included
-  __shared__ uint32_t cc[SM_BINS];  // running count
-  __shared__ uint64_t sh[16];
-  __shared__ float shf[16];
-  __shared__ int found[3];          // kbin, plo, phi
-  const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const RowSet s = row_set(a, b);
-  if (!cuts(s)) return;
-  const float m = row_max(w, b, shf);
-  constexpr int PT = SM_BINS / 256;
+struct Bins {
+  uint64_t cm[SM_BINS];  // running mass, bin included
+  uint32_t cc[SM_BINS];  // running count
+  uint64_t sm[16], sn[16];
+  int found[3];          // kbin, plo, phi
+};
+// The bins in which top-k and top-p cut, from a row's histogram (NT threads; mass and
+// count may be cm and cc).
+template <int NT>
+__device__ RowState cut_bins(const RowSet &s, const uint64_t *mass, const uint32_t *count, Bins &S) {
+  constexpr int PT = SM_BINS / NT;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   uint64_t mv[PT], ms = 0, ns = 0;
   uint32_t nv[PT];
+#pragma unroll
   for (int i = 0; i < PT; ++i) {
-    mv[i] = w.mass[(int64_t)b * SM_BINS + tid * PT + i];
-    nv[i] = w.count[(int64_t)b * SM_BINS + tid * PT + i];
+    mv[i] = mass[tid * PT + i];
+    nv[i] = count[tid * PT + i];
     ms += mv[i];
     ns += nv[i];
   }
-  uint64_t mc = block_scan(ms, sh) - ms, nc = block_scan(ns, sh) - ns;
+  uint64_t mc = wave_scan(ms), nc = wave_scan(ns);
+  if (lane == 63) {
+    S.sm[w] = mc;
+    S.sn[w] = nc;
+  }
+  if (tid < 3) S.found[tid] = -1;
+  __syncthreads();
+  for (int i = 0; i < w; ++i) {
+    mc += S.sm[i];
+    nc += S.sn[i];
+  }
+  mc -= ms;
+  nc -= ns;
+#pragma unroll
   for (int i = 0; i < PT; ++i) {
     mc += mv[i];
     nc += nv[i];
-    cm[tid * PT + i] = mc;
-    cc[tid * PT + i] = (uint32_t)nc;
+    S.cm[tid * PT + i] = mc;
+    S.cc[tid * PT + i] = (uint32_t)nc;
   }
-  if (tid < 3) found[tid] = -1;
   __syncthreads();
-  const uint64_t total = cm[SM_BINS - 1];
-  const uint32_t n = cc[SM_BINS - 1], K = s.k_on && (uint32_t)s.k < n ? (uint32_t)s.k : n;
+  const uint64_t total = S.cm[SM_BINS - 1];
+  const uint32_t n = S.cc[SM_BINS - 1], K = s.k_on && (uint32_t)s.k < n ? (uint32_t)s.k : n;
   if (K < n)
     for (int i = tid * PT; i < tid * PT + PT; ++i)
-      if (cc[i] >= K && (i == 0 || cc[i - 1] < K)) found[0] = i;
+      if (S.cc[i] >= K && (i == 0 || S.cc[i - 1] < K)) S.found[0] = i;
   __syncthreads();
-  const int kbin = found[0];
-  const uint64_t mass_k = kbin > 0 ? cm[kbin - 1] : 0;
+  RowState r;
+  r.kbin = S.found[0];
+  r.total = total;
+  r.mass_k = r.kbin > 0 ? S.cm[r.kbin - 1] : 0;
+  r.r = r.kbin < 0 ? 0 : K - (r.kbin > 0 ? S.cc[r.kbin - 1] : 0);
   if (s.p_on && n > 0) {
     // top-k's sum lies between these; the exact one decides inside the bins
-    const uint64_t lo = share(s.p, kbin < 0 ? total : mass_k), hi = share(s.p, kbin < 0 ? total : cm[kbin]);
+    const uint64_t lo = share(s.p, r.kbin < 0 ? total : r.mass_k), hi = share(s.p, r.kbin < 0 ? total : S.cm[r.kbin]);
     for (int i = tid * PT; i < tid * PT + PT; ++i) {
-      const uint64_t before = i ? cm[i - 1] : 0;
-      if (cm[i] >= lo && before < lo) found[1] = i;
-      if (cm[i] >= hi && before < hi) found[2] = i;
+      const uint64_t before = i ? S.cm[i - 1] : 0;
+      if (S.cm[i] >= lo && before < lo) S.found[1] = i;
+      if (S.cm[i] >= hi && before < hi) S.found[2] = i;
     }
   }
   __syncthreads();
-  const int plo = found[1], phi = found[2];
-  if (c == 0 && tid == 0) {
-    RowState &r = w.st[b];
-    r.kbin = kbin;
-    r.plo = plo;
-    r.phi = phi;
-    r.total = total;
-    r.mass_k = mass_k;
-    r.mass_p = plo > 0 ? cm[plo - 1] : 0;
-    r.r = kbin < 0 ? 0 : K - (kbin > 0 ? cc[kbin - 1] : 0);
-  }
-  if (kbin < 0 && plo < 0) return;
-  const T *row = (const T *)a.z + (int64_t)b * a.stride;
-  each<T>(row, c * w.chunk, min(a.V, (c + 1) * w.chunk), vec, [&](int i, float z) {
-    if (!usable(z)) return;
-    const int bin = bin_of(scaled(z, m, s.invT));
-    if (bin != kbin && !(bin >= plo && bin <= phi && plo >= 0)) return;
-    const uint32_t at = atomicAdd(&w.st[b].nlist, 1u);
-    if (at < (uint32_t)SM_CAP) w.list[(int64_t)b * SM_CAP + at] = key_of(z, i);
-  });
+  r.plo = S.found[1];
+  r.phi = S.found[2];
+  r.mass_p = r.plo > 0 ? S.cm[r.plo - 1] : 0;
+  // all that can be kept lies in bins 0 .. last
+  int last = r.plo >= 0 ? r.phi : r.kbin >= 0 ? r.kbin : SM_BINS - 1;
+  if (s.minp > 0.f) last = min(last, bin_of(log((double)fminf(s.minp, 1.f))) + 1);
+  r.last = S.cc[last] <= (uint32_t)SM_CAP ? last : -1;
+  r.tau = 0;
+  r.nlist = 0;
+  r.done = r.pad = 0;
+  return r;
 }
-
-// candidates of bins [b0, b1]: from the list where it holds them all, else from
-// the row again
-template <typename T>
-struct Source {
-  const uint64_t *list;
-  const T *row;
-  int n, V;  // n < 0: the row
-  float m;
-  double invT;
-  template <typename F>
-  __device__ __forceinline__ void each_key(int b0, int b1, F f) const {
-    const int N = n >= 0 ? n : V;
-    for (int i = threadIdx.x; i < N; i += blockDim.x) {
-      uint64_t key;
-      float z;
-      if (n >= 0) {
-        key = list[i];
-        z = z_of(key);
-      } else {
-        z = logit<T>(row[i]);
-        if (!usable(z)) continue;
-        key = key_of(z, i);
-      }
-      const double t = scaled(z, m, invT);
-      const int bin = bin_of(t);
-      if (bin >= b0 && bin <= b1) f(key, t);
+// Up to SM_RANK candidates (in any order), one a thread: how many of their bins lie
+// above one, and their mass, say where the cuts fall.
+struct Ranks {
+  uint64_t key[SM_RANK], mass[SM_RANK];
+  uint32_t in[SM_RANK];  // 1: of kbin, 2: of plo .. phi
+  uint32_t n;
+  uint64_t tau_k, above_k, tau_p;
+};
+__device__ __forceinline__ uint32_t cut_of(const RowState &r, int bin) {
+  return (bin == r.kbin ? 1u : 0u) | (r.plo >= 0 && bin >= r.plo && bin <= r.phi ? 2u : 0u);
+}
+__device__ uint64_t cut_by_rank(const RowSet &s, const RowState &r, float m, const double *tab, Ranks &S) {
+  const int tid = threadIdx.x, n = (int)S.n;
+  uint64_t key = 0, q = 0;
+  uint32_t in = 0;
+  if (tid < n) {
+    key = S.key[tid];
+    const double t = scaled(z_of(key), m, s.invT);
+    const int bin = bin_of(t);
+    q = mass_of(t, bin, tab);
+    in = cut_of(r, bin);
+    S.mass[tid] = q;
+    S.in[tid] = in;
+  }
+  if (tid == 0) S.tau_k = S.tau_p = S.above_k = 0;
+  __syncthreads();
+  uint64_t mk = 0, mp = 0;
+  uint32_t ck = 0;
+  if (tid < n) {
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const bool over = S.key[j] > key;
+      const uint64_t qj = S.mass[j];
+      const uint32_t ij = S.in[j];
+      ck += over && (ij & 1);
+      mk += over && (ij & 1) ? qj : 0;
+      mp += over && (ij & 2) ? qj : 0;
+    }
+    if ((in & 1) && ck == r.r - 1) {
+      S.tau_k = key;
+      S.above_k = mk + q;
     }
   }
-};
+  __syncthreads();
+  if (tid < n && (in & 2)) {
+    const uint64_t need = share(s.p, r.kbin >= 0 ? r.mass_k + S.above_k : r.total) - r.mass_p;
+    if (mp < need && mp + q >= need) S.tau_p = key;
+  }
+  __syncthreads();
+  return S.tau_k > S.tau_p ? S.tau_k : S.tau_p;
+}
 
-struct CutShared {
+struct Radix {
   unsigned long long amount[256], mass[256];
   uint32_t count[256];
   uint64_t sh[16];
   uint64_t need, prefix, above, key;
-  int bucket, single;
+  int single;
 };
-// The key at which the running amount (elements, or their mass) over falling keys
-// of bins [b0, b1] reaches `need`; above: the mass of the elements over that key, it
-// included.
-template <bool MASS, typename T>
-__device__ uint64_t cut_key(const Source<T> &src, int b0, int b1, uint64_t need, CutShared &S, uint64_t &above) {
+// The key at which the running amount over falling keys reaches `need`; above: the
+// mass of the elements over that key, it included.  each(f): f(key, amount, mass)
+// for this thread's elements, the keys all different.
+template <typename Each>
+__device__ uint64_t find_by_radix(const Each &each, uint64_t need, Radix &S, uint64_t &above) {
   const int tid = threadIdx.x;
-  // bits in which the candidates differ at all
-  uint64_t any = 0, all = ~0ull;
-  src.each_key(b0, b1, [&](uint64_t key, double) {
+  // bits in which the keys differ at all
+  uint64_t any = 0, none = 0;
+  each([&](uint64_t key, uint64_t, uint64_t) {
     any |= key;
-    all &= key;
+    none |= ~key;
   });
   any = block_reduce(any, S.sh, Or());
-  all = ~block_reduce(~all, S.sh, Or());
-  const uint64_t diff = any ^ all;
+  none = block_reduce(none, S.sh, Or());
+  const uint64_t diff = any & none;
   int shift = diff ? (63 - __builtin_clzll(diff)) / 8 * 8 : 0;
   __syncthreads();
   if (tid == 0) {
@@ -388,19 +418,17 @@ __device__ uint64_t cut_key(const Source<T> &src, int b0, int b1, uint64_t need,
     }
     __syncthreads();
     const uint64_t prefix = S.prefix, want = S.need;
-    src.each_key(b0, b1, [&](uint64_t key, double t) {
+    each([&](uint64_t key, uint64_t amount, uint64_t mass) {
       if (shift < 56 && key >> (shift + 8) != prefix) return;
       const int d = 255 - (int)(key >> shift & 255);  // falling order
-      const uint64_t q = mass_of(t);
       atomicAdd(&S.count[d], 1u);
-      atomicAdd(&S.mass[d], (unsigned long long)q);
-      atomicAdd(&S.amount[d], (unsigned long long)(MASS ? q : 1));
+      atomicAdd(&S.mass[d], (unsigned long long)mass);
+      atomicAdd(&S.amount[d], (unsigned long long)amount);
     });
     __syncthreads();
     const uint64_t mine = tid < 256 ? S.amount[tid] : 0, mm = tid < 256 ? S.mass[tid] : 0;
     const uint64_t sum = block_scan(mine, S.sh), summ = block_scan(mm, S.sh);
     if (tid < 256 && sum >= want && sum - mine < want) {
-      S.bucket = tid;
       S.need = want - (sum - mine);
       S.above += summ - mm;
       S.prefix = (shift == 56 ? 0 : prefix << 8) | (uint64_t)(255 - tid);
@@ -408,17 +436,15 @@ __device__ uint64_t cut_key(const Source<T> &src, int b0, int b1, uint64_t need,
       if (S.single || shift == 0) S.above += mm;
     }
     __syncthreads();
-    if (shift == 0) {
-      above = S.above;
-      const uint64_t key = S.prefix;
-      __syncthreads();
-      return key;
-    }
-    if (S.single) {
+    if (shift == 0 || S.single) {
       const uint64_t pre = S.prefix;
-      src.each_key(b0, b1, [&](uint64_t key, double) {
-        if (key >> shift == pre) S.key = key;
-      });
+      if (shift == 0) {
+        if (tid == 0) S.key = pre;
+      } else {
+        each([&](uint64_t key, uint64_t, uint64_t) {
+          if (key >> shift == pre) S.key = key;
+        });
+      }
       __syncthreads();
       above = S.above;
       const uint64_t key = S.key;
@@ -427,100 +453,132 @@ __device__ uint64_t cut_key(const Source<T> &src, int b0, int b1, uint64_t need,
     }
   }
 }
-
-// the exact cut among the candidates
-template <typename T>
-__global__ __launch_bounds__(1024) void sample_cut_kernel(SampleArgs a, SampleWs w) {
-  __shared__ CutShared S;
-  __shared__ float shf[16];
-  const int b = blockIdx.x;
-  const RowSet s = row_set(a, b);
-  if (!cuts(s)) return;
-  const RowState r = w.st[b];
-  if (r.kbin < 0 && r.plo < 0) return;
-  Source<T> src;
-  src.list = w.list + (int64_t)b * SM_CAP;
-  src.row = (const T *)a.z + (int64_t)b * a.stride;
-  src.n = r.nlist <= (uint32_t)SM_CAP ? (int)r.nlist : -1;
-  src.V = a.V;
-  src.m = row_max(w, b, shf);
-  src.invT = s.invT;
+// all(f): f(key) for this thread's candidates, or for all elements of the row
+template <typename All>
+__device__ uint64_t cut_by_radix(const All &all, const RowSet &s, const RowState &r, float m, const double *tab, Radix &S) {
   uint64_t tau = 0, sum = r.total, above;
+  const auto of = [&](uint32_t cut, bool mass, auto f) {
+    all([&](uint64_t key) {
+      const double t = scaled(z_of(key), m, s.invT);
+      const int bin = bin_of(t);
+      if (!(cut_of(r, bin) & cut)) return;
+      const uint64_t q = mass_of(t, bin, tab);
+      f(key, mass ? q : 1, q);
+    });
+  };
   if (r.kbin >= 0) {
-    tau = cut_key<false>(src, r.kbin, r.kbin, r.r, S, above);
+    tau = find_by_radix([&](auto f) { of(1, false, f); }, r.r, S, above);
     sum = r.mass_k + above;
   }
   if (r.plo >= 0) {
-    const uint64_t key = cut_key<true>(src, r.plo, r.phi, share(s.p, sum) - r.mass_p, S, above);
+    const uint64_t key = find_by_radix([&](auto f) { of(2, true, f); }, share(s.p, sum) - r.mass_p, S, above);
     tau = key > tau ? key : tau;
   }
-  if (threadIdx.x == 0) w.st[b].tau = tau;
+  return tau;
 }
 
 // the weight an element keeps, as a whole number
-__device__ __forceinline__ uint64_t kept(float z, int i, float m, const RowSet &s, uint64_t tau) {
+__device__ __forceinline__ uint64_t kept(float z, int i, float m, const RowSet &s, uint64_t tau, const double *tab) {
   if (!usable(z)) return 0;
   if (z == m) return s.greedy || key_of(z, i) >= tau ? 1ull << SM_MASS_BITS : 0;
   if (s.greedy || key_of(z, i) < tau) return 0;
-  const double e = weight_scaled(scaled(z, m, s.invT), SM_MASS_BITS);
+  const double t = scaled(z, m, s.invT), e = weight_of(t, bin_of(t), tab);
   return e >= __builtin_ldexp((double)s.minp, SM_MASS_BITS) ? whole(e) : 0;
 }
-
-template <typename T>
-__global__ __launch_bounds__(256) void sample_sum_kernel(SampleArgs a, SampleWs w, int vec) {
-  __shared__ float shf[16];
-  __shared__ uint64_t sh[16];
-  const int c = blockIdx.x, b = blockIdx.y;
-  const RowSet s = row_set(a, b);
-  const float m = row_max(w, b, shf);
-  const uint64_t tau = w.st[b].tau;
-  const T *row = (const T *)a.z + (int64_t)b * a.stride;
-  uint64_t q = 0;
-  each<T>(row, c * w.chunk, min(a.V, (c + 1) * w.chunk), vec, [&](int i, float z) { q += kept(z, i, m, s, tau); });
-  q = block_reduce(q, sh, Add());
-  if (threadIdx.x == 0) w.csum[(int64_t)b * w.C + c] = q;
+// the place of the draw in kept weights of sum W > 0
+__device__ __forceinline__ uint64_t draw_at(const RowSet &s, float u, uint64_t W) {
+  const uint64_t t = !s.greedy && u > 0.f ? (uint64_t)((double)fminf(u, 1.f) * (double)W) : 0;
+  return t < W ? t : W - 1;
 }
 
-// the chunk, the thread's run in it and the element at which the running sum
-// passes u times the whole
-template <typename T>
-__global__ __launch_bounds__(SM_MAX_CHUNKS) void sample_pick_kernel(SampleArgs a, SampleWs w) {
-  __shared__ float shf[16];
+// ---- rows of up to 16384 logits: every step in one workgroup --------------------
+// A thread's sixteen logits follow each other (runs of 17 words, for the banks), so
+// that a scan over the threads is one over the indexes.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
+  extern __shared__ float z[];
+  __shared__ union {
+    Bins bins;
+    Ranks ranks;
+    Radix radix;
+  } S;
+  __shared__ double tab[SM_BINS];
   __shared__ uint64_t sh[16];
-  __shared__ uint64_t need;
-  __shared__ int at;
+  __shared__ float shf[16];
   const int b = blockIdx.x, tid = threadIdx.x;
   const RowSet s = row_set(a, b);
-  const float m = row_max(w, b, shf);
-  const uint64_t tau = w.st[b].tau;
-  const uint64_t mine = tid < w.C ? w.csum[(int64_t)b * w.C + tid] : 0;
-  const uint64_t sum = block_scan(mine, sh);
-  const uint64_t W = block_reduce(mine, sh, Add());
+  const float u = a.u[b];
+  const T *row = (const T *)a.z + (int64_t)b * a.stride;
+  float m = -INFINITY;
+#pragma unroll 8
+  for (int e = 0; e < 16; ++e) {
+    const int i = e * NT + tid;
+    const float v = i < a.V ? logit<T>(row[i]) : __uint_as_float(0x7fc00000u);
+    z[i + (i >> 4)] = v;
+    m = fmaxf(m, v);  // passes NaN by
+  }
+  const bool cut = cuts(s);
+  for (int i = tid; i < SM_BINS; i += NT) {
+    tab[i] = exp_table.v[i];
+    S.bins.cm[i] = 0;
+    S.bins.cc[i] = 0;
+  }
+  m = block_reduce(m, shf, Max());  // and a barrier for the rest
+  const float *mine = z + tid * 17;
+  uint64_t tau = 0;
+  if (cut) {
+    unsigned long long *hm = (unsigned long long *)S.bins.cm;
+#pragma unroll 4
+    for (int e = 0; e < 16; ++e)
+      if (usable(mine[e])) {
+        const double t = scaled(mine[e], m, s.invT);
+        const int bin = bin_of(t);
+        atomicAdd(&S.bins.cc[bin], 1u);
+        const uint64_t q = mass_of(t, bin, tab);
+        if (q) atomicAdd(&hm[bin], (unsigned long long)q);
+      }
+    __syncthreads();
+    const RowState r = cut_bins<NT>(s, S.bins.cm, S.bins.cc, S.bins);
+    if (r.kbin >= 0 || r.plo >= 0) {
+      __syncthreads();  // the bins are read, the ranks lie in their place
+      if (tid == 0) S.ranks.n = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int e = 0; e < 16; ++e)
+        if (usable(mine[e]) && cut_of(r, bin_of(scaled(mine[e], m, s.invT)))) {
+          const uint32_t at = atomicAdd(&S.ranks.n, 1u);
+          if (at < SM_RANK) S.ranks.key[at] = key_of(mine[e], tid * 16 + e);
+        }
+      __syncthreads();
+      if (S.ranks.n <= SM_RANK) {
+        tau = cut_by_rank(s, r, m, tab, S.ranks);
+      } else {
+        __syncthreads();
+        const auto all = [&](auto f) {
+          for (int e = 0; e < 16; ++e)
+            if (usable(mine[e])) f(key_of(mine[e], tid * 16 + e));
+        };
+        tau = cut_by_radix(all, s, r, m, tab, S.radix);
+      }
+    }
+  }
+  uint64_t q = 0;
+#pragma unroll 4
+  for (int e = 0; e < 16; ++e) q += kept(mine[e], tid * 16 + e, m, s, tau, tab);
+  const uint64_t run = block_scan(q, sh);
+  uint64_t W = 0;
+  for (int i = 0; i < NT / 64; ++i) W += sh[i];
   if (W == 0) {
     if (tid == 0) a.ids[b] = -1;
     return;
   }
-  const float u = a.u[b];
-  uint64_t t = !s.greedy && u > 0.f ? (uint64_t)((double)fminf(u, 1.f) * (double)W) : 0;
-  if (t >= W) t = W - 1;
-  if (sum > t && sum - mine <= t) {
-    at = tid;
-    need = t - (sum - mine);
-  }
-  __syncthreads();
-  const int c = at;
-  t = need;
-  const T *row = (const T *)a.z + (int64_t)b * a.stride;
-  const int run = w.chunk / SM_MAX_CHUNKS, lo = c * w.chunk + tid * run, hi = min(a.V, lo + run);
-  uint64_t q = 0;
-  for (int i = lo; i < hi; ++i) q += kept(logit<T>(row[i]), i, m, s, tau);
-  const uint64_t run_sum = block_scan(q, sh);
-  if (run_sum > t && run_sum - q <= t) {
-    t -= run_sum - q;
-    for (int i = lo; i < hi; ++i) {
-      const uint64_t k = kept(logit<T>(row[i]), i, m, s, tau);
+  uint64_t t = draw_at(s, u, W);
+  if (run > t && run - q <= t) {
+    t -= run - q;
+    for (int e = 0; e < 16; ++e) {
+      const uint64_t k = kept(mine[e], tid * 16 + e, m, s, tau, tab);
       if (k > t) {
-        a.ids[b] = i;
+        a.ids[b] = tid * 16 + e;
         break;
       }
       t -= k;
@@ -528,19 +586,351 @@ __global__ __launch_bounds__(SM_MAX_CHUNKS) void sample_pick_kernel(SampleArgs a
   }
 }
 
+// ---- longer rows -------------------------------------------------------------
+// the chunk's largest logit; clears what the later passes add to
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_max_kernel(SampleArgs a, SampleWs w, int vec) {
+  __shared__ float sh[16];
+  const int c = blockIdx.x, b = blockIdx.y;
+  Lane<T> x;
+  x.load((const T *)a.z + (int64_t)b * a.stride, c * NT * 16 + (threadIdx.x >> 6) * SM_WAVE, a.V, vec);
+  for (int i = c * NT + threadIdx.x; i < SM_BINS; i += w.C * NT) {
+    w.mass[(int64_t)b * SM_BINS + i] = 0;
+    w.count[(int64_t)b * SM_BINS + i] = 0;
+  }
+  if (c == 0 && threadIdx.x == 0) {
+    w.st[b].tau = 0;
+    w.st[b].nlist = 0;
+    w.st[b].done = 0;
+  }
+  const float m = block_reduce(x.max(), sh, Max());
+  if (threadIdx.x == 0) w.cmax[(int64_t)b * w.C + c] = m;
+}
+
+// counts and weights by distance from the maximum
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_hist_kernel(SampleArgs a, SampleWs w, int vec) {
+  __shared__ unsigned long long hm[SM_BINS];
+  __shared__ uint32_t hc[SM_BINS];
+  __shared__ double tab[SM_BINS];
+  const int c = blockIdx.x, b = blockIdx.y;
+  Lane<T> x;
+  x.load((const T *)a.z + (int64_t)b * a.stride, c * NT * 16 + (threadIdx.x >> 6) * SM_WAVE, a.V, vec);
+  const RowSet s = row_set(a, b);
+  if (!cuts(s)) return;
+  const float m = row_max(w, b);
+  for (int i = threadIdx.x; i < SM_BINS; i += NT) {
+    hm[i] = 0;
+    hc[i] = 0;
+    tab[i] = exp_table.v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (usable(x.z[e])) {
+      const double t = scaled(x.z[e], m, s.invT);
+      const int bin = bin_of(t);
+      atomicAdd(&hc[bin], 1u);
+      const uint64_t q = mass_of(t, bin, tab);
+      if (q) atomicAdd(&hm[bin], (unsigned long long)q);
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < SM_BINS; i += NT)
+    if (hc[i]) {
+      atomicAdd(&w.count[(int64_t)b * SM_BINS + i], hc[i]);
+      if (hm[i]) atomicAdd((unsigned long long *)&w.mass[(int64_t)b * SM_BINS + i], hm[i]);
+    }
+}
+
+// the candidates into the row's list: all that can be kept where that is few, else
+// the elements of the bins in which top-k and top-p cut.  Every chunk finds the same
+// bins from the histogram.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_gather_kernel(SampleArgs a, SampleWs w, int vec) {
+  __shared__ Bins S;
+  const int c = blockIdx.x, b = blockIdx.y;
+  Lane<T> x;
+  x.load((const T *)a.z + (int64_t)b * a.stride, c * NT * 16 + (threadIdx.x >> 6) * SM_WAVE, a.V, vec);
+  const RowSet s = row_set(a, b);
+  if (!cuts(s)) return;
+  const float m = row_max(w, b);
+  const RowState r = cut_bins<NT>(s, w.mass + (int64_t)b * SM_BINS, w.count + (int64_t)b * SM_BINS, S);
+  if (c == 0 && threadIdx.x == 0) {
+    RowState &o = w.st[b];  // all but tau, nlist and done
+    o.kbin = r.kbin;
+    o.plo = r.plo;
+    o.phi = r.phi;
+    o.last = r.last;
+    o.total = r.total;
+    o.mass_k = r.mass_k;
+    o.mass_p = r.mass_p;
+    o.r = r.r;
+  }
+  uint32_t take = 0;  // this lane's candidates, a bit each
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int bin = bin_of(scaled(x.z[e], m, s.invT));
+    if (usable(x.z[e]) && (bin <= r.last || cut_of(r, bin))) take |= 1u << e;
+  }
+  // a wave takes its places in the list at once
+  const int mine = __popc(take), lane = threadIdx.x & 63;
+  int run = mine;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(run, o, 64);
+    if (lane >= o) run += y;
+  }
+  const int all = __shfl(run, 63, 64);
+  if (all == 0) return;
+  uint32_t at = 0;
+  if (lane == 0) at = atomicAdd(&w.st[b].nlist, (uint32_t)all);
+  at = __shfl(at, 0, 64) + run - mine;
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (take >> e & 1) {
+      if (at < (uint32_t)SM_CAP) w.list[(int64_t)b * SM_CAP + at] = key_of(x.z[e], x.index(e));
+      ++at;
+    }
+}
+
+// The exact cut among the candidates: few are ranked, more take the radix, from the
+// list or, where it does not hold them all, from the row.  Where the list holds all
+// that is kept the draw is made here too: the kept weights by the upper bits of
+// their indexes, then those of one of these 1024 runs of indexes against each other.
+template <typename T>
+__global__ __launch_bounds__(512) void sample_cut_kernel(SampleArgs a, SampleWs w) {
+  constexpr int NT = 512, PER = SM_CAP / NT;
+  __shared__ union {
+    Ranks ranks;
+    Radix radix;
+    unsigned long long run[1024];
+  } S;
+  __shared__ double tab[SM_BINS];
+  __shared__ uint64_t sh[16], need;
+  __shared__ int which;
+  __shared__ uint32_t found;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const RowSet s = row_set(a, b);
+  const RowState r = w.st[b];
+  if (!cuts(s)) return;
+  const uint64_t *list = w.list + (int64_t)b * SM_CAP;
+  const bool listed = r.nlist <= (uint32_t)SM_CAP;
+  const int n = listed ? (int)r.nlist : 0;
+  uint64_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = i * NT + tid < n ? list[i * NT + tid] : 0;  // no key is 0
+  for (int i = tid; i < SM_BINS; i += NT) tab[i] = exp_table.v[i];
+  if (tid == 0) S.ranks.n = 0;
+  const float m = row_max(w, b), u = a.u[b];
+  __syncthreads();
+  uint64_t tau = 0;
+  if (r.kbin >= 0 || r.plo >= 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] && cut_of(r, bin_of(scaled(z_of(key[i]), m, s.invT)))) {
+        const uint32_t at = atomicAdd(&S.ranks.n, 1u);
+        if (at < SM_RANK) S.ranks.key[at] = key[i];
+      }
+    __syncthreads();
+    if (listed && S.ranks.n <= SM_RANK) {
+      tau = cut_by_rank(s, r, m, tab, S.ranks);
+    } else {
+      __syncthreads();
+      const T *row = (const T *)a.z + (int64_t)b * a.stride;
+      const auto all = [&](auto f) {
+        if (listed) {
+          for (int i = tid; i < n; i += NT) f(list[i]);
+        } else {
+          for (int i = tid; i < a.V; i += NT) {
+            const float z = logit<T>(row[i]);
+            if (usable(z)) f(key_of(z, i));
+          }
+        }
+      };
+      tau = cut_by_radix(all, s, r, m, tab, S.radix);
+    }
+    if (tid == 0) w.st[b].tau = tau;
+  }
+  if (r.last < 0 || !listed) return;
+  const auto index = [](uint64_t k) { return (int)(0xffffffffu - (uint32_t)k); };
+  const int shift = a.V > 1 ? max(0, 32 - __clz(a.V - 1) - 10) : 0;  // indexes to 1024 runs
+  __syncthreads();
+  for (int i = tid; i < 1024; i += NT) S.run[i] = 0;
+  __syncthreads();
+  uint64_t q[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    q[i] = key[i] ? kept(z_of(key[i]), index(key[i]), m, s, tau, tab) : 0;
+    if (q[i]) atomicAdd(&S.run[index(key[i]) >> shift], (unsigned long long)q[i]);
+  }
+  __syncthreads();
+  const uint64_t r0 = S.run[tid * 2], r1 = S.run[tid * 2 + 1];
+  const uint64_t upto = block_scan(r0 + r1, sh);
+  uint64_t W = 0;
+  for (int i = 0; i < NT / 64; ++i) W += sh[i];
+  if (W > 0) {
+    const uint64_t t = draw_at(s, u, W), before = upto - r0 - r1;
+    if (t >= before && t < upto) {
+      which = tid * 2 + (t >= before + r0);
+      need = t - before - (t >= before + r0 ? r0 : 0);
+      found = 0xffffffffu;
+    }
+    __syncthreads();
+    // of that run: its kept elements, in a list of their own
+    if (tid == 0) S.ranks.n = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (q[i] && index(key[i]) >> shift == which) {
+        const uint32_t at = atomicAdd(&S.ranks.n, 1u);
+        if (at < SM_RANK) {
+          S.ranks.key[at] = (uint64_t)index(key[i]);
+          S.ranks.mass[at] = q[i];
+        }
+      }
+    __syncthreads();
+    const int k = (int)S.ranks.n;
+    if (k <= SM_RANK) {
+      if (tid < k) {
+        const uint64_t at = S.ranks.key[tid];
+        uint64_t under = 0;
+        for (int j = 0; j < k; ++j) under += S.ranks.key[j] < at ? S.ranks.mass[j] : 0;
+        if (need >= under && need < under + S.ranks.mass[tid]) found = (uint32_t)at;
+      }
+    } else {
+      __syncthreads();
+      // falling lower halves of the keys are rising indexes
+      const auto all = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (q[i] && index(key[i]) >> shift == which) f(key[i] & 0xffffffffu, q[i], q[i]);
+      };
+      uint64_t above;
+      const uint64_t low = find_by_radix(all, need + 1, S.radix, above);
+      if (tid == 0) found = (uint32_t)index(low);
+    }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    a.ids[b] = W > 0 ? (int32_t)found : -1;
+    w.st[b].done = 1;
+  }
+}
+
+// kept weights of every 1024 logits, where the list does not hold them
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_sum_kernel(SampleArgs a, SampleWs w, int vec) {
+  const int c = blockIdx.x, b = blockIdx.y, wave = c * (NT / 64) + (threadIdx.x >> 6);
+  if (w.st[b].done) return;
+  Lane<T> x;
+  x.load((const T *)a.z + (int64_t)b * a.stride, wave * SM_WAVE, a.V, vec);
+  const RowSet s = row_set(a, b);
+  const float m = row_max(w, b);
+  const uint64_t tau = w.st[b].tau;
+  uint64_t q = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) q += kept(x.z[e], x.index(e), m, s, tau, exp_table.v);
+  q = wave_reduce(q, Add());
+  if ((threadIdx.x & 63) == 0) w.wsum[(int64_t)b * w.C * w.waves + wave] = q;
+}
+
+// the 1024 logits and the one of them at which the running sum passes the draw
+template <typename T>
+__global__ __launch_bounds__(256) void sample_pick_kernel(SampleArgs a, SampleWs w, int vec) {
+  constexpr int PT = SAMPLE_MAX_V / SM_WAVE / 256, N = Lane<T>::N;
+  __shared__ uint64_t sh[16], need;
+  __shared__ int at;
+  const int b = blockIdx.x, tid = threadIdx.x, n = w.C * w.waves;
+  if (w.st[b].done) return;
+  const RowSet s = row_set(a, b);
+  const float m = row_max(w, b);
+  const uint64_t tau = w.st[b].tau;
+  uint64_t v[PT], mine = 0;
+#pragma unroll
+  for (int i = 0; i < PT; ++i) {
+    v[i] = tid * PT + i < n ? w.wsum[(int64_t)b * n + tid * PT + i] : 0;
+    mine += v[i];
+  }
+  uint64_t sum = block_scan(mine, sh), W = 0;
+  for (int i = 0; i < 4; ++i) W += sh[i];
+  if (W == 0) {
+    if (tid == 0) a.ids[b] = -1;
+    return;
+  }
+  const uint64_t t0 = draw_at(s, a.u[b], W);
+  sum -= mine;
+#pragma unroll
+  for (int i = 0; i < PT; ++i) {
+    if (t0 >= sum && t0 < sum + v[i]) {
+      at = tid * PT + i;
+      need = t0 - sum;
+    }
+    sum += v[i];
+  }
+  __syncthreads();
+  if (tid >= 64) return;
+  Lane<T> x;
+  x.load((const T *)a.z + (int64_t)b * a.stride, at * SM_WAVE, a.V, vec);
+  uint64_t t = need;
+#pragma unroll
+  for (int g = 0; g < Lane<T>::Q; ++g) {
+    uint64_t k[N], q = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      k[e] = kept(x.z[g * N + e], x.index(g * N + e), m, s, tau, exp_table.v);
+      q += k[e];
+    }
+    const uint64_t run = wave_scan(q), all = __shfl(run, 63, 64);
+    if (t < all) {
+      if (run > t && run - q <= t) {
+        t -= run - q;
+        int e = 0;
+        bool more = true;
+#pragma unroll
+        for (int i = 0; i < N - 1; ++i) {
+          more = more && t >= k[i];
+          e += more;
+          t -= more ? k[i] : 0;
+        }
+        a.ids[b] = x.index(g * N) + e;
+      }
+      return;
+    }
+    t -= all;
+  }
+}
+
+template <typename T, int NT>
+hipError_t sample_row(const SampleArgs &a, hipStream_t s) {
+  const int lds = NT * 17 * 4;
+  const auto fn = sample_row_kernel<T, NT>;
+  if (NT == 1024) {  // with its other arrays beyond 64 KiB
+    static std::atomic<int> set[kAttrDevices];
+    const hipError_t e = ensure_lds_attr((const void *)fn, lds, set);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(fn, dim3(a.B), dim3(NT), lds, s, a);
+  return hipGetLastError();
+}
+template <typename T, int NT>
+hipError_t sample_chunks(const SampleArgs &a, const SampleWs &w, hipStream_t s) {
+  const int vec = ((uintptr_t)a.z & 15) == 0 && (a.stride * sizeof(T)) % 16 == 0;
+  const dim3 grid(w.C, a.B);
+  hipLaunchKernelGGL((sample_max_kernel<T, NT>), grid, dim3(NT), 0, s, a, w, vec);
+  if (a.top_k || a.top_p) {
+    hipLaunchKernelGGL((sample_hist_kernel<T, NT>), grid, dim3(NT), 0, s, a, w, vec);
+    hipLaunchKernelGGL((sample_gather_kernel<T, NT>), grid, dim3(NT), 0, s, a, w, vec);
+    hipLaunchKernelGGL(sample_cut_kernel<T>, dim3(a.B), dim3(512), 0, s, a, w);
+  }
+  hipLaunchKernelGGL((sample_sum_kernel<T, NT>), grid, dim3(NT), 0, s, a, w, vec);
+  hipLaunchKernelGGL(sample_pick_kernel<T>, dim3(a.B), dim3(256), 0, s, a, w, vec);
+  return hipGetLastError();
+}
 template <typename T>
 hipError_t sample_run(const SampleArgs &a, const SampleWs &w, hipStream_t s) {
-  const dim3 grid(w.C, a.B);
-  const int vec = ((uintptr_t)a.z & 15) == 0 && (a.stride * sizeof(T)) % 16 == 0;
-  hipLaunchKernelGGL(sample_max_kernel<T>, grid, dim3(256), 0, s, a, w, vec);
-  if (a.top_k || a.top_p) {
-    hipLaunchKernelGGL(sample_hist_kernel<T>, grid, dim3(256), 0, s, a, w, vec);
-    hipLaunchKernelGGL(sample_gather_kernel<T>, grid, dim3(256), 0, s, a, w, vec);
-    hipLaunchKernelGGL(sample_cut_kernel<T>, dim3(a.B), dim3(1024), 0, s, a, w);
-  }
-  hipLaunchKernelGGL(sample_sum_kernel<T>, grid, dim3(256), 0, s, a, w, vec);
-  hipLaunchKernelGGL(sample_pick_kernel<T>, dim3(a.B), dim3(SM_MAX_CHUNKS), 0, s, a, w);
-  return hipGetLastError();
+  if (a.V <= SM_ONE / 4) return sample_row<T, 256>(a, s);
+  if (a.V <= SM_ONE / 2) return sample_row<T, 512>(a, s);
+  if (a.V <= SM_ONE) return sample_row<T, 1024>(a, s);
+  return w.waves == 4 ? sample_chunks<T, 256>(a, w, s) : sample_chunks<T, 1024>(a, w, s);
 }
 
 }  // namespace
