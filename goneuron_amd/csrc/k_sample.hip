@@ -147,29 +147,26 @@ __device__ __forceinline__ float z_of(uint64_t key) {
   const uint32_t k = (uint32_t)(key >> 32);
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
-// (z - max) / T in float64, falling with z; 0 for the maximum itself, also where
-// it is infinite
-__device__ __forceinline__ double scaled(float z, float m, double invT) {
-  return z == m ? 0.0 : ((double)z - (double)m) * invT;
+// 32 (max - z) / T in float64 (per: 32 / T), rising as z falls; 0 for the maximum
+// itself, also where it is infinite
+__device__ __forceinline__ double scaled(float z, float m, double per) {
+  return z == m ? 0.0 : ((double)m - (double)z) * per;
 }
-__device__ __forceinline__ int bin_of(double t) {
-  const double x = t * -(double)SM_PER;
-  return x < (double)(SM_BINS - 1) ? (int)x : SM_BINS - 1;
-}
-// 2^43 exp(t) for t <= 0 of bin `bin`: the table's value times the series of the
+__device__ __forceinline__ int bin_of(double x) { return x < (double)(SM_BINS - 1) ? (int)x : SM_BINS - 1; }
+// 2^43 exp(-x / 32) for x of bin `bin`: the table's value times the series of the
 // rest, 1/32 at most (its first omitted term is below 6e-15 of the value); 0 in the
 // last bin, where a weight is below 2^-46
-__device__ __forceinline__ double weight_of(double t, int bin, const double *tab) {
-  if (bin >= SM_BINS - 1) return 0.0;
-  const double y = __builtin_fma((double)bin, 1.0 / SM_PER, t);
-  double p = 1.0 / 720.0;
-  p = __builtin_fma(p, y, 1.0 / 120.0);
-  p = __builtin_fma(p, y, 1.0 / 24.0);
-  p = __builtin_fma(p, y, 1.0 / 6.0);
-  p = __builtin_fma(p, y, 0.5);
-  p = __builtin_fma(p, y, 1.0);
-  p = __builtin_fma(p, y, 1.0);
-  return p * tab[bin];
+__device__ __forceinline__ double weight_of(double x, int bin, const double *tab) {
+  constexpr double c = -1.0 / SM_PER;
+  const double f = x - (double)bin;
+  double p = c * c * c * c * c * c / 720.0;
+  p = __builtin_fma(p, f, c * c * c * c * c / 120.0);
+  p = __builtin_fma(p, f, c * c * c * c / 24.0);
+  p = __builtin_fma(p, f, c * c * c / 6.0);
+  p = __builtin_fma(p, f, c * c / 2.0);
+  p = __builtin_fma(p, f, c);
+  p = __builtin_fma(p, f, 1.0);
+  return bin < SM_BINS - 1 ? p * tab[bin] : 0.0;
 }
 // a number of [0, 2^43] to the nearest whole one
 __device__ __forceinline__ uint64_t whole(double w) {
@@ -179,20 +176,22 @@ __device__ __forceinline__ uint64_t mass_of(double t, int bin, const double *tab
 
 struct RowSet {
   bool greedy, k_on, p_on;
-  double invT;
+  double per;  // bins a unit of the logit: 32 / T
   int k;
   float p, minp;
+  double least;  // min_p as a weight
 };
 __device__ __forceinline__ RowSet row_set(const SampleArgs &a, int b) {
   RowSet s;
   const float T = a.temperature ? a.temperature[b] : 1.f;
   s.greedy = !(T > 0.f);
-  s.invT = s.greedy ? 1.0 : 1.0 / (double)T;
+  s.per = s.greedy ? 1.0 : (double)SM_PER / (double)T;
   s.k = a.top_k ? a.top_k[b] : 0;
   s.k_on = s.k > 0;
   s.p = a.top_p ? a.top_p[b] : 1.f;
   s.p_on = s.p < 1.f;
   s.minp = a.min_p ? a.min_p[b] : 0.f;
+  s.least = __builtin_ldexp((double)s.minp, SM_MASS_BITS);
   return s;
 }
 // whether the row needs the histogram
@@ -222,12 +221,24 @@ struct Add {
 struct Or {
   __device__ uint64_t operator()(uint64_t a, uint64_t b) const { return a | b; }
 };
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
-  const int lane = threadIdx.x & 63;
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t x = __shfl_up(v, o, 64);
-    if (lane >= o) v += x;
-  }
+// running sums over a wave: within rows of 16 lanes, then the rows before (DPP moves
+// on the vector unit; a shuffle through LDS per step takes four times as long)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp(uint64_t v) {
+  return (uint64_t)dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp<CTRL, ROWS>((uint32_t)v);
+}
+template <typename X>
+__device__ __forceinline__ X wave_scan(X v) {
+  v += dpp<0x111, 0xf>(v);
+  v += dpp<0x112, 0xf>(v);
+  v += dpp<0x114, 0xf>(v);
+  v += dpp<0x118, 0xf>(v);
+  v += dpp<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
+  v += dpp<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
   return v;
 }
 // running sum over the workgroup's threads, this one's value included
@@ -256,7 +267,8 @@ __device__ __forceinline__ uint64_t share(float p, uint64_t sum) {
 struct Bins {
   uint64_t cm[SM_BINS];  // running mass, bin included
   uint32_t cc[SM_BINS];  // running count
-  uint64_t sm[16], sn[16];
+  uint64_t sm[16];
+  uint32_t sn[16];
   int found[3];          // kbin, plo, phi
 };
 // The bins in which top-k and top-p cut, from a row's histogram (NT threads; mass and
@@ -265,8 +277,8 @@ template <int NT>
 __device__ RowState cut_bins(const RowSet &s, const uint64_t *mass, const uint32_t *count, Bins &S) {
   constexpr int PT = SM_BINS / NT;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  uint64_t mv[PT], ms = 0, ns = 0;
-  uint32_t nv[PT];
+  uint64_t mv[PT], ms = 0;
+  uint32_t nv[PT], ns = 0;
 #pragma unroll
   for (int i = 0; i < PT; ++i) {
     mv[i] = mass[tid * PT + i];
@@ -274,7 +286,8 @@ __device__ RowState cut_bins(const RowSet &s, const uint64_t *mass, const uint32
     ms += mv[i];
     ns += nv[i];
   }
-  uint64_t mc = wave_scan(ms), nc = wave_scan(ns);
+  uint64_t mc = wave_scan(ms);
+  uint32_t nc = wave_scan(ns);
   if (lane == 63) {
     S.sm[w] = mc;
     S.sn[w] = nc;
@@ -292,7 +305,7 @@ __device__ RowState cut_bins(const RowSet &s, const uint64_t *mass, const uint32
     mc += mv[i];
     nc += nv[i];
     S.cm[tid * PT + i] = mc;
-    S.cc[tid * PT + i] = (uint32_t)nc;
+    S.cc[tid * PT + i] = nc;
   }
   __syncthreads();
   const uint64_t total = S.cm[SM_BINS - 1];
@@ -321,7 +334,7 @@ __device__ RowState cut_bins(const RowSet &s, const uint64_t *mass, const uint32
   r.mass_p = r.plo > 0 ? S.cm[r.plo - 1] : 0;
   // all that can be kept lies in bins 0 .. last
   int last = r.plo >= 0 ? r.phi : r.kbin >= 0 ? r.kbin : SM_BINS - 1;
-  if (s.minp > 0.f) last = min(last, bin_of(log((double)fminf(s.minp, 1.f))) + 1);
+  if (s.minp > 0.f) last = min(last, bin_of(-(double)SM_PER * log((double)fminf(s.minp, 1.f))) + 1);
   r.last = S.cc[last] <= (uint32_t)SM_CAP ? last : -1;
   r.tau = 0;
   r.nlist = 0;
@@ -330,41 +343,45 @@ __device__ RowState cut_bins(const RowSet &s, const uint64_t *mass, const uint32
 }
 // Up to SM_RANK candidates (in any order), one a thread: how many of their bins lie
 // above one, and their mass, say where the cuts fall.
+struct Rank {
+  uint64_t key, mass;  // mass: bit 62 of kbin, bit 63 of plo .. phi
+};
 struct Ranks {
-  uint64_t key[SM_RANK], mass[SM_RANK];
-  uint32_t in[SM_RANK];  // 1: of kbin, 2: of plo .. phi
+  Rank at[SM_RANK];
   uint32_t n;
   uint64_t tau_k, above_k, tau_p;
 };
+constexpr uint64_t RANK_K = 1ull << 62, RANK_P = 1ull << 63, RANK_MASS = RANK_K - 1;
+// 1: of kbin, 2: of plo .. phi
 __device__ __forceinline__ uint32_t cut_of(const RowState &r, int bin) {
   return (bin == r.kbin ? 1u : 0u) | (r.plo >= 0 && bin >= r.plo && bin <= r.phi ? 2u : 0u);
 }
+// S.at[..].key holds the n candidates
 __device__ uint64_t cut_by_rank(const RowSet &s, const RowState &r, float m, const double *tab, Ranks &S) {
   const int tid = threadIdx.x, n = (int)S.n;
   uint64_t key = 0, q = 0;
   uint32_t in = 0;
   if (tid < n) {
-    key = S.key[tid];
-    const double t = scaled(z_of(key), m, s.invT);
-    const int bin = bin_of(t);
-    q = mass_of(t, bin, tab);
+    key = S.at[tid].key;
+    const double x = scaled(z_of(key), m, s.per);
+    const int bin = bin_of(x);
+    q = mass_of(x, bin, tab);
     in = cut_of(r, bin);
-    S.mass[tid] = q;
-    S.in[tid] = in;
+    S.at[tid].mass = q | (in & 1 ? RANK_K : 0) | (in & 2 ? RANK_P : 0);
   }
   if (tid == 0) S.tau_k = S.tau_p = S.above_k = 0;
   __syncthreads();
   uint64_t mk = 0, mp = 0;
   uint32_t ck = 0;
   if (tid < n) {
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < n; ++j) {
-      const bool over = S.key[j] > key;
-      const uint64_t qj = S.mass[j];
-      const uint32_t ij = S.in[j];
-      ck += over && (ij & 1);
-      mk += over && (ij & 1) ? qj : 0;
-      mp += over && (ij & 2) ? qj : 0;
+      const Rank o = S.at[j];
+      const bool over = o.key > key, k = over && (o.mass & RANK_K), p = over && (o.mass & RANK_P);
+      const uint64_t qj = o.mass & RANK_MASS;
+      ck += k;
+      mk += k ? qj : 0;
+      mp += p ? qj : 0;
     }
     if ((in & 1) && ck == r.r - 1) {
       S.tau_k = key;
@@ -459,7 +476,7 @@ __device__ uint64_t cut_by_radix(const All &all, const RowSet &s, const RowState
   uint64_t tau = 0, sum = r.total, above;
   const auto of = [&](uint32_t cut, bool mass, auto f) {
     all([&](uint64_t key) {
-      const double t = scaled(z_of(key), m, s.invT);
+      const double t = scaled(z_of(key), m, s.per);
       const int bin = bin_of(t);
       if (!(cut_of(r, bin) & cut)) return;
       const uint64_t q = mass_of(t, bin, tab);
@@ -477,13 +494,12 @@ __device__ uint64_t cut_by_radix(const All &all, const RowSet &s, const RowState
   return tau;
 }
 
-// the weight an element keeps, as a whole number
+// the weight an element keeps, as a whole number; no branch, so that a lane's
+// elements run beside each other
 __device__ __forceinline__ uint64_t kept(float z, int i, float m, const RowSet &s, uint64_t tau, const double *tab) {
-  if (!usable(z)) return 0;
-  if (z == m) return s.greedy || key_of(z, i) >= tau ? 1ull << SM_MASS_BITS : 0;
-  if (s.greedy || key_of(z, i) < tau) return 0;
-  const double t = scaled(z, m, s.invT), e = weight_of(t, bin_of(t), tab);
-  return e >= __builtin_ldexp((double)s.minp, SM_MASS_BITS) ? whole(e) : 0;
+  const double x = scaled(z, m, s.per), e = weight_of(x, bin_of(x), tab);
+  const bool top = z == m, in = usable(z) && key_of(z, i) >= tau && (top || (!s.greedy && e >= s.least));
+  return in ? (top ? 1ull << SM_MASS_BITS : whole(e)) : 0;
 }
 // the place of the draw in kept weights of sum W > 0
 __device__ __forceinline__ uint64_t draw_at(const RowSet &s, float u, uint64_t W) {
@@ -492,9 +508,9 @@ __device__ __forceinline__ uint64_t draw_at(const RowSet &s, float u, uint64_t W
 }
 
 // ---- rows of up to 16384 logits: every step in one workgroup --------------------
-// A thread's sixteen logits follow each other (runs of 17 words, for the banks), so
-// that a scan over the threads is one over the indexes.
-template <typename T, int NT>
+// A thread's E logits follow each other (runs of E + 1 words, for the banks), so that
+// a scan over the threads is one over the indexes.
+template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
   extern __shared__ float z[];
   __shared__ union {
@@ -510,11 +526,14 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
   const float u = a.u[b];
   const T *row = (const T *)a.z + (int64_t)b * a.stride;
   float m = -INFINITY;
-#pragma unroll 8
-  for (int e = 0; e < 16; ++e) {
+  T raw[E];  // all loads in flight, behind the row's end of its last logit
+#pragma unroll
+  for (int e = 0; e < E; ++e) raw[e] = row[min(e * NT + tid, a.V - 1)];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
     const int i = e * NT + tid;
-    const float v = i < a.V ? logit<T>(row[i]) : __uint_as_float(0x7fc00000u);
-    z[i + (i >> 4)] = v;
+    const float v = i < a.V ? logit<T>(raw[e]) : __uint_as_float(0x7fc00000u);
+    z[i + (i / E)] = v;
     m = fmaxf(m, v);  // passes NaN by
   }
   const bool cut = cuts(s);
@@ -524,30 +543,34 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
     S.bins.cc[i] = 0;
   }
   m = block_reduce(m, shf, Max());  // and a barrier for the rest
-  const float *mine = z + tid * 17;
+  float zr[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) zr[e] = z[tid * (E + 1) + e];
   uint64_t tau = 0;
   if (cut) {
     unsigned long long *hm = (unsigned long long *)S.bins.cm;
-#pragma unroll 4
-    for (int e = 0; e < 16; ++e)
-      if (usable(mine[e])) {
-        const double t = scaled(mine[e], m, s.invT);
-        const int bin = bin_of(t);
-        atomicAdd(&S.bins.cc[bin], 1u);
-        const uint64_t q = mass_of(t, bin, tab);
-        if (q) atomicAdd(&hm[bin], (unsigned long long)q);
-      }
+    int bin[E];  // -2: no logit to choose
+#pragma unroll
+    for (int e = 0; e < E; ++e) {  // no branch on the way: all chains at once
+      const double x = scaled(zr[e], m, s.per);
+      bin[e] = bin_of(x);
+      const uint64_t q = mass_of(x, bin[e], tab);
+      const bool ok = usable(zr[e]);
+      if (ok) atomicAdd(&S.bins.cc[bin[e]], 1u);
+      if (ok && q) atomicAdd(&hm[bin[e]], (unsigned long long)q);
+      bin[e] = ok ? bin[e] : -2;
+    }
     __syncthreads();
     const RowState r = cut_bins<NT>(s, S.bins.cm, S.bins.cc, S.bins);
     if (r.kbin >= 0 || r.plo >= 0) {
       __syncthreads();  // the bins are read, the ranks lie in their place
       if (tid == 0) S.ranks.n = 0;
       __syncthreads();
-#pragma unroll 4
-      for (int e = 0; e < 16; ++e)
-        if (usable(mine[e]) && cut_of(r, bin_of(scaled(mine[e], m, s.invT)))) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (cut_of(r, bin[e])) {
           const uint32_t at = atomicAdd(&S.ranks.n, 1u);
-          if (at < SM_RANK) S.ranks.key[at] = key_of(mine[e], tid * 16 + e);
+          if (at < SM_RANK) S.ranks.at[at].key = key_of(zr[e], tid * E + e);
         }
       __syncthreads();
       if (S.ranks.n <= SM_RANK) {
@@ -555,16 +578,20 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
       } else {
         __syncthreads();
         const auto all = [&](auto f) {
-          for (int e = 0; e < 16; ++e)
-            if (usable(mine[e])) f(key_of(mine[e], tid * 16 + e));
+#pragma unroll 1
+          for (int e = 0; e < E; ++e)
+            if (usable(z[tid * (E + 1) + e])) f(key_of(z[tid * (E + 1) + e], tid * E + e));
         };
         tau = cut_by_radix(all, s, r, m, tab, S.radix);
       }
     }
   }
-  uint64_t q = 0;
-#pragma unroll 4
-  for (int e = 0; e < 16; ++e) q += kept(mine[e], tid * 16 + e, m, s, tau, tab);
+  uint64_t k[E], q = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    k[e] = kept(zr[e], tid * E + e, m, s, tau, tab);
+    q += k[e];
+  }
   const uint64_t run = block_scan(q, sh);
   uint64_t W = 0;
   for (int i = 0; i < NT / 64; ++i) W += sh[i];
@@ -575,14 +602,15 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
   uint64_t t = draw_at(s, u, W);
   if (run > t && run - q <= t) {
     t -= run - q;
-    for (int e = 0; e < 16; ++e) {
-      const uint64_t k = kept(mine[e], tid * 16 + e, m, s, tau, tab);
-      if (k > t) {
-        a.ids[b] = tid * 16 + e;
-        break;
-      }
-      t -= k;
+    int e = 0;
+    bool more = true;
+#pragma unroll
+    for (int i = 0; i < E - 1; ++i) {
+      more = more && t >= k[i];
+      e += more;
+      t -= more ? k[i] : 0;
     }
+    a.ids[b] = tid * E + e;
   }
 }
 
@@ -626,14 +654,14 @@ __global__ __launch_bounds__(NT) void sample_hist_kernel(SampleArgs a, SampleWs 
   }
   __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 16; ++e)
-    if (usable(x.z[e])) {
-      const double t = scaled(x.z[e], m, s.invT);
-      const int bin = bin_of(t);
-      atomicAdd(&hc[bin], 1u);
-      const uint64_t q = mass_of(t, bin, tab);
-      if (q) atomicAdd(&hm[bin], (unsigned long long)q);
-    }
+  for (int e = 0; e < 16; ++e) {
+    const double d = scaled(x.z[e], m, s.per);
+    const int bin = bin_of(d);
+    const uint64_t q = mass_of(d, bin, tab);
+    const bool ok = usable(x.z[e]);
+    if (ok) atomicAdd(&hc[bin], 1u);
+    if (ok && q) atomicAdd(&hm[bin], (unsigned long long)q);
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < SM_BINS; i += NT)
     if (hc[i]) {
@@ -642,43 +670,42 @@ __global__ __launch_bounds__(NT) void sample_hist_kernel(SampleArgs a, SampleWs 
     }
 }
 
+// the bins in which a row's cuts fall
+__global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a, SampleWs w) {
+  __shared__ Bins S;
+  const int b = blockIdx.x;
+  const RowSet s = row_set(a, b);
+  if (!cuts(s)) return;
+  const RowState r = cut_bins<256>(s, w.mass + (int64_t)b * SM_BINS, w.count + (int64_t)b * SM_BINS, S);
+  if (threadIdx.x == 0) w.st[b] = r;
+}
+
 // the candidates into the row's list: all that can be kept where that is few, else
-// the elements of the bins in which top-k and top-p cut.  Every chunk finds the same
-// bins from the histogram.
+// the elements of the bins in which top-k and top-p cut
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_gather_kernel(SampleArgs a, SampleWs w, int vec) {
-  __shared__ Bins S;
   const int c = blockIdx.x, b = blockIdx.y;
   Lane<T> x;
   x.load((const T *)a.z + (int64_t)b * a.stride, c * NT * 16 + (threadIdx.x >> 6) * SM_WAVE, a.V, vec);
   const RowSet s = row_set(a, b);
   if (!cuts(s)) return;
+  const RowState r = w.st[b];
   const float m = row_max(w, b);
-  const RowState r = cut_bins<NT>(s, w.mass + (int64_t)b * SM_BINS, w.count + (int64_t)b * SM_BINS, S);
-  if (c == 0 && threadIdx.x == 0) {
-    RowState &o = w.st[b];  // all but tau, nlist and done
-    o.kbin = r.kbin;
-    o.plo = r.plo;
-    o.phi = r.phi;
-    o.last = r.last;
-    o.total = r.total;
-    o.mass_k = r.mass_k;
-    o.mass_p = r.mass_p;
-    o.r = r.r;
-  }
+  // logits below this lie behind every bin of interest, with half a bin and more of
+  // slack for the comparison in float32; most waves pass most of theirs by
+  const int deepest = max(max(r.last, r.kbin), r.phi);
+  const double edge = (double)m - ((double)deepest + 1.5) / s.per - fabs((double)m) * 0x1p-22;
+  const float least = edge > -3.4e38 && edge < 3.4e38 ? (float)edge : -INFINITY;
   uint32_t take = 0;  // this lane's candidates, a bit each
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int bin = bin_of(scaled(x.z[e], m, s.invT));
-    if (usable(x.z[e]) && (bin <= r.last || cut_of(r, bin))) take |= 1u << e;
-  }
+  for (int e = 0; e < 16; ++e)
+    if (x.z[e] >= least) {
+      const int bin = bin_of(scaled(x.z[e], m, s.per));
+      if (usable(x.z[e]) && (bin <= r.last || cut_of(r, bin))) take |= 1u << e;
+    }
   // a wave takes its places in the list at once
   const int mine = __popc(take), lane = threadIdx.x & 63;
-  int run = mine;
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(run, o, 64);
-    if (lane >= o) run += y;
-  }
+  const int run = (int)wave_scan((uint32_t)mine);
   const int all = __shfl(run, 63, 64);
   if (all == 0) return;
   uint32_t at = 0;
@@ -726,9 +753,9 @@ __global__ __launch_bounds__(512) void sample_cut_kernel(SampleArgs a, SampleWs 
   if (r.kbin >= 0 || r.plo >= 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (key[i] && cut_of(r, bin_of(scaled(z_of(key[i]), m, s.invT)))) {
+      if (key[i] && cut_of(r, bin_of(scaled(z_of(key[i]), m, s.per)))) {
         const uint32_t at = atomicAdd(&S.ranks.n, 1u);
-        if (at < SM_RANK) S.ranks.key[at] = key[i];
+        if (at < SM_RANK) S.ranks.at[at].key = key[i];
       }
     __syncthreads();
     if (listed && S.ranks.n <= SM_RANK) {
@@ -782,19 +809,17 @@ __global__ __launch_bounds__(512) void sample_cut_kernel(SampleArgs a, SampleWs 
     for (int i = 0; i < PER; ++i)
       if (q[i] && index(key[i]) >> shift == which) {
         const uint32_t at = atomicAdd(&S.ranks.n, 1u);
-        if (at < SM_RANK) {
-          S.ranks.key[at] = (uint64_t)index(key[i]);
-          S.ranks.mass[at] = q[i];
-        }
+        if (at < SM_RANK) S.ranks.at[at] = Rank{(uint64_t)index(key[i]), q[i]};
       }
     __syncthreads();
     const int k = (int)S.ranks.n;
     if (k <= SM_RANK) {
       if (tid < k) {
-        const uint64_t at = S.ranks.key[tid];
+        const Rank at = S.ranks.at[tid];
         uint64_t under = 0;
-        for (int j = 0; j < k; ++j) under += S.ranks.key[j] < at ? S.ranks.mass[j] : 0;
-        if (need >= under && need < under + S.ranks.mass[tid]) found = (uint32_t)at;
+#pragma unroll 8
+        for (int j = 0; j < k; ++j) under += S.ranks.at[j].key < at.key ? S.ranks.at[j].mass : 0;
+        if (need >= under && need < under + at.mass) found = (uint32_t)at.key;
       }
     } else {
       __syncthreads();
@@ -899,11 +924,11 @@ __global__ __launch_bounds__(256) void sample_pick_kernel(SampleArgs a, SampleWs
   }
 }
 
-template <typename T, int NT>
+template <typename T, int NT, int E>
 hipError_t sample_row(const SampleArgs &a, hipStream_t s) {
-  const int lds = NT * 17 * 4;
-  const auto fn = sample_row_kernel<T, NT>;
-  if (NT == 1024) {  // with its other arrays beyond 64 KiB
+  const int lds = NT * (E + 1) * 4;
+  const auto fn = sample_row_kernel<T, NT, E>;
+  if (E == 16) {  // with its other arrays beyond 64 KiB
     static std::atomic<int> set[kAttrDevices];
     const hipError_t e = ensure_lds_attr((const void *)fn, lds, set);
     if (e != hipSuccess) return e;
@@ -918,6 +943,7 @@ hipError_t sample_chunks(const SampleArgs &a, const SampleWs &w, hipStream_t s) 
   hipLaunchKernelGGL((sample_max_kernel<T, NT>), grid, dim3(NT), 0, s, a, w, vec);
   if (a.top_k || a.top_p) {
     hipLaunchKernelGGL((sample_hist_kernel<T, NT>), grid, dim3(NT), 0, s, a, w, vec);
+    hipLaunchKernelGGL(sample_bins_kernel, dim3(a.B), dim3(256), 0, s, a, w);
     hipLaunchKernelGGL((sample_gather_kernel<T, NT>), grid, dim3(NT), 0, s, a, w, vec);
     hipLaunchKernelGGL(sample_cut_kernel<T>, dim3(a.B), dim3(512), 0, s, a, w);
   }
@@ -927,9 +953,10 @@ hipError_t sample_chunks(const SampleArgs &a, const SampleWs &w, hipStream_t s) 
 }
 template <typename T>
 hipError_t sample_run(const SampleArgs &a, const SampleWs &w, hipStream_t s) {
-  if (a.V <= SM_ONE / 4) return sample_row<T, 256>(a, s);
-  if (a.V <= SM_ONE / 2) return sample_row<T, 512>(a, s);
-  if (a.V <= SM_ONE) return sample_row<T, 1024>(a, s);
+  // as many waves as hide the chains of float64 operations behind each other
+  if (a.V <= SM_ONE / 8) return sample_row<T, 256, 8>(a, s);
+  if (a.V <= SM_ONE / 2) return sample_row<T, 1024, 8>(a, s);
+  if (a.V <= SM_ONE) return sample_row<T, 1024, 16>(a, s);
   return w.waves == 4 ? sample_chunks<T, 256>(a, w, s) : sample_chunks<T, 1024>(a, w, s);
 }
 
