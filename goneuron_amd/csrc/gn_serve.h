@@ -31,7 +31,7 @@ struct KvAppendArgs {
   const float *cs, *sn;  // null: no rotation
   int rope_len, H;
   int touch;             // pages a sequence's new tokens can lie in
-  int qtok, qtiles;      // tokens of one rotation block, blocks a sequence
+  int qtiles;            // rotation blocks a sequence
   int vec;               // rows, tables and halves allow 4-value accesses
 };
 hipError_t launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s);

@@ -31,6 +31,12 @@ __device__ __forceinline__ float block_scale(float amax) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
+// a pair turned by an angle, in float64 and rounded once
+__device__ __forceinline__ void turn(float &x, float &y, float c, float s) {
+  const double a = (double)x * (double)c - (double)y * (double)s, b = (double)x * (double)s + (double)y * (double)c;
+  x = (float)a;
+  y = (float)b;
+}
 // four values of one token's head from column d on, rotated (rot) in float64 and
 // rounded once: products of two float32 are exact there, so every reader of
 // the definition gets the same float32.  Columns beyond hd are 0.
@@ -73,6 +79,7 @@ __device__ __forceinline__ void load_rotated(const T *row, const float *cs, cons
 }
 
 constexpr int KV_SLOTS = 8;  // four-value groups of new tokens a thread holds
+constexpr int KV_TURNS = 2;  // groups of four pairs of queries a thread turns
 
 // One workgroup per (sequence, touched page, kv head, K or V): it owns that
 // block, so its new maximum, the growth of its scale and the bytes of tokens
@@ -89,37 +96,47 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   const int limit0 = c.max_pages * c.P;
   const int limit = a.cs ? min(limit0, a.rope_len) : limit0;
   const int half = c.hd >> 1;
-  if ((int)blockIdx.x >= items) {  // queries: qtok tokens of one sequence
-    const int i = blockIdx.x - items, b = i / a.qtiles;
+  if ((int)blockIdx.x >= items) {  // queries: KV_TURNS groups of four pairs a thread
+    const int i = blockIdx.x - items, b = i / a.qtiles, tile = i % a.qtiles;
     const Seq s = kv_seq(c, b, limit);
-    const int t0 = (i % a.qtiles) * a.qtok, t1 = min(t0 + a.qtok, s.n);
     const T *q = (const T *)a.q;
     T *qo = (T *)a.qo;
-    const int per = (half + 3) >> 2, pairs = a.H * per;  // groups of four pairs
-    for (int g = tid; g < (t1 - t0) * pairs; g += NT) {
-      const int t = t0 + g / pairs, h = g % pairs / per, d = (g % per) * 4;
+    const int per = (half + 3) >> 2, row_groups = a.H * per;  // of a head, of a token
+    const int64_t g0 = (int64_t)tile * KV_TURNS * NT;
+    const int t0 = per ? (int)(g0 / row_groups) : s.n, first = per ? (int)(g0 % row_groups) : 0;
+#pragma unroll
+    for (int u = 0; u < KV_TURNS; ++u) {
+      const int gi = first + u * NT + tid, t = t0 + gi / max(row_groups, 1);
+      if (t >= s.n) break;
+      const int g = gi % row_groups, h = g / per, d = g % per * 4;
       const T *row = q + (int64_t)(s.start + t) * a.qs + h * c.hd;
       T *out = qo + (int64_t)(s.start + t) * a.qos + h * c.hd;
       const float *cs = a.cs ? a.cs + (int64_t)(s.len + t) * half : nullptr;
       const float *sn = a.cs ? a.sn + (int64_t)(s.len + t) * half : nullptr;
       float lo[4], hi[4];
       if (a.vec) {
-        load_rotated(row, cs, sn, c.hd, d, a.cs != nullptr, 1, lo);
-        load_rotated(row, cs, sn, c.hd, d + half, a.cs != nullptr, 1, hi);
+        Elem<T>::get4(row + d, lo);
+        Elem<T>::get4(row + d + half, hi);
+        if (a.cs) {
+          const float4 c4 = *reinterpret_cast<const float4 *>(cs + d), s4 = *reinterpret_cast<const float4 *>(sn + d);
+          const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) turn(lo[j], hi[j], cc[j], ss[j]);
+        }
         Elem<T>::put4(out + d, lo);
         Elem<T>::put4(out + d + half, hi);
       } else {
-        load_rotated(row, cs, sn, c.hd, d, a.cs != nullptr, 0, lo);
-        load_rotated(row, cs, sn, c.hd, d + half, a.cs != nullptr, 0, hi);
-        for (int j = 0; j < 4 && d + j < half; ++j) {
-          Elem<T>::put(out + d + j, lo[j]);
-          Elem<T>::put(out + d + j + half, hi[j]);
+        for (int j = d; j < min(d + 4, half); ++j) {
+          float x = Elem<T>::get(row + j), y = Elem<T>::get(row + j + half);
+          if (a.cs) turn(x, y, cs[j], sn[j]);
+          Elem<T>::put(out + j, x);
+          Elem<T>::put(out + j + half, y);
         }
       }
     }
-    if (c.hd & 1)  // the middle-less last column
-      for (int g = tid; g < (t1 - t0) * a.H; g += NT) {
-        const int t = t0 + g / a.H, h = g % a.H;
+    if (c.hd & 1)  // the last column has no partner; every tile takes its share of the rows
+      for (int64_t g = (int64_t)tile * NT + tid; g < (int64_t)s.n * a.H; g += (int64_t)a.qtiles * NT) {
+        const int t = (int)(g / a.H), h = (int)(g % a.H);
         Elem<T>::put(qo + (int64_t)(s.start + t) * a.qos + h * c.hd + c.hd - 1,
                      Elem<T>::get(q + (int64_t)(s.start + t) * a.qs + h * c.hd + c.hd - 1));
       }
@@ -137,15 +154,9 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   const int first = pi << c.lgP;                   // its first position
   const int lo = max(s.len - first, 0), hi = min(s.len + s.n - first, c.P);
   if (s.n == 0 || hi <= lo) return;
+  // the rows do not wait for the page, nor the old scale for the maximum
   const int page = c.table[(int64_t)b * c.max_pages + pi];
-  if (page < 0 || page >= c.pages) {
-    if (c.bad && tid == 0) c.bad[b] = 1;
-    return;
-  }
   const int R = c.R, P = c.P, per = R >> 2;
-  const int64_t blk = (int64_t)page * c.KVH + h;
-  uint8_t *dst = (which ? c.v : c.k) + blk * P * R;
-  float *sp = (which ? c.vs : c.ks) + blk;
   const bool rot = !which && a.cs;
   const T *x = (const T *)a.x[which] + h * c.hd;
   const int groups = (hi - lo) * per;
@@ -167,6 +178,14 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
       if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
     }
   }
+  if (page < 0 || page >= c.pages) {
+    if (c.bad && tid == 0) c.bad[b] = 1;
+    return;
+  }
+  const int64_t blk = (int64_t)page * c.KVH + h;
+  uint8_t *dst = (which ? c.v : c.k) + blk * P * R;
+  float *sp = (which ? c.vs : c.ks) + blk;
+  const float old = lo > 0 ? *sp : 0.f;
   // the block's maximum
   for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
   if (NT > 64) {
@@ -178,7 +197,6 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   }
   float scale = block_scale(amax);
   if (lo > 0) {
-    const float old = *sp;
     if (old > scale) {
       scale = old;
     } else if (old < scale) {  // the tokens already here move to the larger scale
@@ -255,10 +273,11 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   // a thread holds up to 32 new values of a block
   int nt = (most * c.R / (4 * KV_SLOTS) + 63) / 64 * 64;
   nt = nt < 64 ? 64 : nt;
-  const int half = c.hd / 2 > 0 ? c.hd / 2 : 1;
-  a.qtok = 8192 / (a.H * half);
-  a.qtok = a.qtok < 1 ? 1 : a.qtok > c.max_new ? c.max_new : a.qtok;
-  a.qtiles = (c.max_new + a.qtok - 1) / a.qtok;
+  // a thread with eight groups waited eight times for memory: 18 us for 256 tokens of
+  // 32 heads, where two take 6
+  const int64_t turns = (int64_t)c.max_new * a.H * ((c.hd / 2 + 3) / 4);
+  a.qtiles = (int)((turns + KV_TURNS * nt - 1) / (KV_TURNS * nt));
+  a.qtiles = a.qtiles < 1 ? 1 : a.qtiles;
   const int64_t blocks = (int64_t)c.B * a.touch * c.KVH * 2 + (a.qo ? (int64_t)c.B * a.qtiles : 0);
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   const size_t sh = most > 1 ? (size_t)c.R * (c.P + 16) : 0;
