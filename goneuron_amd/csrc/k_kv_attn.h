@@ -21,7 +21,9 @@ namespace {
 //
 // float32 queries are cut into three bf16 numbers (8 bits each, nothing lost), and
 // so are the weights: three products each, as exact as float32's.  bfloat16
-// queries take one, with the weights rounded to bf16.
+// queries take one; their weights are rounded to bf16 in prompts, whose time is the
+// products' (an output's error is then 1.4 times that of its own rounding), and cut
+// into two where the products wait for memory.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -119,7 +121,8 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
 // A wave's 16 RT rows.  Lane n + 16 g holds, for row n of a tile: the queries'
 // columns of its k slots, sixteen keys' scores of a step, and columns 4 g + i of
 // each 16 of the output.
-template <typename T, int R, int RT>
+// WPARTS: bf16 numbers that a weight is cut into.
+template <typename T, int R, int RT, int WPARTS>
 struct Rows {
   static constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
   static constexpr int NK = R / 32, ND = R / 16;
@@ -180,7 +183,7 @@ struct Rows {
   }
   // scores S (before the factor sf > 0) of tile r to weights, as the second
   // product's operands
-  __device__ __forceinline__ void weights(int r, const f32x4 (&S)[4], float sf, bf16x8 (&p)[2][PARTS]) {
+  __device__ __forceinline__ void weights(int r, const f32x4 (&S)[4], float sf, bf16x8 (&p)[2][WPARTS]) {
     float mx = -INFINITY;
 #pragma unroll
     for (int k = 0; k < 16; ++k) mx = fmaxf(mx, S[k >> 2][k & 3]);
@@ -203,9 +206,9 @@ struct Rows {
       float v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * h + (i >> 2)][i & 3], sf, sub));
-      to_parts<PARTS>(v, p[h]);
+      to_parts<WPARTS>(v, p[h]);
 #pragma unroll
-      for (int i = 0; i < PARTS; ++i)
+      for (int i = 0; i < WPARTS; ++i)
         L[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(ones), p[h][i], L[r], 0, 0, 0);
     }
   }
@@ -232,9 +235,9 @@ struct Rows {
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[r][step][p], S, 0, 0, 0);
   }
-  static __device__ __forceinline__ f32x4 product(const bf16x8 &v, const bf16x8 (&p)[PARTS], f32x4 o) {
+  static __device__ __forceinline__ f32x4 product(const bf16x8 &v, const bf16x8 (&p)[WPARTS], f32x4 o) {
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[i], o, 0, 0, 0);
+    for (int i = 0; i < WPARTS; ++i) o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[i], o, 0, 0, 0);
     return o;
   }
 
@@ -321,7 +324,8 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
   const int my_last = min(x.rows, row0 + 16 * RT) - 1;
   const int my_end = row0 >= x.rows ? 0 : a.causal ? x.s.len + my_last / a.G + 1 : x.total;
   const float sf = kv_factor(a.scale);
-  Rows<T, R, RT> A;
+  constexpr int WPARTS = sizeof(T) == 4 ? 3 : 1;
+  Rows<T, R, RT, WPARTS> A;
   A.init(a, x, row0, n, [&](int k) { return k * 32 + g * 8; });
 
   const int32_t *table = c.table + (int64_t)x.b * c.max_pages;
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
     } else {
       A.every = true;
     }
-    bf16x8 pf[RT][2][A.PARTS];
+    bf16x8 pf[RT][2][WPARTS];
 #pragma unroll
     for (int r = 0; r < RT; ++r) A.weights(r, S[r], sf, pf[r]);
     __builtin_amdgcn_sched_barrier(0);
@@ -528,7 +532,8 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
   if (!x.any) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, g = lane >> 4;
   const float factor = kv_factor(a.scale);
-  Rows<T, R, 1> A;
+  constexpr int WPARTS = sizeof(T) == 4 ? 3 : 2;  // the matrix units wait for memory here
+  Rows<T, R, 1, WPARTS> A;
   A.init(a, x, x.row0, n, [&](int k) { return k < R / 64 * 2 ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 : R / 64 * 64 + g * 8; });
 
   const int32_t *table = c.table + (int64_t)x.b * c.max_pages;
@@ -594,7 +599,7 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
       for (int k = 0; k < NK; ++k) A.scores(from_e4m3(kr[t][2 * k], kr[t][2 * k + 1], 1.f), k, 0, S[t]);
     }
     between();  // K's registers are free
-    bf16x8 pf[2][A.PARTS];
+    bf16x8 pf[2][WPARTS];
     const int see = CLEAN ? 16 : was_ok ? max(0, min(16, A.lim[0] - first + 1)) : 0;
     if constexpr (CLEAN) A.every = true;
     else A.mask(0, S, see);

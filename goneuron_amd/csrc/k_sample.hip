@@ -554,10 +554,12 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
     for (int e = 0; e < E; ++e) {  // no branch on the way: all chains at once
       const double x = scaled(zr[e], m, s.per);
       bin[e] = bin_of(x);
-      const uint64_t q = mass_of(x, bin[e], tab);
       const bool ok = usable(zr[e]);
       if (ok) atomicAdd(&S.bins.cc[bin[e]], 1u);
-      if (ok && q) atomicAdd(&hm[bin[e]], (unsigned long long)q);
+      if (s.p_on) {  // top-k alone goes by the counts
+        const uint64_t q = mass_of(x, bin[e], tab);
+        if (ok && q) atomicAdd(&hm[bin[e]], (unsigned long long)q);
+      }
       bin[e] = ok ? bin[e] : -2;
     }
     __syncthreads();
@@ -657,10 +659,12 @@ __global__ __launch_bounds__(NT) void sample_hist_kernel(SampleArgs a, SampleWs 
   for (int e = 0; e < 16; ++e) {
     const double d = scaled(x.z[e], m, s.per);
     const int bin = bin_of(d);
-    const uint64_t q = mass_of(d, bin, tab);
     const bool ok = usable(x.z[e]);
     if (ok) atomicAdd(&hc[bin], 1u);
-    if (ok && q) atomicAdd(&hm[bin], (unsigned long long)q);
+    if (s.p_on) {  // top-k alone goes by the counts
+      const uint64_t q = mass_of(d, bin, tab);
+      if (ok && q) atomicAdd(&hm[bin], (unsigned long long)q);
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < SM_BINS; i += NT)
@@ -692,10 +696,11 @@ __global__ __launch_bounds__(NT) void sample_gather_kernel(SampleArgs a, SampleW
   const RowState r = w.st[b];
   const float m = row_max(w, b);
   // logits below this lie behind every bin of interest, with half a bin and more of
-  // slack for the comparison in float32; most waves pass most of theirs by
+  // slack for the comparison in float32; most waves pass most of theirs by.  The last
+  // bin has no end.
   const int deepest = max(max(r.last, r.kbin), r.phi);
   const double edge = (double)m - ((double)deepest + 1.5) / s.per - fabs((double)m) * 0x1p-22;
-  const float least = edge > -3.4e38 && edge < 3.4e38 ? (float)edge : -INFINITY;
+  const float least = deepest < SM_BINS - 1 && edge > -3.4e38 && edge < 3.4e38 ? (float)edge : -INFINITY;
   uint32_t take = 0;  // this lane's candidates, a bit each
 #pragma unroll
   for (int e = 0; e < 16; ++e)
