@@ -864,6 +864,8 @@ __global__ __launch_bounds__(1024) void sample_cut_kernel(SampleArgs a, SampleWs
   }
   __syncthreads();
   Cuts r = cut_bins<NT>(s, m, masses, S.bins);
+  // top-p's share is of all that top-k keeps: its last bin is wanted too
+  if (r.plo >= 0 && r.kbin > r.last) r.last = -1;
   if (r.last >= 0) {  // at most SM_CAP logits, so no more groups of 16
     for (int i0 = 0; i0 < ngroup; i0 += AHEAD * NT) {
       uint32_t take = 0;

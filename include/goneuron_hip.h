@@ -626,7 +626,9 @@ int gn_mha_cached_forward(gn_ctx *ctx, const gn_kv_cache *kv, const float *x, co
  * equal logits go by the lowest index.  ids[b] is the first index, in rising
  * order, at which the kept weights' running sum exceeds u[b] times their sum; -1
  * for a row without a logit to choose.  A temperature that is not above 0 takes
- * the largest logit.  All settings are device arrays of B; temperature (1),
+ * the largest logit; beside an infinite logit finite ones weigh nothing.  A top_p
+ * that is NaN keeps all, a min_p that is NaN the largest.  All settings are device
+ * arrays of B; temperature (1),
  * top_k, top_p and min_p may be null.  Weights are float64 exponentials rounded
  * to whole multiples of 2^-43 and summed as integers, so a result does not
  * depend on any order of sums.  V <= 2^20.  work: gn_sample_workspace floats,

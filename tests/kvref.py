@@ -172,7 +172,8 @@ def sample(z, u, temperature=None, top_k=None, top_p=None, min_p=None):
     if not T > 0:
         return int(ok[z[ok] == m][0])
     with np.errstate(invalid="ignore", over="ignore"):
-        t = np.where(z[ok] == m, 0.0, (z[ok] - m) / T)
+        # an infinite distance stays one at an infinite temperature
+        t = np.where(z[ok] == m, 0.0, np.where(np.isinf(z[ok] - m), -np.inf, (z[ok] - m) / T))
     w = np.exp(t)
     order = np.argsort(-z[ok], kind="stable")
     if top_k is not None and top_k > 0:

@@ -128,6 +128,59 @@ def test_largest_vocabulary(dev):
     draw(dev, np.zeros((1, V)), [0.999], top_p=[0.7])
 
 
+@pytest.mark.parametrize("V", [2048, 2049, 8192, 8193, 16384, 16385, 262143, 262145])
+def test_sizes_at_which_the_way_changes(dev, V):
+    log(f"sample V={V}")
+    rng = np.random.default_rng(V)
+    B = 6
+    z, u = rng.normal(size=(B, V)) * 3, rng.random(B)
+    k = [1, 2047, 2048, 2049, min(V, 9000), 0]
+    for dtype in ("f32", "bf16"):
+        for kw in (dict(), dict(top_k=k), dict(top_p=[0.85] * B), dict(top_k=k, top_p=[0.85, 0.3, 0.99, 0.6, 0.9, 0.4]),
+                   dict(top_k=k, top_p=[0.9] * B, min_p=[0.05] * B), dict(top_k=k, min_p=[0.02] * B)):
+            draw(dev, z, u, dtype, **kw)
+
+
+@pytest.mark.parametrize("V", [5000, 20011, 70001])
+def test_more_equal_logits_than_a_list_of_candidates(dev, V):
+    log(f"sample ties V={V}")
+    rng = np.random.default_rng(V + 1)
+    z = np.zeros((6, V))
+    z[1] = rng.integers(0, 2, V)
+    z[2, V // 3] = 4.0
+    z[3] = np.where(np.arange(V) < V - 100, -1.0, -1.0 - 2.0 ** -20)
+    z[4] = -np.inf
+    z[4, ::2] = 2.5
+    z[5, :40] = np.linspace(1, 2, 40)
+    u = rng.random(6)
+    for k in (50, 2048, 4096):
+        for kw in (dict(), dict(min_p=[0.2] * 6)):
+            for q in (0.61, 0.999):
+                draw(dev, z, u, top_k=[k] * 6, top_p=[q] * 6, **kw)
+                draw(dev, z, u, "bf16", top_k=[k] * 6, top_p=[q] * 6, **kw)
+
+
+@pytest.mark.parametrize("V", [3001, 33333])
+def test_large_numbers_and_temperatures(dev, V):
+    """Grid lines far from zero, where float32 holds no single one of them."""
+    log(f"sample large V={V}")
+    rng = np.random.default_rng(V + 2)
+    z = rng.normal(size=(8, V)).astype(np.float32) * np.float32(3)
+    z[1] += np.float32(1e6)
+    z[2] -= np.float32(3e7)
+    z[3] *= np.float32(1e30)
+    z[4] *= np.float32(1e-30)
+    z[5] *= np.float32(1e-42)                     # denormal
+    z[6, rng.random(V) < 0.4] = -np.inf
+    z[6, 11] = np.nan
+    z[7, rng.integers(0, V, 3)] = np.inf
+    u = rng.random(8)
+    for T in (1.0, 0.01, 300.0, 1e-30, 1e-40, 1e30, np.inf):
+        for kw in (dict(), dict(top_k=[700] * 8), dict(top_p=[0.8] * 8), dict(min_p=[0.3] * 8),
+                   dict(top_k=[1500] * 8, top_p=[0.8] * 8, min_p=[1e-3] * 8), dict(top_k=[2500] * 8, top_p=[0.7] * 8)):
+            draw(dev, z, u, temperature=[T] * 8, **kw)
+
+
 def test_draws_follow_the_weights(dev):
     """One row drawn at many equally spaced u: each index as often as its weight says, to one draw."""
     z = np.log(np.array([0.1, 0.2, 0.05, 0.4, 0.25]))
