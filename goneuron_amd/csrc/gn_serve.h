@@ -7,6 +7,7 @@
 namespace gn {
 
 constexpr int KV_MAX_HEAD = 256;
+constexpr int KV_MAX_TOKENS = 0x7fffffff - 4096;  // of a sequence; of a call's (token, head) rows
 constexpr int KV_MAX_SCALE_EXP = -100;  // smallest block scale: 2^-100
 // the padded row of a head: what the kernels are built for
 inline int kv_row(int hd) {

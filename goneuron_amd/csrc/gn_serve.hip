@@ -14,6 +14,10 @@
 namespace {
 
 constexpr int64_t kMaxRows = (int64_t)1 << 26;
+// (token, query head) rows that the kernels count in 32 bits
+bool too_many_rows(int B, int max_new, int heads) {
+  return B > 0 && max_new > 0 && heads > KV_MAX_TOKENS / B / max_new;
+}
 
 int cache_check(gn_ctx *c, const gn_kv_cache *kv, KvArgs &a) {
   if (!kv || !kv->k || !kv->v || !kv->k_scale || !kv->v_scale || !kv->table)
@@ -23,7 +27,7 @@ int cache_check(gn_ctx *c, const gn_kv_cache *kv, KvArgs &a) {
   if (kv->head_dim < 1 || kv->head_dim > KV_MAX_HEAD)
     return set_err(c, GN_ERR_UNSUPPORTED, "kv cache: head size %d is not 1 to %d", kv->head_dim, KV_MAX_HEAD);
   if (kv->pages < 1 || kv->kv_heads < 1 || kv->max_pages < 1 ||
-      (int64_t)kv->max_pages * kv->page_size > 0x7fffffff - 4096)
+      (int64_t)kv->max_pages * kv->page_size > KV_MAX_TOKENS)
     return set_err(c, GN_ERR_INVALID, "kv cache: %d pages, %d heads, %d pages a sequence", kv->pages, kv->kv_heads,
                    kv->max_pages);
   if (((uintptr_t)kv->k | (uintptr_t)kv->v) & 15)
@@ -50,7 +54,7 @@ int batch_check(gn_ctx *c, KvArgs &a, const int32_t *starts, const int32_t *lens
   if (B < 0 || N < 0 || max_new < 0 || max_len < 0 || heads < 1 || heads % a.KVH)
     return set_err(c, GN_ERR_INVALID, "B %d, N %d, max_new %d, max_len %d, %d heads over %d", B, N, max_new, max_len,
                    heads, a.KVH);
-  if (B > 65535 || N > kMaxRows || heads > 65535 || (int64_t)B * max_new > kMaxRows)
+  if (B > 65535 || N > kMaxRows || heads > 65535 || (int64_t)B * max_new > kMaxRows || too_many_rows(B, max_new, heads))
     return set_err(c, GN_ERR_UNSUPPORTED, "B %d, N %d, max_new %d or %d heads beyond the launch limits", B, N, max_new, heads);
   a.starts = starts;
   a.lens = lens;
@@ -184,7 +188,7 @@ extern "C" int gn_kv_append(gn_ctx *c, const gn_kv_cache *kv, const void *q, con
 extern "C" int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max_len, int32_t heads, int32_t kv_heads,
                                          int32_t head_dim, int64_t *floats) {
   if (!floats || B < 0 || max_new < 0 || max_len < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 ||
-      head_dim > KV_MAX_HEAD)
+      head_dim > KV_MAX_HEAD || too_many_rows(B, max_new, heads))
     return GN_ERR_INVALID;
   *floats = kv_attn_work_floats(B, max_new, max_len, heads, kv_heads, head_dim);
   return GN_OK;
@@ -218,7 +222,7 @@ extern "C" int gn_kv_attention(gn_ctx *c, const gn_kv_cache *kv, const void *q, 
 extern "C" int gn_mha_cached_workspace(int32_t B, int32_t N, int32_t max_new, int32_t max_len, int32_t D, int32_t heads,
                                        int64_t *floats) {
   if (!floats || B < 0 || N < 0 || max_new < 0 || max_len < 0 || D < 1 || heads < 1 || D % heads ||
-      D / heads > KV_MAX_HEAD)
+      D / heads > KV_MAX_HEAD || too_many_rows(B, max_new, heads))
     return GN_ERR_INVALID;
   *floats = 4 * (((int64_t)N * D + 63) / 64 * 64) +
             kv_attn_work_floats(B, max_new, max_len, heads, heads, D / heads);

@@ -276,8 +276,8 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   // a thread with eight groups waited eight times for memory: 18 us for 256 tokens of
   // 32 heads, where two take 6
   const int64_t turns = (int64_t)c.max_new * a.H * ((c.hd / 2 + 3) / 4);
-  a.qtiles = (int)((turns + KV_TURNS * nt - 1) / (KV_TURNS * nt));
-  a.qtiles = a.qtiles < 1 ? 1 : a.qtiles;
+  const int64_t qtiles = (turns + KV_TURNS * nt - 1) / (KV_TURNS * nt);  // below 2^31: rows are
+  a.qtiles = qtiles < 1 ? 1 : (int)qtiles;
   const int64_t blocks = (int64_t)c.B * a.touch * c.KVH * 2 + (a.qo ? (int64_t)c.B * a.qtiles : 0);
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   const size_t sh = most > 1 ? (size_t)c.R * (c.P + 16) : 0;

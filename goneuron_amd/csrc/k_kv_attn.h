@@ -113,7 +113,7 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
   const int last = min(x.rows, x.row0 + pl.rows_wg) - 1;
   x.end = a.causal ? x.s.len + max(last, 0) / a.G + 1 : x.total;
   x.k0 = x.split * pl.chunk;
-  x.k1 = min(x.k0 + pl.chunk, x.end);
+  x.k1 = x.end - x.k0 < pl.chunk ? x.end : x.k0 + pl.chunk;  // the sum alone could pass 32 bits
   x.any = x.row0 < x.rows && (x.split == 0 || x.k0 < x.end);
   return x;
 }
@@ -709,7 +709,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void kv_join_kernel(
   const int wg_last = min(s.n * a.G, wg0 + pl.rows_wg) - 1;
   const int wg_end = a.causal ? s.len + wg_last / a.G + 1 : s.len + s.n;
   if (wg_end <= pl.chunk) return;
-  const int n = (wg_end + pl.chunk - 1) / pl.chunk;
+  const int n = (wg_end - 1) / pl.chunk + 1;
   const float *ml = a.work + slot * 2;
   // the maximum over all splits; l of a split whose scores are all -inf is NaN
   float M = -INFINITY;

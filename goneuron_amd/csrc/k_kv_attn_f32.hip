@@ -19,11 +19,12 @@ static KvPlan kv_plan(int B, int max_new, int max_len, int H, int KVH, int R, in
   // least.
   const int64_t items = (int64_t)B * KVH * p.tiles, unit = p.by_rows ? 64 : 256;
   int64_t splits = p.by_rows ? 512 / items : std::min<int64_t>(4096 / items, 64);
-  splits = std::min(splits, max_len / (p.by_rows ? 128 : 512) + 0l);
+  const int64_t len = std::min(std::max(max_len, 1), KV_MAX_TOKENS);  // no table holds more
+  splits = std::min(splits, len / (p.by_rows ? 128 : 512));
   splits = std::max<int64_t>(splits, 1);
-  const int64_t chunk = (std::max(max_len, 1) + splits - 1) / splits;
+  const int64_t chunk = (len + splits - 1) / splits;
   p.chunk = (int)((chunk + unit - 1) / unit * unit);
-  p.splits = (std::max(max_len, 1) + p.chunk - 1) / p.chunk;
+  p.splits = (int)((len + p.chunk - 1) / p.chunk);
   return p;
 }
 

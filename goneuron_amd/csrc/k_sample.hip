@@ -95,7 +95,7 @@ size_t sample_carve(char *base, int B, int V, SampleWs *w) {
     t.gmax = (float *)take((size_t)B * t.C * t.waves * 64 * 4);
   }
   if (w) *w = t;
-  return off;
+  return off ? off : 64;  // callers hand over some workspace whatever the size
 }
 
 template <typename T>

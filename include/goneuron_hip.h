@@ -536,7 +536,9 @@ int gn_moe_backward(gn_ctx *ctx, const float *x, const float *params, const floa
  * starts[b + 1] - 1 (starts: B + 1 int32) of the inputs and outputs, at the
  * positions lens[b], lens[b] + 1, ... (lens: B int32, the tokens cached before
  * the call; the caller advances it after the step).  A sequence may have no
- * new token; rows outside every sequence are neither read nor written. */
+ * new token; rows outside every sequence are neither read nor written.  B and
+ * heads are 65535 at most, N and B * max_new 2^26, a sequence's tokens and B *
+ * max_new * heads 2^31 - 4097. */
 #define GN_DTYPE_F32 0
 #define GN_DTYPE_BF16 1
 
@@ -595,9 +597,10 @@ int gn_kv_append(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, const void *
  * in dtype.  max_len: an upper bound of lens[b] + new tokens, from which (with
  * max_new) the work is split; a sequence beyond it is skipped.  Sums and
  * maxima are float32; the products of float32 queries have float32's precision,
- * those of bfloat16 ones may round the weights to bfloat16.  Tokens in pages outside [0,
- * pages) are left out; a query that sees none gives 0.  bad as above.  work:
- * gn_kv_attention_workspace floats for the same sizes, 16-byte aligned (may be
+ * those of bfloat16 ones may round the weights to bfloat16.  Tokens in pages
+ * outside [0, pages) are left out; a query that sees none gives 0.  A NaN that a
+ * query sees, in its keys or values, makes its output NaN; one that it does not see
+ * is nothing to it.  bad as above.  work: gn_kv_attention_workspace floats for the same sizes, 16-byte aligned (may be
  * 0: then work may be null). */
 int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max_len, int32_t heads, int32_t kv_heads,
                               int32_t head_dim, int64_t *floats);
@@ -610,7 +613,8 @@ int gn_kv_attention(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out
  * gn_mha_forward's; Q, K, V of the new tokens, rotated where cos and sin are
  * given (gn_rope_tables), K and V appended, causal attention over the cache, wOut.
  * kv->kv_heads x kv->head_dim must be D.  With all tokens at once and empty sequences it
- * computes gn_mha_forward's causal layer, keys and values rounded to 8 bits. */
+ * computes gn_mha_forward's causal layer, keys and values rounded to 8 bits.  Rows
+ * outside every sequence, and of a sequence that is skipped, get wOut's bias. */
 int gn_mha_cached_workspace(int32_t B, int32_t N, int32_t max_new, int32_t max_len, int32_t D, int32_t heads,
                             int64_t *floats);
 int gn_mha_cached_forward(gn_ctx *ctx, const gn_kv_cache *kv, const float *x, const float *params, float *out,
@@ -628,10 +632,9 @@ int gn_mha_cached_forward(gn_ctx *ctx, const gn_kv_cache *kv, const float *x, co
  * for a row without a logit to choose.  A temperature that is not above 0 takes
  * the largest logit; beside an infinite logit finite ones weigh nothing.  A top_p
  * that is NaN keeps all, a min_p that is NaN the largest.  All settings are device
- * arrays of B; temperature (1),
- * top_k, top_p and min_p may be null.  Weights are float64 exponentials rounded
- * to whole multiples of 2^-43 and summed as integers, so a result does not
- * depend on any order of sums.  V <= 2^20.  work: gn_sample_workspace floats,
+ * arrays of B; temperature (1), top_k, top_p and min_p may be null.  Weights are
+ * float64 exponentials rounded to whole multiples of 2^-43 and summed as integers,
+ * so a result does not depend on any order of sums.  V <= 2^20.  work: gn_sample_workspace floats,
  * 8-byte aligned. */
 int gn_sample_workspace(int32_t B, int32_t V, int64_t *floats);
 int gn_sample(gn_ctx *ctx, const void *logits, int64_t stride, int32_t dtype, const float *temperature,

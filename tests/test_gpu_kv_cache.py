@@ -552,3 +552,73 @@ def test_generating_steps_together(dev):
         for b in range(B):
             assert ids[b] == kvref.sample(z[b], u[b], T[b], k[b], p[b])
             tokens[b].append(int(ids[b]))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 3]])
+def test_attention_with_loose_bounds(dev, new):
+    """Lengths' bounds far beyond the sequences, up to the largest number there is."""
+    for max_len in (5000, 2 ** 30, 2 ** 31 - 1):
+        attention_case(dev, "bf16", 64, 16, 2, 2, [77, 0], new, 1, max_len=max_len)
+
+
+def test_more_rows_than_32_bits_count(dev):
+    L, _ = _lib()
+    n = C.c_int64()
+    assert L.gn_kv_attention_workspace(1, 1 << 20, 64, 4096, 1, 32, C.byref(n)) == -1
+    assert L.gn_mha_cached_workspace(64, 1, 1 << 20, 64, 64, 64, C.byref(n)) == -1
+    ref = kvref.Cache(4, 16, 2, 32, np.arange(4).reshape(1, 4), np.random.default_rng(1))
+    on = OnDevice(dev, ref)
+    x, i = DBuf(dev, np.zeros(4096, np.float32)), DBuf(dev, np.zeros(8, np.int32))
+    w = 4096 * 32
+    assert L.gn_kv_attention(dev.h, C.byref(on.kv), x.p, x.p, w, w, i.p, i.p, 1, 1, 1 << 20, 64, 4096, 1.0, 1, 0, x.p, None) == -4
+    assert L.gn_kv_append(dev.h, C.byref(on.kv), x.p, x.p, x.p, x.p, w, w, w, w, None, None, 0, i.p, i.p, 1, 1, 1 << 20, 4096, 0,
+                          None) == -4
+
+
+def test_two_contexts_at_once(gn, dev):
+    """Two streams append to caches of their own, attend over them and draw, their work
+    queued in turn without a wait between."""
+    other = gn.HIPDevice(0)
+    try:
+        on_two_streams(dev, other)   # its buffers go before their context
+    finally:
+        other.close()
+
+
+def on_two_streams(dev, other):
+    L, check = _lib()
+    rng = np.random.default_rng(9)
+    hd, kvh, H, P, T = 64, 2, 8, 32, 200
+    V = 20000
+    runs = []
+    for d in (dev, other):
+        ref = kvref.Cache(10, P, kvh, hd, rng.permutation(10)[:8].reshape(1, 8).astype(np.int32), rng)
+        on = OnDevice(d, ref)
+        k, v, q = (rng.normal(size=(T, n * hd)).astype(np.float32) for n in (kvh, kvh, H))
+        n = C.c_int64()
+        check(None, L.gn_kv_attention_workspace(1, T, 256, H, kvh, hd, C.byref(n)))
+        work = DBuf(d, np.full(max(1, n.value), np.nan, np.float32))
+        check(None, L.gn_sample_workspace(1, V, C.byref(n)))
+        draw = DBuf(d, np.full(n.value, np.nan, np.float32))
+        z = rng.normal(size=(1, V)).astype(np.float32) * 3
+        runs.append(dict(d=d, ref=ref, on=on, host=(k, v, q), k=DBuf(d, k), v=DBuf(d, v), q=DBuf(d, q),
+                         out=DBuf(d, np.zeros((T, H * hd), np.float32)), st=DBuf(d, np.array([0, T], np.int32)),
+                         ln=DBuf(d, np.zeros(1, np.int32)), work=work, draw=draw, z=z, dz=DBuf(d, z),
+                         u=DBuf(d, np.array([0.37], np.float32)), p=DBuf(d, np.array([0.9], np.float32)),
+                         ids=DBuf(d, np.full(1, -7, np.int32))))
+    for r in runs:
+        check(r["d"].h, L.gn_kv_append(r["d"].h, C.byref(r["on"].kv), None, r["k"].p, r["v"].p, None, 0, kvh * hd, kvh * hd, 0,
+                                       None, None, 0, r["st"].p, r["ln"].p, 1, T, T, H, F32, None))
+    for _ in range(3):
+        for r in runs:
+            check(r["d"].h, L.gn_kv_attention(r["d"].h, C.byref(r["on"].kv), r["q"].p, r["out"].p, H * hd, H * hd, r["st"].p,
+                                              r["ln"].p, 1, T, T, 256, H, 0.125, 1, F32, r["work"].p, None))
+            check(r["d"].h, L.gn_sample(r["d"].h, r["dz"].p, V, F32, None, None, r["p"].p, None, r["u"].p, r["ids"].p, 1, V,
+                                        r["draw"].p))
+    for r in runs:
+        k, v, q = r["host"]
+        r["ref"].append(0, 0, k.reshape(T, kvh, hd), v.reshape(T, kvh, hd))
+        want, size, lost = kvref.attend(r["ref"], 0, 0, q.reshape(T, H, hd).astype(np.float64), 0.125, 1)
+        got = r["out"].get().reshape(T, H, hd).astype(np.float64)
+        assert (np.abs(got - want) <= kvref.bound(want, size, lost, T, "f32")).all()
+        assert int(r["ids"].get()[0]) == kvref.sample(r["z"][0].astype(np.float64), np.float32(0.37), top_p=np.float32(0.9))
