@@ -311,6 +311,9 @@ __device__ __forceinline__ int v_place(int row, int chunk) { return chunk ^ ((ro
 // step's K and V bytes are loaded a step ahead, turned into bf16 once for all
 // waves (scales included, keys behind the sequence 0) and read as operands from
 // LDS; two steps' operands lie there, so one barrier a step is enough.
+// Bound by the matrix units and what feeds them: two prompts of 2048 tokens behind
+// 2048, 32 heads of 128 over 8, bfloat16, in 241 us, 849 TFLOP/s (a product of 16384^3
+// reaches 1369 here); the units are 40 % busy, the waves wait for LDS and the barrier.
 template <typename T, int R, int RT>
 __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int NK = R / 32, ND = R / 16;
@@ -522,6 +525,9 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
 // operands come straight from memory into the lanes that need them: four times
 // the loads in flight for one set of rows, and no barrier until the waves are
 // joined through LDS.
+// Bound by memory: one sequence of 131072 tokens, 8 key heads of 128, in 58 us with its
+// join, 4.6 TB/s of cache (45 us alone with 64 splits: 6.0, as fast as memory is read
+// here); 64 sequences of up to 8192 in 122 us, 4.4 TB/s.  A step of 5 us at the least.
 template <typename T, int R>
 __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void kv_attn_keys_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int NK = R / 32, ND = R / 16;
