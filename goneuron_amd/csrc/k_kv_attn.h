@@ -526,8 +526,8 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
 // the loads in flight for one set of rows, and no barrier until the waves are
 // joined through LDS.
 // Bound by memory: one sequence of 131072 tokens, 8 key heads of 128, in 58 us with its
-// join, 4.6 TB/s of cache (45 us alone with 64 splits: 6.0, as fast as memory is read
-// here); 64 sequences of up to 8192 in 122 us, 4.4 TB/s.  A step of 5 us at the least.
+// join, 4.6 TB/s of cache (44 us alone: 6.1, as fast as memory is read here); 64
+// sequences of up to 8192 in 122 us, 4.4 TB/s.  A step of 5 us at the least.
 template <typename T, int R>
 __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void kv_attn_keys_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int NK = R / 32, ND = R / 16;

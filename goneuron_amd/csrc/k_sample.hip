@@ -1162,7 +1162,11 @@ hipError_t sample_run(const SampleArgs &a, const SampleWs &w, hipStream_t s) {
 
 }  // namespace
 
-int64_t sample_work_floats(int B, int V) { return (int64_t)(sample_carve(nullptr, B, V, nullptr) / 4); }
+// enough for fewer rows too, which may be cut into smaller and more chunks
+int64_t sample_work_floats(int B, int V) {
+  const int fewer = std::min(B, 2048 / std::max(1, (V + 4 * SM_WAVE - 1) / (4 * SM_WAVE)));
+  return (int64_t)(std::max(sample_carve(nullptr, B, V, nullptr), sample_carve(nullptr, fewer, V, nullptr)) / 4);
+}
 
 hipError_t launch_sample(const SampleArgs &a, int dtype, hipStream_t s) {
   SampleWs w{};

@@ -600,8 +600,9 @@ int gn_kv_append(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, const void *
  * those of bfloat16 ones may round the weights to bfloat16.  Tokens in pages
  * outside [0, pages) are left out; a query that sees none gives 0.  A NaN that a
  * query sees, in its keys or values, makes its output NaN; one that it does not see
- * is nothing to it.  bad as above.  work: gn_kv_attention_workspace floats for the same sizes, 16-byte aligned (may be
- * 0: then work may be null). */
+ * is nothing to it.  bad as above.  work: gn_kv_attention_workspace floats for the
+ * same sizes, 16-byte aligned (may be 0: then work may be null); fewer sequences are
+ * split further and may need more. */
 int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max_len, int32_t heads, int32_t kv_heads,
                               int32_t head_dim, int64_t *floats);
 int gn_kv_attention(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,
@@ -634,8 +635,8 @@ int gn_mha_cached_forward(gn_ctx *ctx, const gn_kv_cache *kv, const float *x, co
  * that is NaN keeps all, a min_p that is NaN the largest.  All settings are device
  * arrays of B; temperature (1), top_k, top_p and min_p may be null.  Weights are
  * float64 exponentials rounded to whole multiples of 2^-43 and summed as integers,
- * so a result does not depend on any order of sums.  V <= 2^20.  work: gn_sample_workspace floats,
- * 8-byte aligned. */
+ * so a result does not depend on any order of sums.  V <= 2^20.  work: gn_sample_workspace floats
+ * for V and as many rows or more, 8-byte aligned. */
 int gn_sample_workspace(int32_t B, int32_t V, int64_t *floats);
 int gn_sample(gn_ctx *ctx, const void *logits, int64_t stride, int32_t dtype, const float *temperature,
               const int32_t *top_k, const float *top_p, const float *min_p, const float *u, int32_t *ids, int32_t B,

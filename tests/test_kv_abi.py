@@ -53,3 +53,12 @@ def test_null_context(L):
     assert L.gn_sample(None, None, 0, 0, *[None] * 6, 1, 1, None) == -1
     assert L.gn_rope_tables(None, None, None, 1, 2) == -1
     assert L.gn_model_sample(None, None, 1, *[None] * 6) == -1
+
+
+@pytest.mark.parametrize("V", [8000, 16385, 20001, 131072, 262145, 1 << 20])
+def test_sampling_workspace_serves_fewer_rows(L, V):
+    n, last = C.c_int64(), 0
+    for B in list(range(1, 600)) + [1000, 2047, 2048, 2049, 5000, 65535]:
+        assert L.gn_sample_workspace(B, V, C.byref(n)) == 0
+        assert n.value >= last
+        last = n.value
