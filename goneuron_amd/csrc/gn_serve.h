@@ -33,6 +33,7 @@ struct KvAppendArgs {
   int rope_len, H;
   int touch;             // pages a sequence's new tokens can lie in
   int qtiles;            // rotation blocks a sequence
+  uint32_t per_inv, group_inv, pair_inv;  // inverses of a query head's groups, a row's, a key head's pairs of them
   int vec;               // rows, tables and halves allow 4-value accesses
 };
 hipError_t launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s);

@@ -17,6 +17,14 @@ __device__ __forceinline__ uint32_t to_e4m3(float x, float inv) {
   const uint32_t b = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x * inv, 0.f, 0, false) & 0xff;
   return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? 0x7fu : b;
 }
+// four of them
+__device__ __forceinline__ uint32_t to_e4m3(float x, float y, float z, float w, float inv) {
+  const uint32_t most = max(max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu),
+                            max(__float_as_uint(z) & 0x7fffffffu, __float_as_uint(w) & 0x7fffffffu));
+  if (most >= 0x7f800000u) return to_e4m3(x, inv) | to_e4m3(y, inv) << 8 | to_e4m3(z, inv) << 16 | to_e4m3(w, inv) << 24;
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x * inv, y * inv, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z * inv, w * inv, lo, true);
+}
 // a stored byte under a larger scale; NaN stays
 __device__ __forceinline__ uint32_t rescaled(uint32_t byte, float ratio) {
   if ((byte & 0x7f) == 0x7f) return byte;
@@ -42,28 +50,8 @@ __device__ __forceinline__ void turn(float &x, float &y, float c, float s) {
 // the definition gets the same float32.  Columns beyond hd are 0.
 template <typename T>
 __device__ __forceinline__ void load_rotated(const T *row, const float *cs, const float *sn, int hd, int d, bool rot,
-                                             int vec, float (&o)[4]) {
+                                             float (&o)[4]) {
   const int half = hd >> 1;
-  if (vec) {  // hd a multiple of 8: the four and their partners lie on one side of the middle
-    if (d >= hd) {
-      o[0] = o[1] = o[2] = o[3] = 0.f;
-      return;
-    }
-    Elem<T>::get4(row + d, o);
-    if (!rot) return;
-    const bool up = d >= half;
-    float p[4];
-    Elem<T>::get4(row + (up ? d - half : d + half), p);
-    const float4 c4 = *reinterpret_cast<const float4 *>(cs + (up ? d - half : d));
-    const float4 s4 = *reinterpret_cast<const float4 *>(sn + (up ? d - half : d));
-    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const double a = (double)o[i] * (double)c[i], b = (double)p[i] * (double)s[i];
-      o[i] = (float)(up ? b + a : a - b);
-    }
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int j = d + i;
@@ -78,6 +66,10 @@ __device__ __forceinline__ void load_rotated(const T *row, const float *cs, cons
   }
 }
 
+// g / n by ceil(2^32 / n), exact while g n < 2^32: a division takes twenty times as long
+__device__ __forceinline__ int divided(int g, uint32_t inv, int n) { return n == 1 ? g : (int)__umulhi((uint32_t)g, inv); }
+inline uint32_t inverse(int n) { return n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / n) : 0; }
+
 constexpr int KV_SLOTS = 8;  // four-value groups of new tokens a thread holds
 constexpr int KV_TURNS = 2;  // groups of four pairs of queries a thread turns
 
@@ -86,9 +78,11 @@ constexpr int KV_TURNS = 2;  // groups of four pairs of queries a thread turns
 // already there need no other workgroup.  New values stay in registers between
 // the maximum and the rounding.  Blocks behind those rotate the queries.
 // Bound by latency for single tokens (a chain of table, row and scale reads, one
-// reduction: 9.4 us for a bfloat16 token of 256 sequences, 32 query heads and 8 key
+// reduction: 10 us for a bfloat16 token of 256 sequences, 32 query heads and 8 key
 // heads of 128, whose 5.9 MB a copy moves in 1.2) and by memory for prompts (six of up to
-// 2048: 51 us for 163 MB, 3.2 TB/s; a copy reaches 4.9).
+// 2048: 45 us for 163 MB, 3.6 TB/s, where a copy reaches 4.9).  Prompts also wait for the
+// vector unit: indexes without divisions, pairs turned once and bytes rounded two at a
+// time brought them from 60.
 template <typename T>
 __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
@@ -108,9 +102,16 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
     const int t0 = per ? (int)(g0 / row_groups) : s.n, first = per ? (int)(g0 % row_groups) : 0;
 #pragma unroll
     for (int u = 0; u < KV_TURNS; ++u) {
-      const int gi = first + u * NT + tid, t = t0 + gi / max(row_groups, 1);
+      int g = first + u * NT + tid, t = t0;
+      if (row_groups >= KV_TURNS * NT) {  // one token's end at most lies between
+        t += g >= row_groups;
+        g -= g >= row_groups ? row_groups : 0;
+      } else if (per) {
+        t += g / row_groups;
+        g %= row_groups;
+      }
       if (t >= s.n) break;
-      const int g = gi % row_groups, h = g / per, d = g % per * 4;
+      const int h = divided(g, a.per_inv, per), d = (g - h * per) * 4;
       const T *row = q + (int64_t)(s.start + t) * a.qs + h * c.hd;
       T *out = qo + (int64_t)(s.start + t) * a.qos + h * c.hd;
       const float *cs = a.cs ? a.cs + (int64_t)(s.len + t) * half : nullptr;
@@ -161,25 +162,84 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   const int R = c.R, P = c.P, per = R >> 2;
   const bool rot = !which && a.cs;
   const T *x = (const T *)a.x[which] + h * c.hd;
-  const int groups = (hi - lo) * per;
+  // Of a whole page of V a thread takes four columns of eight tokens, which it can
+  // store by itself; of K both halves of a pair, so that a pair is read and turned
+  // once.
+  const bool tall = a.vec && which && hi - lo == P, pairs = a.vec && !which;
+  // the token and column of this thread's u-th group of four; false: none
+  const auto place = [&](int u, int &t, int &d) {
+    if (tall) {
+      t = (tid & ((P >> 3) - 1)) * 8 + u;
+      d = (tid >> (c.lgP - 3)) * 4;
+      return d < R;
+    }
+    const int n = pairs ? c.hd >> 3 : per, g = tid + (pairs ? u >> 1 : u) * NT, q = divided(g, pairs ? a.pair_inv : a.group_inv, n);
+    t = lo + q;
+    d = (g - q * n) * 4 + (pairs && (u & 1) ? half : 0);
+    return t < hi;
+  };
 
   float v[KV_SLOTS][4];
-  float amax = 0.f;
+  const T *xs = x + (int64_t)(s.start + first - s.len) * a.xs[which];
+  // No branch between the loads, all of them under way at once: 45 us for the prompts
+  // below.  Leaving out those that a single token does not need saved it 0.3 of 10 us,
+  // but took registers that cost the prompts 7.
+  if (a.vec) {
 #pragma unroll
-  for (int u = 0; u < KV_SLOTS; ++u) {
-    const int g = tid + u * NT;
-    if (g >= groups) break;
-    const int t = lo + g / per, d = (g % per) * 4;
-    const int pos = first + t;
-    const T *row = x + (int64_t)(s.start + pos - s.len) * a.xs[which];
-    load_rotated(row, rot ? a.cs + (int64_t)pos * half : nullptr, rot ? a.sn + (int64_t)pos * half : nullptr, c.hd, d, rot,
-                 a.vec, v[u]);
+    for (int u = 0; u < KV_SLOTS; ++u) {
+      int t, d;
+      const bool on = place(u, t, d) && d < c.hd;
+      Elem<T>::get4(xs + (on ? t : lo) * a.xs[which] + (on ? d : 0), v[u]);
+    }
+    if (rot) {
+      float4 cs[KV_SLOTS / 2], sn[KV_SLOTS / 2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float m = fabsf(v[u][k]);
-      if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
+      for (int u = 0; u < KV_SLOTS; u += 2) {
+        int t, d;
+        const bool on = place(u, t, d);
+        const int64_t at = (int64_t)(first + (on ? t : lo)) * half + (on ? d : 0);
+        cs[u / 2] = *reinterpret_cast<const float4 *>(a.cs + at);
+        sn[u / 2] = *reinterpret_cast<const float4 *>(a.sn + at);
+      }
+#pragma unroll
+      for (int u = 0; u < KV_SLOTS; u += 2) {
+        const float4 c4 = cs[u / 2], s4 = sn[u / 2];
+        turn(v[u][0], v[u + 1][0], c4.x, s4.x);
+        turn(v[u][1], v[u + 1][1], c4.y, s4.y);
+        turn(v[u][2], v[u + 1][2], c4.z, s4.z);
+        turn(v[u][3], v[u + 1][3], c4.w, s4.w);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < KV_SLOTS; ++u) {
+      int t, d;
+      const bool on = place(u, t, d) && d < c.hd;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[u][k] = on ? v[u][k] : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < KV_SLOTS; ++u) {
+      int t, d;
+      if (!place(u, t, d)) break;
+      const int64_t pos = first + t;
+      load_rotated(xs + t * a.xs[which], rot ? a.cs + pos * half : nullptr, rot ? a.sn + pos * half : nullptr, c.hd, d, rot,
+                   v[u]);
     }
   }
+  const auto largest = [&](auto of) {
+    float m = 0.f;
+#pragma unroll
+    for (int u = 0; u < KV_SLOTS; ++u) {
+      int t, d;
+      if (!place(u, t, d)) break;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m = fmaxf(m, of(fabsf(v[u][k])));  // passes NaN by
+    }
+    return m;
+  };
+  float amax = largest([](float y) { return y; });
+  if (amax == INFINITY) amax = largest([](float y) { return y == INFINITY ? 0.f : y; });
   if (page < 0 || page >= c.pages) {
     if (c.bad && tid == 0) c.bad[b] = 1;
     return;
@@ -225,37 +285,51 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   if (!which) {
 #pragma unroll
     for (int u = 0; u < KV_SLOTS; ++u) {
-      const int g = tid + u * NT;
-      if (g >= groups) break;
-      reinterpret_cast<uint32_t *>(dst + (int64_t)lo * R)[g] = to_e4m3(v[u][0], inv) | to_e4m3(v[u][1], inv) << 8 |
-                                                               to_e4m3(v[u][2], inv) << 16 | to_e4m3(v[u][3], inv) << 24;
+      int t, d;
+      if (!place(u, t, d)) break;
+      *reinterpret_cast<uint32_t *>(dst + t * R + d) = to_e4m3(v[u][0], v[u][1], v[u][2], v[u][3], inv);
+    }
+    const int pad = (R - c.hd) >> 2;
+    if (pairs && pad)  // the rows' ends, which no pair covers
+      for (int g = tid; g < (hi - lo) * pad; g += NT)
+        *reinterpret_cast<uint32_t *>(dst + (lo + g / pad) * R + c.hd + g % pad * 4) = 0;
+    return;
+  }
+  if (tall) {
+    int t, d;
+    if (!place(0, t, d) || d >= c.hd) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint2 w;
+      w.x = to_e4m3(v[0][k], v[1][k], v[2][k], v[3][k], inv);
+      w.y = to_e4m3(v[4][k], v[5][k], v[6][k], v[7][k], inv);
+      *reinterpret_cast<uint2 *>(dst + (d + k) * P + t) = w;
     }
     return;
   }
   if (hi - lo == 1) {  // one token: a byte of every row
 #pragma unroll
     for (int u = 0; u < KV_SLOTS; ++u) {
-      const int g = tid + u * NT;
-      if (g >= groups) break;
+      int t, d;
+      if (!place(u, t, d)) break;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (g * 4 + k < c.hd) dst[(int64_t)(g * 4 + k) * P + lo] = (uint8_t)to_e4m3(v[u][k], inv);
+        if (d + k < c.hd) dst[(d + k) * P + lo] = (uint8_t)to_e4m3(v[u][k], inv);
     }
     return;
   }
   const int LP = P + 16;  // rows stay 16-byte aligned
 #pragma unroll
   for (int u = 0; u < KV_SLOTS; ++u) {
-    const int g = tid + u * NT;
-    if (g >= groups) break;
-    const int t = lo + g / per, d = (g % per) * 4;
+    int t, d;
+    if (!place(u, t, d)) break;
 #pragma unroll
     for (int k = 0; k < 4; ++k) lds[(d + k) * LP + t] = (uint8_t)to_e4m3(v[u][k], inv);
   }
   __syncthreads();
   const int seg = P >> 4;
   for (int g = tid; g < c.hd * seg; g += NT) {
-    const int d = g / seg, t = (g % seg) * 16;
+    const int d = g >> (c.lgP - 4), t = (g & (seg - 1)) * 16;
     if (t + 16 <= lo || t >= hi) continue;
     if (t >= lo && t + 16 <= hi) {
       *reinterpret_cast<uint4 *>(dst + (int64_t)d * P + t) = *reinterpret_cast<const uint4 *>(lds + d * LP + t);
@@ -280,6 +354,9 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   const int64_t turns = (int64_t)c.max_new * a.H * ((c.hd / 2 + 3) / 4);
   const int64_t qtiles = (turns + KV_TURNS * nt - 1) / (KV_TURNS * nt);  // below 2^31: rows are
   a.qtiles = qtiles < 1 ? 1 : (int)qtiles;
+  a.per_inv = inverse((c.hd / 2 + 3) / 4);
+  a.group_inv = inverse(c.R / 4);
+  a.pair_inv = inverse(c.hd / 8);
   const int64_t blocks = (int64_t)c.B * a.touch * c.KVH * 2 + (a.qo ? (int64_t)c.B * a.qtiles : 0);
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   const size_t sh = most > 1 ? (size_t)c.R * (c.P + 16) : 0;
