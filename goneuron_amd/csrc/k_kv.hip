@@ -350,7 +350,7 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   int nt = (most * c.R / (4 * KV_SLOTS) + 63) / 64 * 64;
   nt = nt < 64 ? 64 : nt;
   // a thread with eight groups waits eight times for memory: 17 us for 256 tokens of
-  // 32 heads of 128, where two take 9.4
+  // 32 heads of 128, where two take 10
   const int64_t turns = (int64_t)c.max_new * a.H * ((c.hd / 2 + 3) / 4);
   const int64_t qtiles = (turns + KV_TURNS * nt - 1) / (KV_TURNS * nt);  // below 2^31: rows are
   a.qtiles = qtiles < 1 ? 1 : (int)qtiles;
