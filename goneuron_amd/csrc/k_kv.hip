@@ -70,7 +70,8 @@ __device__ __forceinline__ void load_rotated(const T *row, const float *cs, cons
 __device__ __forceinline__ int divided(int g, uint32_t inv, int n) { return n == 1 ? g : (int)__umulhi((uint32_t)g, inv); }
 inline uint32_t inverse(int n) { return n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / n) : 0; }
 
-constexpr int KV_SLOTS = 8;  // four-value groups of new tokens a thread holds
+constexpr int KV_MANY = 8;  // four-value groups of new tokens a thread holds, of single tokens
+constexpr int KV_ONE = 2;
 constexpr int KV_TURNS = 2;  // groups of four pairs of queries a thread turns
 
 // One workgroup per (sequence, touched page, kv head, K or V): it owns that
@@ -78,12 +79,12 @@ constexpr int KV_TURNS = 2;  // groups of four pairs of queries a thread turns
 // already there need no other workgroup.  New values stay in registers between
 // the maximum and the rounding.  Blocks behind those rotate the queries.
 // Bound by latency for single tokens (a chain of table, row and scale reads, one
-// reduction: 10 us for a bfloat16 token of 256 sequences, 32 query heads and 8 key
+// reduction: 9.5 us for a bfloat16 token of 256 sequences, 32 query heads and 8 key
 // heads of 128, whose 5.9 MB a copy moves in 1.2) and by memory for prompts (six of up to
 // 2048: 45 us for 163 MB, 3.6 TB/s, where a copy reaches 4.9).  Prompts also wait for the
 // vector unit: indexes without divisions, pairs turned once and bytes rounded two at a
 // time brought them from 60.
-template <typename T>
+template <typename T, int KV_SLOTS>
 __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
   const KvArgs &c = a.c;
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   // Of a whole page of V a thread takes four columns of eight tokens, which it can
   // store by itself; of K both halves of a pair, so that a pair is read and turned
   // once.
-  const bool tall = a.vec && which && hi - lo == P, pairs = a.vec && !which;
+  const bool tall = KV_SLOTS == KV_MANY && a.vec && which && hi - lo == P, pairs = a.vec && !which;
   // the token and column of this thread's u-th group of four; false: none
   const auto place = [&](int u, int &t, int &d) {
     if (tall) {
@@ -181,9 +182,7 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
 
   float v[KV_SLOTS][4];
   const T *xs = x + (int64_t)(s.start + first - s.len) * a.xs[which];
-  // No branch between the loads, all of them under way at once: 45 us for the prompts
-  // below.  Leaving out those that a single token does not need saved it 0.3 of 10 us,
-  // but took registers that cost the prompts 7.
+  // no branch between the loads: all of them under way at once
   if (a.vec) {
 #pragma unroll
     for (int u = 0; u < KV_SLOTS; ++u) {
@@ -300,9 +299,10 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
     if (!place(0, t, d) || d >= c.hd) return;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      constexpr int L = KV_SLOTS - 1;  // no slot beyond: single tokens are not tall
       uint2 w;
-      w.x = to_e4m3(v[0][k], v[1][k], v[2][k], v[3][k], inv);
-      w.y = to_e4m3(v[4][k], v[5][k], v[6][k], v[7][k], inv);
+      w.x = to_e4m3(v[0][k], v[1][k], v[min(2, L)][k], v[min(3, L)][k], inv);
+      w.y = to_e4m3(v[min(4, L)][k], v[min(5, L)][k], v[min(6, L)][k], v[L][k], inv);
       *reinterpret_cast<uint2 *>(dst + (d + k) * P + t) = w;
     }
     return;
@@ -347,10 +347,10 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   const int most = c.max_new < c.P ? c.max_new : c.P;
   a.touch = (c.max_new + 2 * c.P - 2) / c.P;
   // a thread holds up to 32 new values of a block
-  int nt = (most * c.R / (4 * KV_SLOTS) + 63) / 64 * 64;
+  int nt = (most * c.R / (4 * KV_MANY) + 63) / 64 * 64;
   nt = nt < 64 ? 64 : nt;
   // a thread with eight groups waits eight times for memory: 17 us for 256 tokens of
-  // 32 heads of 128, where two take 10
+  // 32 heads of 128, where two take 9.5
   const int64_t turns = (int64_t)c.max_new * a.H * ((c.hd / 2 + 3) / 4);
   const int64_t qtiles = (turns + KV_TURNS * nt - 1) / (KV_TURNS * nt);  // below 2^31: rows are
   a.qtiles = qtiles < 1 ? 1 : (int)qtiles;
@@ -360,10 +360,12 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   const int64_t blocks = (int64_t)c.B * a.touch * c.KVH * 2 + (a.qo ? (int64_t)c.B * a.qtiles : 0);
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   const size_t sh = most > 1 ? (size_t)c.R * (c.P + 16) : 0;
-  if (dtype == GN_DTYPE_F32)
-    hipLaunchKernelGGL(kv_append_kernel<float>, dim3((unsigned)blocks), dim3(nt), sh, s, a);
-  else
-    hipLaunchKernelGGL(kv_append_kernel<uint16_t>, dim3((unsigned)blocks), dim3(nt), sh, s, a);
+  // single tokens fill two groups of a thread at most: loads of eight took 6.1 us where
+  // theirs take 4 (a token of 4 sequences, 8 heads of 32)
+  const bool one = c.max_new == 1;
+  auto fn = one ? kv_append_kernel<float, KV_ONE> : kv_append_kernel<float, KV_MANY>;
+  if (dtype != GN_DTYPE_F32) fn = one ? kv_append_kernel<uint16_t, KV_ONE> : kv_append_kernel<uint16_t, KV_MANY>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(nt), sh, s, a);
   return hipGetLastError();
 }
 
