@@ -16,14 +16,16 @@ namespace {
 // keys of a step are dealt to the four 16-row tiles of K so that a lane's sixteen
 // scores belong to sixteen keys in a row of its group of 16: the operand P^T
 // of the second product then is the first one's result in place, and V^T's operand
-// 16 consecutive bytes of a row of the transposed cache.  K, V, P and O pass
-// through registers only; a row's maximum and sum live in its four lanes.
+// 16 consecutive bytes of a row of the transposed cache.  P and O pass through
+// registers only, for single tokens K and V too; a row's maximum and sum live in its
+// four lanes.
 //
 // float32 queries are cut into three bf16 numbers (8 bits each, nothing lost), and
 // so are the weights: three products each, as exact as float32's.  bfloat16
-// queries take one; their weights are rounded to bf16 in prompts, whose time is the
-// products' (an output's error is then 1.4 times that of its own rounding), and cut
-// into two where the products wait for memory.
+// queries take one and their weights are cut into two (16 bits: off by less than 2^-15
+// of themselves), so that an output's error is its own rounding's.  Weights of one
+// number would take 241 us where two take 307 (the prompts below), with an error
+// against 64 bits of 0.0023 where rounding alone makes 0.0017.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -42,8 +44,8 @@ __device__ __forceinline__ bf16x8 from_e4m3(uint32_t lo, uint32_t hi, float scal
 __device__ __forceinline__ uint32_t pack_high(float lo, float hi) {  // the upper halves of two float32
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
-// PARTS bf16 numbers that sum to each of eight float32: rounded (1) or cut at 8
-// bits, the rest cut again (3)
+// PARTS bf16 numbers that sum to each of eight float32: rounded (1), or cut at 8
+// bits, the rest cut again (2, 3)
 template <int PARTS>
 __device__ __forceinline__ void to_parts(const float (&v)[8], bf16x8 (&o)[PARTS]) {
   if constexpr (PARTS == 1) {
@@ -121,10 +123,10 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
 // A wave's 16 RT rows.  Lane n + 16 g holds, for row n of a tile: the queries'
 // columns of its k slots, sixteen keys' scores of a step, and columns 4 g + i of
 // each 16 of the output.
-// WPARTS: bf16 numbers that a weight is cut into.
-template <typename T, int R, int RT, int WPARTS>
+template <typename T, int R, int RT>
 struct Rows {
-  static constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
+  // bf16 numbers that a query and a weight are cut into
+  static constexpr int PARTS = sizeof(T) == 4 ? 3 : 1, WPARTS = sizeof(T) == 4 ? 3 : 2;
   static constexpr int NK = R / 32, ND = R / 16;
   bf16x8 q[RT][NK][PARTS];
   f32x4 O[RT][ND], L[RT];  // outputs; sums, as a product with ones (four equal rows)
@@ -312,8 +314,9 @@ __device__ __forceinline__ int v_place(int row, int chunk) { return chunk ^ ((ro
 // waves (scales included, keys behind the sequence 0) and read as operands from
 // LDS; two steps' operands lie there, so one barrier a step is enough.
 // Bound by the matrix units and what feeds them: two prompts of 2048 tokens behind
-// 2048, 32 heads of 128 over 8, bfloat16, in 241 us, 849 TFLOP/s (a product of 16384^3
-// reaches 1369 here); the units are 40 % busy, the waves wait for LDS and the barrier.
+// 2048, 32 heads of 128 over 8, bfloat16, in 307 us, 206 GFLOP at 672 TFLOP/s of the
+// definition's products and, the weights' second part among them, 1007 of the units' (a
+// product of 16384^3 reaches 1369 here); the waves wait for LDS and the barrier.
 template <typename T, int R, int RT>
 __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int NK = R / 32, ND = R / 16;
@@ -327,8 +330,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
   const int my_last = min(x.rows, row0 + 16 * RT) - 1;
   const int my_end = row0 >= x.rows ? 0 : a.causal ? x.s.len + my_last / a.G + 1 : x.total;
   const float sf = kv_factor(a.scale);
-  constexpr int WPARTS = sizeof(T) == 4 ? 3 : 1;
-  Rows<T, R, RT, WPARTS> A;
+  Rows<T, R, RT> A;
   A.init(a, x, row0, n, [&](int k) { return k * 32 + g * 8; });
 
   const int32_t *table = c.table + (int64_t)x.b * c.max_pages;
@@ -471,7 +473,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
     } else {
       A.every = true;
     }
-    bf16x8 pf[RT][2][WPARTS];
+    bf16x8 pf[RT][2][A.WPARTS];
 #pragma unroll
     for (int r = 0; r < RT; ++r) A.weights(r, S[r], sf, pf[r]);
     __builtin_amdgcn_sched_barrier(0);
@@ -538,8 +540,7 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
   if (!x.any) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, g = lane >> 4;
   const float factor = kv_factor(a.scale);
-  constexpr int WPARTS = sizeof(T) == 4 ? 3 : 2;  // the matrix units wait for memory here
-  Rows<T, R, 1, WPARTS> A;
+  Rows<T, R, 1> A;
   A.init(a, x, x.row0, n, [&](int k) { return k < R / 64 * 2 ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 : R / 64 * 64 + g * 8; });
 
   const int32_t *table = c.table + (int64_t)x.b * c.max_pages;
@@ -605,7 +606,7 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
       for (int k = 0; k < NK; ++k) A.scores(from_e4m3(kr[t][2 * k], kr[t][2 * k + 1], 1.f), k, 0, S[t]);
     }
     between();  // K's registers are free
-    bf16x8 pf[2][WPARTS];
+    bf16x8 pf[2][A.WPARTS];
     const int see = CLEAN ? 16 : was_ok ? max(0, min(16, A.lim[0] - first + 1)) : 0;
     if constexpr (CLEAN) A.every = true;
     else A.mask(0, S, see);

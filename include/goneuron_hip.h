@@ -597,7 +597,7 @@ int gn_kv_append(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, const void *
  * in dtype.  max_len: an upper bound of lens[b] + new tokens, from which (with
  * max_new) the work is split; a sequence beyond it is skipped.  Sums and
  * maxima are float32; the products of float32 queries have float32's precision,
- * those of bfloat16 ones may round the weights to bfloat16.  Tokens in pages
+ * the weights of bfloat16 ones keep 16 bits.  Tokens in pages
  * outside [0, pages) are left out; a query that sees none gives 0.  A NaN that a
  * query sees, in its keys or values, makes its output NaN; one that it does not see
  * is nothing to it.  bad as above.  work: gn_kv_attention_workspace floats for the
