@@ -55,13 +55,18 @@ struct KvPlan {
   int rt, rows_wg;    // 16-row tiles of a wave, rows of a workgroup
   bool by_rows;       // the workgroup's waves take rows of their own (else keys)
   int tiles;
+  bool work;          // the splits meet in the caller's workspace (else, if any, in the context's scratch)
 };
+// Single tokens of sequences of up to this length need no workspace of the caller's: their
+// splits are few enough for the context's scratch.
+constexpr int KV_SHORT = 4096;
 // padded heads up to this size leave registers for two 16-row tiles a wave
 constexpr int kv_two_tiles(int bytes) { return bytes == 4 ? 64 : 128; }
 // the workspace: (maximum, sum) of every split's rows, then their outputs
 __host__ __device__ inline int64_t kv_part_at(int splits, int64_t slots) { return (splits * slots * 2 + 3) / 4 * 4; }
 int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd);
-hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, hipStream_t s);
+bool kv_attn_uses_work(const KvArgs &c, int H, int dtype);  // whether a call of these very sizes does
+hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, float *scratch, int64_t scratch_floats, hipStream_t s);
 hipError_t launch_kv_attn_bf16(const KvAttnArgs &a, const KvPlan &p, hipStream_t s);
 
 struct SampleArgs {

@@ -122,7 +122,7 @@ int attn_impl(gn_ctx *c, const KvArgs &kv, const void *q, void *out, int64_t qs,
   a.work = work;
   // the cache's lengths are on the device: the bound stands for them
   KTimer kt(c, GN_KCLASS_OTHER, "kv_attention", 2.0 * kv.B * kv.max_len * (double)kv.KVH * kv.hd);
-  HIP_OK(c, launch_kv_attn(a, dtype, c->stream));
+  HIP_OK(c, launch_kv_attn(a, dtype, c->scratch, (int64_t)c->scratch_floats, c->stream));
   return GN_OK;
 }
 
@@ -208,7 +208,7 @@ extern "C" int gn_kv_attention(gn_ctx *c, const gn_kv_cache *kv, const void *q, 
   if (B == 0 || N == 0 || max_new == 0) return GN_OK;
   const int64_t w = (int64_t)heads * a.hd;
   if ((rc = row_check(c, "q", q, q_stride, w, dtype)) || (rc = row_check(c, "out", out, out_stride, w, dtype))) return rc;
-  if (!work && kv_attn_work_floats(B, max_new, max_len, heads, a.KVH, a.hd) > 0)
+  if (!work && kv_attn_uses_work(a, heads, dtype))
     return set_err(c, GN_ERR_INVALID, "kv_attention needs its workspace");
   if ((uintptr_t)work & 15) return set_err(c, GN_ERR_INVALID, "kv_attention: work must be 16-byte aligned");
   return attn_impl(c, a, q, out, q_stride, out_stride, heads, scale, causal, dtype, work);

@@ -600,9 +600,10 @@ int gn_kv_append(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, const void *
  * the weights of bfloat16 ones keep 16 bits.  Tokens in pages
  * outside [0, pages) are left out; a query that sees none gives 0.  A NaN that a
  * query sees, in its keys or values, makes its output NaN; one that it does not see
- * is nothing to it.  bad as above.  work: gn_kv_attention_workspace floats for the
- * same sizes, 16-byte aligned (may be 0: then work may be null); fewer sequences are
- * split further and may need more. */
+ * is nothing to it.  bad as above.  work: gn_kv_attention_workspace floats, 16-byte
+ * aligned (may be 0: then work may be null).  What it asks for serves every call with the
+ * same heads whose B, max_new and max_len are no larger, so that a program asks once for
+ * its largest sizes. */
 int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max_len, int32_t heads, int32_t kv_heads,
                               int32_t head_dim, int64_t *floats);
 int gn_kv_attention(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,
@@ -615,7 +616,8 @@ int gn_kv_attention(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out
  * given (gn_rope_tables), K and V appended, causal attention over the cache, wOut.
  * kv->kv_heads x kv->head_dim must be D.  With all tokens at once and empty sequences it
  * computes gn_mha_forward's causal layer, keys and values rounded to 8 bits.  Rows
- * outside every sequence, and of a sequence that is skipped, get wOut's bias. */
+ * outside every sequence, and of a sequence that is skipped, get wOut's bias.  work:
+ * gn_mha_cached_workspace floats for B, N, max_new and max_len as large or larger. */
 int gn_mha_cached_workspace(int32_t B, int32_t N, int32_t max_new, int32_t max_len, int32_t D, int32_t heads,
                             int64_t *floats);
 int gn_mha_cached_forward(gn_ctx *ctx, const gn_kv_cache *kv, const float *x, const float *params, float *out,

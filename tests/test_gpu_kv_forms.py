@@ -61,3 +61,61 @@ def test_bf16_prompts_are_as_good_as_their_rounding(dev, hd, G, past, new):
     over = np.abs(got - want) / lim
     log(f"{over.max():.3f} of the bound")
     assert over.max() <= 1
+
+
+def test_one_workspace_for_every_smaller_call(dev):
+    """The workspace of the largest sizes, with a border of marks behind it, and calls of
+    fewer sequences, new tokens and tokens in it."""
+    L, check = _lib()
+    rng = np.random.default_rng(21)
+    kvh, G, hd = 2, 2, 64
+    heads, scale = kvh * G, 0.125
+    ref = filled(rng, 64, kvh, hd, [8300, 700, 4200, 40])
+    on = OnDevice(dev, ref)
+    floats = attention_floats(4, 70, 8300, heads, kvh, hd)
+    assert floats > 0
+    work = DBuf(dev, np.full(floats + 4096, 3.25, np.float32))
+    for B, new, bound in ((4, 1, 8300), (4, 1, 8192), (3, 1, 4400), (1, 1, 8300), (1, 1, 8192), (1, 8, 8200), (2, 9, 8300),
+                          (1, 32, 8300), (1, 33, 8192), (2, 64, 8300), (4, 70, 8300), (1, 70, 8300)):
+        log(f"attention in a larger workspace: B={B} new={new} max_len={bound}")
+        total = [min(n, bound) for n in (8300, 700, 4200, 40)][:B]
+        if new > min(total):
+            total[total.index(min(total))] = new
+        past = [t - new for t in total]
+        q, q64 = as_dtype(rng.normal(size=(B * new, heads * hd)), "f32")
+        dq, do, st = DBuf(dev, q), DBuf(dev, q * 0), DBuf(dev, starts_of([new] * B))
+        ln = DBuf(dev, np.asarray(past, np.int32))
+        check(dev.h, L.gn_kv_attention(dev.h, C.byref(on.kv), dq.p, do.p, heads * hd, heads * hd, st.p, ln.p, B, B * new, new, bound,
+                                       heads, scale, 1, F32, work.p, None))
+        assert (work.get()[floats:] == 3.25).all()
+        got = do.get().astype(np.float64).reshape(B, new, heads, hd)
+        for b in range(B):  # the first and the last of the new tokens
+            for t in {0, new - 1}:
+                want, size, lost = kvref.attend(ref, b, past[b] + t, q64.reshape(B, new, heads, hd)[b, t:t + 1], scale, 1)
+                near = np.abs(got[b, t] - want[0]) <= kvref.bound(want, size, lost, total[b], "f32")[0]
+                # where a call looks behind what was appended, to pages without a scale: NaN on both sides
+                assert (near | (np.isnan(got[b, t]) & np.isnan(want[0]))).all(), (b, t)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_splits_that_the_scratch_does_not_hold(dev, dtype):
+    """512 sequences of one key head of 256 with 16 query heads, told to be up to 4096 long:
+    their splits would take more than the context's scratch, so they are not split."""
+    L, check = _lib()
+    rng = np.random.default_rng(22)
+    B, G, hd = 512, 16, 256
+    lens = [1 + b % 5 for b in range(B)]
+    lens[7] = 300
+    ref = filled(rng, 16, 1, hd, lens)
+    on = OnDevice(dev, ref)
+    assert attention_floats(B, 1, 4096, G, 1, hd) == 0
+    q, q64 = as_dtype(rng.normal(size=(B, G * hd)), dtype)
+    dq, do, st = DBuf(dev, q), DBuf(dev, q * 0), DBuf(dev, np.arange(B + 1, dtype=np.int32))
+    ln = DBuf(dev, np.asarray(lens, np.int32) - 1)
+    for bound in (4096, 4000, 3000):
+        check(dev.h, L.gn_kv_attention(dev.h, C.byref(on.kv), dq.p, do.p, G * hd, G * hd, st.p, ln.p, B, B, 1, bound, G, 0.0625, 1,
+                                       F32 if dtype == "f32" else BF16, None, None))
+        got = values(do.get(), dtype).reshape(B, G, hd)
+        for b in list(range(0, B, 37)) + [7, B - 1]:
+            want, size, lost = kvref.attend(ref, b, lens[b] - 1, q64.reshape(B, 1, G, hd)[b], 0.0625, 1)
+            assert (np.abs(got[b] - want[0]) <= kvref.bound(want, size, lost, lens[b], dtype)[0]).all(), (bound, b)
