@@ -43,22 +43,21 @@ struct Elem<uint16_t> {
 };
 
 // A sequence as the call's arrays describe it; n = 0 where there is nothing to
-// do.  bad: its bounds lie outside the inputs or the table, or it is larger
-// than the sizes the launch was made for.
+// do.  bad: its bounds lie outside the inputs or the call's limit, or it has more
+// new tokens than the launch was made for.
 struct Seq {
   int start, n, len;
   bool bad;
 };
-__device__ __forceinline__ Seq kv_seq(const KvArgs &c, int b, int limit) {
+__device__ __forceinline__ Seq kv_seq(const KvArgs &c, int b) {
   Seq s;
   s.start = c.starts[b];
   const int end = c.starts[b + 1];
   s.len = c.lens[b];
   s.bad = s.start < 0 || end < s.start || end > c.N || end - s.start > c.max_new || s.len < 0 ||
-          (int64_t)s.len + (end - s.start) > limit;
+          (int64_t)s.len + (end - s.start) > c.limit;
   s.n = s.bad ? 0 : end - s.start;
   return s;
 }
-
 
 }  // namespace gn

@@ -22,6 +22,7 @@ struct KvArgs {
   int32_t *bad;
   int pages, P, lgP, KVH, hd, R, max_pages;
   int B, N, max_new, max_len;
+  int limit;  // tokens that a sequence may have, its new ones among them
 };
 
 struct KvAppendArgs {
@@ -30,7 +31,7 @@ struct KvAppendArgs {
   void *qo;
   int64_t qs, xs[2], qos;
   const float *cs, *sn;  // null: no rotation
-  int rope_len, H;
+  int H;
   int touch;             // pages a sequence's new tokens can lie in
   int qtiles;            // rotation blocks a sequence
   uint32_t per_inv, group_inv, pair_inv;  // inverses of a query head's groups, a row's, a key head's pairs of them

@@ -62,6 +62,7 @@ int batch_check(gn_ctx *c, KvArgs &a, const int32_t *starts, const int32_t *lens
   a.N = N;
   a.max_new = max_new;
   a.max_len = max_len;
+  a.limit = std::min(max_len, a.max_pages * a.P);
   a.bad = bad;
   return GN_OK;
 }
@@ -80,8 +81,8 @@ bool aligned4(const void *p, int64_t stride, int dtype) {
 }
 
 int append_impl(gn_ctx *c, const KvArgs &kv, const void *q, const void *k, const void *v, void *q_out, int64_t q_stride,
-                int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos, const float *sin, int rope_len,
-                int heads, int dtype) {
+                int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos, const float *sin, int heads,
+                int dtype) {
   KvAppendArgs a{};
   a.c = kv;
   a.c.max_new = std::min(kv.max_new, kv.N);  // no sequence has more, whatever the bound
@@ -95,7 +96,6 @@ int append_impl(gn_ctx *c, const KvArgs &kv, const void *q, const void *k, const
   a.qos = q_out_stride;
   a.cs = cos;
   a.sn = sin;
-  a.rope_len = rope_len;
   a.H = heads;
   a.vec = kv.hd % 8 == 0 && aligned4(k, k_stride, dtype) && aligned4(v, v_stride, dtype) &&
           (!q || (aligned4(q, q_stride, dtype) && aligned4(q_out, q_out_stride, dtype))) &&
@@ -175,6 +175,7 @@ extern "C" int gn_kv_append(gn_ctx *c, const gn_kv_cache *kv, const void *q, con
   if (rc) return rc;
   if (!cos != !sin || (cos && rope_len < 0)) return set_err(c, GN_ERR_INVALID, "cos and sin come together");
   if (!q != !q_out) return set_err(c, GN_ERR_INVALID, "q and q_out come together");
+  if (cos) a.limit = std::min(a.limit, rope_len);
   if (B == 0 || N == 0 || max_new == 0) return GN_OK;
   const int64_t kw = (int64_t)a.KVH * a.hd, qw = (int64_t)heads * a.hd;
   if ((rc = row_check(c, "k", k, k_stride, kw, dtype)) || (rc = row_check(c, "v", v, v_stride, kw, dtype))) return rc;
@@ -182,7 +183,7 @@ extern "C" int gn_kv_append(gn_ctx *c, const gn_kv_cache *kv, const void *q, con
     return rc;
   if (q == q_out && q && q_stride != q_out_stride)
     return set_err(c, GN_ERR_INVALID, "q_out in place of q needs q's stride");
-  return append_impl(c, a, q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, cos, sin, rope_len, heads, dtype);
+  return append_impl(c, a, q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, cos, sin, heads, dtype);
 }
 
 extern "C" int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max_len, int32_t heads, int32_t kv_heads,
@@ -239,6 +240,8 @@ extern "C" int gn_mha_cached_forward(gn_ctx *c, const gn_kv_cache *kv, const flo
   if (rc) return rc;
   rc = batch_check(c, a, starts, lens, B, N, max_new, max_len, a.KVH, GN_DTYPE_F32, bad);
   if (rc) return rc;
+  // one limit for both halves: what is not appended is not attended to, nor the other way
+  if (cos) a.limit = std::min(a.limit, rope_len);
   if ((int64_t)a.KVH * a.hd != D) return set_err(c, GN_ERR_SHAPE, "%d heads of %d are not D = %d", a.KVH, a.hd, D);
   if (!cos != !sin || (cos && rope_len < 0)) return set_err(c, GN_ERR_INVALID, "cos and sin come together");
   if (B == 0 || N == 0 || max_new == 0) return GN_OK;
@@ -257,7 +260,7 @@ extern "C" int gn_mha_cached_forward(gn_ctx *c, const gn_kv_cache *kv, const flo
     KTimer kt(c, GN_KCLASS_GEMM, "gemm_fwd", gemm_flops(g));
     HIP_OK(c, launch_gemm('N', 'T', EPI_BIAS_ACT, g, c->stream));
   }
-  rc = append_impl(c, a, qkv, qkv + rows, qkv + 2 * rows, qkv, D, D, D, D, cos, sin, rope_len, a.KVH, GN_DTYPE_F32);
+  rc = append_impl(c, a, qkv, qkv + rows, qkv + 2 * rows, qkv, D, D, D, D, cos, sin, a.KVH, GN_DTYPE_F32);
   if (rc) return rc;
   // rows outside every sequence are not attention's to write, but wOut reads them
   HIP_OK(c, launch_fill(o, 0.f, (int64_t)N * D, c->stream));

@@ -90,12 +90,10 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   const KvArgs &c = a.c;
   const int tid = threadIdx.x, NT = blockDim.x;
   const int items = c.B * a.touch * c.KVH * 2;
-  const int limit0 = c.max_pages * c.P;
-  const int limit = a.cs ? min(limit0, a.rope_len) : limit0;
   const int half = c.hd >> 1;
   if ((int)blockIdx.x >= items) {  // queries: KV_TURNS groups of four pairs a thread
     const int i = blockIdx.x - items, b = i / a.qtiles, tile = i % a.qtiles;
-    const Seq s = kv_seq(c, b, limit);
+    const Seq s = kv_seq(c, b);
     const T *q = (const T *)a.q;
     T *qo = (T *)a.qo;
     const int per = (half + 3) >> 2, row_groups = a.H * per;  // of a head, of a token
@@ -152,7 +150,7 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   const int h = i % c.KVH;
   i /= c.KVH;
   const int j = i % a.touch, b = i / a.touch;
-  const Seq s = kv_seq(c, b, limit);
+  const Seq s = kv_seq(c, b);
   if (s.bad && c.bad && j == 0 && tid == 0) c.bad[b] = 1;
   const int pi = (s.len >> c.lgP) + j;             // page of the sequence
   const int first = pi << c.lgP;                   // its first position

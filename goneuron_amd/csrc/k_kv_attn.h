@@ -107,7 +107,7 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
   id /= pl.splits;
   const int tile = pl.tiles - 1 - id % pl.tiles;  // the rows that see most first
   x.b = id / pl.tiles;
-  x.s = kv_seq(c, x.b, min(c.max_len, c.max_pages * c.P));
+  x.s = kv_seq(c, x.b);
   if (x.s.bad && c.bad && threadIdx.x == 0) c.bad[x.b] = 1;
   x.total = x.s.len + x.s.n;
   x.rows = x.s.n * a.G;
@@ -709,7 +709,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void kv_join_kernel(
   const int64_t slots = (int64_t)c.B * c.max_new * a.H, slot = WAVES == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x;
   if (slot >= slots) return;
   const int h = (int)(slot % a.H), t = (int)(slot / a.H % c.max_new), b = (int)(slot / a.H / c.max_new);
-  const Seq s = kv_seq(c, b, min(c.max_len, c.max_pages * c.P));
+  const Seq s = kv_seq(c, b);
   if (t >= s.n) return;
   // what the row's workgroup saw, as it counted it
   const int row = t * a.G + h % a.G, wg0 = row / pl.rows_wg * pl.rows_wg;

@@ -615,7 +615,8 @@ int gn_kv_attention(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out
  * gn_mha_forward's; Q, K, V of the new tokens, rotated where cos and sin are
  * given (gn_rope_tables), K and V appended, causal attention over the cache, wOut.
  * kv->kv_heads x kv->head_dim must be D.  With all tokens at once and empty sequences it
- * computes gn_mha_forward's causal layer, keys and values rounded to 8 bits.  Rows
+ * computes gn_mha_forward's causal layer, keys and values rounded to 8 bits.  A sequence
+ * beyond max_len, the table or rope_len is neither appended nor attended to.  Rows
  * outside every sequence, and of a sequence that is skipped, get wOut's bias.  work:
  * gn_mha_cached_workspace floats for B, N, max_new and max_len as large or larger. */
 int gn_mha_cached_workspace(int32_t B, int32_t N, int32_t max_new, int32_t max_len, int32_t D, int32_t heads,

@@ -119,3 +119,51 @@ def test_splits_that_the_scratch_does_not_hold(dev, dtype):
         for b in list(range(0, B, 37)) + [7, B - 1]:
             want, size, lost = kvref.attend(ref, b, lens[b] - 1, q64.reshape(B, 1, G, hd)[b], 0.0625, 1)
             assert (np.abs(got[b] - want[0]) <= kvref.bound(want, size, lost, lens[b], dtype)[0]).all(), (bound, b)
+
+
+def test_layer_skips_a_sequence_whole(dev):
+    """gn_mha_cached_forward beside a good sequence with one whose positions end behind the
+    rotation tables but within max_len, one behind max_len but within the tables, and one
+    with negative length: flagged, nothing of theirs stored, their rows wOut's bias, and
+    the good sequence's rows as if it were alone."""
+    L, check = _lib()
+    rng = np.random.default_rng(31)
+    heads, hd, page = 2, 32, 16
+    D = heads * hd
+    nd = D * D + D
+    params = (rng.normal(size=4 * nd) / math.sqrt(D)).astype(np.float32)
+    cos, sin = kvref.tables(64, hd)
+    x = rng.normal(size=(11, D)).astype(np.float32)
+    new, past = [3, 3, 3, 2], [9, 30, 46, -1]
+
+    def run(which, rope_len, max_len):
+        r = np.random.default_rng(32)
+        ref = filled(r, page, heads, hd, [9, 30, 46, 1])
+        on = OnDevice(dev, ref)
+        before = [a.get() for a in (on.k, on.v, on.ks, on.vs)]
+        n = C.c_int64()
+        B, N = len(which), sum(new[b] for b in which)
+        check(None, L.gn_mha_cached_workspace(B, N, 3, max_len, D, heads, C.byref(n)))
+        rows = np.concatenate([x[sum(new[:b]):sum(new[:b + 1])] for b in which])
+        dx, dp, do = DBuf(dev, rows), DBuf(dev, params), DBuf(dev, rows * 0 + 5)
+        dc, ds, work = DBuf(dev, cos), DBuf(dev, sin), DBuf(dev, np.full(n.value, np.nan, np.float32))
+        st, ln, bad = DBuf(dev, starts_of([new[b] for b in which])), DBuf(dev, np.array([past[b] for b in which], np.int32)), \
+            DBuf(dev, np.zeros(B, np.int32))
+        check(dev.h, L.gn_mha_cached_forward(dev.h, C.byref(on.kv), dx.p, dp.p, do.p, dc.p, ds.p, rope_len, st.p, ln.p, B, N, 3,
+                                             max_len, D, work.p, bad.p))
+        return ref, before, [a.get() for a in (on.k, on.v, on.ks, on.vs)], do.get(), bad.get().tolist()
+
+    bias = params[3 * nd + D * D:]
+    for rope_len, max_len, flags in ((32, 64, [0, 1, 1, 1]), (64, 40, [0, 0, 1, 1]), (64, 12, [0, 1, 1, 1]), (33, 48, [0, 0, 1, 1])):
+        ref, before, after, out, bad = run([0, 1, 2, 3], rope_len, max_len)
+        assert bad == flags
+        alone = run([0], rope_len, max_len)
+        assert np.array_equal(out[:3], alone[3][:3])
+        s = starts_of(new)
+        for b in range(1, 4):
+            if flags[b]:
+                assert np.array_equal(out[s[b]:s[b + 1]], np.broadcast_to(bias, (new[b], D))), (rope_len, max_len, b)
+                for was, now in zip(before, after):
+                    assert np.array_equal(was[ref.table[b]], now[ref.table[b]], equal_nan=True), (rope_len, max_len, b)
+            else:
+                assert not np.array_equal(out[s[b]:s[b + 1]], np.broadcast_to(bias, (new[b], D)))
