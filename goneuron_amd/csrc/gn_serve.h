@@ -38,6 +38,7 @@ struct KvAppendArgs {
   int vec;               // rows, tables and halves allow 4-value accesses
 };
 hipError_t launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s);
+hipError_t launch_kv_check(const KvArgs &c, hipStream_t s);
 
 struct KvAttnArgs {
   KvArgs c;

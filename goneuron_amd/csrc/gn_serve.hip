@@ -67,6 +67,12 @@ int batch_check(gn_ctx *c, KvArgs &a, const int32_t *starts, const int32_t *lens
   return GN_OK;
 }
 
+// a call without rows: its sequences are still looked at
+int no_rows(gn_ctx *c, const KvArgs &a) {
+  if (a.B > 0 && a.bad) HIP_OK(c, launch_kv_check(a, c->stream));
+  return GN_OK;
+}
+
 int row_check(gn_ctx *c, const char *what, const void *p, int64_t stride, int64_t width, int dtype) {
   if (!p) return set_err(c, GN_ERR_INVALID, "%s is null", what);
   if (stride < width)
@@ -176,7 +182,7 @@ extern "C" int gn_kv_append(gn_ctx *c, const gn_kv_cache *kv, const void *q, con
   if (!cos != !sin || (cos && rope_len < 0)) return set_err(c, GN_ERR_INVALID, "cos and sin come together");
   if (!q != !q_out) return set_err(c, GN_ERR_INVALID, "q and q_out come together");
   if (cos) a.limit = std::min(a.limit, rope_len);
-  if (B == 0 || N == 0 || max_new == 0) return GN_OK;
+  if (B == 0 || N == 0 || max_new == 0) return no_rows(c, a);
   const int64_t kw = (int64_t)a.KVH * a.hd, qw = (int64_t)heads * a.hd;
   if ((rc = row_check(c, "k", k, k_stride, kw, dtype)) || (rc = row_check(c, "v", v, v_stride, kw, dtype))) return rc;
   if (q && ((rc = row_check(c, "q", q, q_stride, qw, dtype)) || (rc = row_check(c, "q_out", q_out, q_out_stride, qw, dtype))))
@@ -206,7 +212,7 @@ extern "C" int gn_kv_attention(gn_ctx *c, const gn_kv_cache *kv, const void *q, 
   rc = batch_check(c, a, starts, lens, B, N, max_new, max_len, heads, dtype, bad);
   if (rc) return rc;
   if (!isfinite(scale)) return set_err(c, GN_ERR_INVALID, "scale is not finite");
-  if (B == 0 || N == 0 || max_new == 0) return GN_OK;
+  if (B == 0 || N == 0 || max_new == 0) return no_rows(c, a);
   const int64_t w = (int64_t)heads * a.hd;
   if ((rc = row_check(c, "q", q, q_stride, w, dtype)) || (rc = row_check(c, "out", out, out_stride, w, dtype))) return rc;
   if (!work && kv_attn_uses_work(a, heads, dtype))
@@ -244,7 +250,7 @@ extern "C" int gn_mha_cached_forward(gn_ctx *c, const gn_kv_cache *kv, const flo
   if (cos) a.limit = std::min(a.limit, rope_len);
   if ((int64_t)a.KVH * a.hd != D) return set_err(c, GN_ERR_SHAPE, "%d heads of %d are not D = %d", a.KVH, a.hd, D);
   if (!cos != !sin || (cos && rope_len < 0)) return set_err(c, GN_ERR_INVALID, "cos and sin come together");
-  if (B == 0 || N == 0 || max_new == 0) return GN_OK;
+  if (B == 0 || N == 0 || max_new == 0) return no_rows(c, a);
   if (!x || !params || !out || !work) return set_err(c, GN_ERR_INVALID, "null pointer");
   if ((uintptr_t)work & 15) return set_err(c, GN_ERR_INVALID, "mha_cached: work must be 16-byte aligned");
   const int64_t nd = (int64_t)D * D + D, rows = ((int64_t)N * D + 63) / 64 * 64;

@@ -337,7 +337,18 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   }
 }
 
+// what the other kernels flag, where a call has no row for them
+__global__ __launch_bounds__(256) void kv_check_kernel(KvArgs c) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b < c.B && kv_seq(c, b).bad) c.bad[b] = 1;
+}
+
 }  // namespace
+
+hipError_t launch_kv_check(const KvArgs &c, hipStream_t s) {
+  hipLaunchKernelGGL(kv_check_kernel, dim3((c.B + 255) / 256), dim3(256), 0, s, c);
+  return hipGetLastError();
+}
 
 hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   KvAppendArgs a = a0;

@@ -167,3 +167,28 @@ def test_layer_skips_a_sequence_whole(dev):
                     assert np.array_equal(was[ref.table[b]], now[ref.table[b]], equal_nan=True), (rope_len, max_len, b)
             else:
                 assert not np.array_equal(out[s[b]:s[b + 1]], np.broadcast_to(bias, (new[b], D)))
+
+
+def test_calls_without_rows_flag_their_sequences(dev):
+    """N = 0 or max_new = 0: nothing is stored or written, but what would be skipped is
+    flagged as in any other call."""
+    L, check = _lib()
+    rng = np.random.default_rng(41)
+    ref = filled(rng, 16, 1, 32, [20, 20, 20])
+    on = OnDevice(dev, ref)
+    x = DBuf(dev, np.full(4096, 7, np.float32))
+    ln = DBuf(dev, np.array([20, 1000, -1], np.int32))
+    for N, max_new, starts, flags in ((0, 5, [0, 0, 0, 0], [0, 1, 1]), (0, 0, [0, 0, 0, 0], [0, 1, 1]), (9, 0, [0, 2, 2, 2], [1, 1, 1]),
+                                      (9, 0, [0, 0, 0, 0], [0, 1, 1]), (0, 1, [0, 1, 1, 1], [1, 1, 1])):
+        st = DBuf(dev, np.array(starts, np.int32))
+        for call in ("append", "attention"):
+            bad = DBuf(dev, np.zeros(3, np.int32))
+            if call == "append":
+                check(dev.h, L.gn_kv_append(dev.h, C.byref(on.kv), x.p, x.p, x.p, x.p, 32, 32, 32, 32, None, None, 0, st.p, ln.p, 3, N,
+                                            max_new, 1, F32, bad.p))
+            else:
+                check(dev.h, L.gn_kv_attention(dev.h, C.byref(on.kv), x.p, x.p, 32, 32, st.p, ln.p, 3, N, max_new, 64, 1, 1.0, 1, F32,
+                                               None, bad.p))
+            assert bad.get().tolist() == flags, (call, N, max_new, starts)
+            on.same()
+            assert (x.get() == 7).all()
