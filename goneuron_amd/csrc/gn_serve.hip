@@ -250,12 +250,14 @@ extern "C" int gn_mha_cached_forward(gn_ctx *c, const gn_kv_cache *kv, const flo
   if (cos) a.limit = std::min(a.limit, rope_len);
   if ((int64_t)a.KVH * a.hd != D) return set_err(c, GN_ERR_SHAPE, "%d heads of %d are not D = %d", a.KVH, a.hd, D);
   if (!cos != !sin || (cos && rope_len < 0)) return set_err(c, GN_ERR_INVALID, "cos and sin come together");
-  if (B == 0 || N == 0 || max_new == 0) return no_rows(c, a);
+  const bool some = B > 0 && N > 0 && max_new > 0;
+  if (!some && (rc = no_rows(c, a))) return rc;
+  if (N == 0) return GN_OK;
   if (!x || !params || !out || !work) return set_err(c, GN_ERR_INVALID, "null pointer");
   if ((uintptr_t)work & 15) return set_err(c, GN_ERR_INVALID, "mha_cached: work must be 16-byte aligned");
   const int64_t nd = (int64_t)D * D + D, rows = ((int64_t)N * D + 63) / 64 * 64;
   float *qkv = work, *o = work + 3 * rows;
-  {
+  if (some) {
     GemmArgs g{};
     g.M = N; g.N = D; g.K = D;
     g.A = x; g.lda = D; g.B = params; g.ldb = D;
@@ -265,13 +267,15 @@ extern "C" int gn_mha_cached_forward(gn_ctx *c, const gn_kv_cache *kv, const flo
     g.bstride_B = nd; g.bstride_bias = nd; g.bstride_C = rows;
     KTimer kt(c, GN_KCLASS_GEMM, "gemm_fwd", gemm_flops(g));
     HIP_OK(c, launch_gemm('N', 'T', EPI_BIAS_ACT, g, c->stream));
+    rc = append_impl(c, a, qkv, qkv + rows, qkv + 2 * rows, qkv, D, D, D, D, cos, sin, a.KVH, GN_DTYPE_F32);
+    if (rc) return rc;
   }
-  rc = append_impl(c, a, qkv, qkv + rows, qkv + 2 * rows, qkv, D, D, D, D, cos, sin, a.KVH, GN_DTYPE_F32);
-  if (rc) return rc;
   // rows outside every sequence are not attention's to write, but wOut reads them
   HIP_OK(c, launch_fill(o, 0.f, (int64_t)N * D, c->stream));
-  rc = attn_impl(c, a, qkv, o, D, D, a.KVH, (float)(1.0 / sqrt((double)a.hd)), 1, GN_DTYPE_F32, work + 4 * rows);
-  if (rc) return rc;
+  if (some) {
+    rc = attn_impl(c, a, qkv, o, D, D, a.KVH, (float)(1.0 / sqrt((double)a.hd)), 1, GN_DTYPE_F32, work + 4 * rows);
+    if (rc) return rc;
+  }
   GemmArgs g{};
   g.M = N; g.N = D; g.K = D;
   g.A = o; g.lda = D; g.B = params + 3 * nd; g.ldb = D;

@@ -192,3 +192,29 @@ def test_calls_without_rows_flag_their_sequences(dev):
             assert bad.get().tolist() == flags, (call, N, max_new, starts)
             on.same()
             assert (x.get() == 7).all()
+
+
+def test_layer_rows_of_no_sequence(dev):
+    """Rows outside every sequence get wOut's bias, where there is no sequence and where
+    none may have a token too."""
+    L, check = _lib()
+    rng = np.random.default_rng(42)
+    D, heads, N = 64, 2, 5
+    nd = D * D + D
+    params = rng.normal(size=4 * nd).astype(np.float32)
+    ref = filled(rng, 16, heads, 32, [20, 3])
+    on = OnDevice(dev, ref)
+    n = C.c_int64()
+    dx, dp, x = DBuf(dev, rng.normal(size=(N, D)).astype(np.float32)), DBuf(dev, params), np.full((N, D), 9, np.float32)
+    for B, max_new, starts, flags in ((0, 4, [0, 0, 0], [0, 0]), (2, 0, [0, 0, 0], [0, 0]), (2, 0, [0, 3, 3], [1, 0]),
+                                      (2, 4, [2, 2, 2], [0, 0])):
+        check(None, L.gn_mha_cached_workspace(B, N, max_new, 64, D, heads, C.byref(n)))
+        do, work = DBuf(dev, x), DBuf(dev, np.full(n.value, np.nan, np.float32))
+        st, ln, bad = DBuf(dev, np.array(starts, np.int32)), DBuf(dev, np.array([20, 3], np.int32)), DBuf(dev, np.zeros(2, np.int32))
+        check(dev.h, L.gn_mha_cached_forward(dev.h, C.byref(on.kv), dx.p, dp.p, do.p, None, None, 0, st.p, ln.p, B, N, max_new, 64, D,
+                                             work.p, bad.p))
+        assert bad.get().tolist() == flags
+        assert np.array_equal(do.get(), np.broadcast_to(params[3 * nd + D * D:], (N, D))), (B, max_new)
+        on.same()
+    assert L.gn_mha_cached_forward(dev.h, C.byref(on.kv), dx.p, dp.p, None, None, None, 0, st.p, ln.p, 0, N, 4, 64, D, work.p, None) == -1
+    assert L.gn_mha_cached_forward(dev.h, C.byref(on.kv), None, None, None, None, None, 0, st.p, ln.p, 2, 0, 4, 64, D, None, None) == 0
