@@ -539,7 +539,7 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
   const Work x = kv_work(a, pl);
   if (!x.any) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, g = lane >> 4;
-  const float factor = kv_factor(a.scale);
+  const float sf = kv_factor(a.scale);
   Rows<T, R, 1> A;
   A.init(a, x, x.row0, n, [&](int k) { return k < R / 64 * 2 ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 : R / 64 * 64 + g * 8; });
 
@@ -554,8 +554,10 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
   // lane n holds key 16 (n >> 2) + 4 t + (n & 3) of tile t, 16 bytes of each 64
   // columns; of V row 16 d + n, 16 keys of group g
   uint32_t kr[4][R / 16], vr[ND][4];
+  float ksc = 0.f, vsc = 0.f;  // scales of that K and that V
   const auto load_k = [&](int j, int page) {
     const int pk = __shfl(page, (n >> 2) * 16, 64);
+    ksc = c.ks[(int64_t)pk * c.KVH + x.kvh];
     const uint8_t *base = kb + pk * page_bytes + (int64_t)((j + 16 * (n >> 2) + (n & 3)) & (c.P - 1)) * R;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -582,13 +584,11 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
 
   int j = x.k0 + w * 64, page = 0, next = 0;
   bool ok = false;
-  float ksc = 0.f, vsc = 0.f;
   // a step's page (0 where there is none), K and scales, and the page after it
   const auto advance = [&](int at, int p) {
     ok = (unsigned)p < (unsigned)c.pages;
     page = ok ? p : 0;
     load_k(at, page);
-    ksc = c.ks[(int64_t)page * c.KVH + x.kvh];
     vsc = c.vs[(int64_t)page * c.KVH + x.kvh];
     next = page_at(at + STEP);
   };
@@ -597,13 +597,13 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
     constexpr bool CLEAN = decltype(clean_)::value != 0;
     const bool was_ok = ok;
     const int first = j + 16 * g;  // this lane's scores are of the keys first + 4 t + i
-    const float sf = (ok ? ksc : 1.f) * factor, vs = ok ? vsc : 1.f;
+    const float vs = ok ? vsc : 1.f;
     f32x4 S[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < NK; ++k) A.scores(from_e4m3(kr[t][2 * k], kr[t][2 * k + 1], 1.f), k, 0, S[t]);
+      for (int k = 0; k < NK; ++k) A.scores(from_e4m3(kr[t][2 * k], kr[t][2 * k + 1], ksc), k, 0, S[t]);
     }
     between();  // K's registers are free
     bf16x8 pf[2][A.WPARTS];

@@ -218,3 +218,31 @@ def test_layer_rows_of_no_sequence(dev):
         on.same()
     assert L.gn_mha_cached_forward(dev.h, C.byref(on.kv), dx.p, dp.p, None, None, None, 0, st.p, ln.p, 0, N, 4, 64, D, work.p, None) == -1
     assert L.gn_mha_cached_forward(dev.h, C.byref(on.kv), None, None, None, None, None, 0, st.p, ln.p, 2, 0, 4, 64, D, None, None) == 0
+
+
+@pytest.mark.parametrize("dtype,hd,new", [("f32", 64, 1), ("bf16", 128, 1), ("bf16", 256, 1), ("f32", 192, 1), ("bf16", 64, 40),
+                                          ("f32", 32, 20)])
+def test_score_scales_of_any_size(dev, dtype, hd, new):
+    """Score scales down to the smallest number, over keys of 0 (whose block scale is 2^-100)
+    and ordinary ones; 0 and negative scales."""
+    L, check = _lib()
+    rng = np.random.default_rng(hd + new)
+    ref = kvref.Cache(20, 16, 2, hd, rng.permutation(20).reshape(2, 10).astype(np.int32), rng)
+    lens = [75 + new, 5 + new]
+    for b, n in enumerate(lens):
+        x = rng.normal(size=(2, n, 2, hd))
+        x[0, :40] = 0
+        ref.append(b, 0, x[0], x[1])
+    on = OnDevice(dev, ref)
+    q, q64 = as_dtype(rng.normal(size=(2 * new, 2 * hd)), dtype)
+    work = DBuf(dev, np.zeros(max(1, attention_floats(2, new, 160, 2, 2, hd)), np.float32))
+    dq, do, st = DBuf(dev, q), DBuf(dev, q * 0), DBuf(dev, starts_of([new, new]))
+    ln = DBuf(dev, np.asarray(lens, np.int32) - new)
+    for scale in (1e-20, 1e-36, 1e-45, 0.0, -0.25, 4.0):
+        scale = float(np.float32(scale))
+        check(dev.h, L.gn_kv_attention(dev.h, C.byref(on.kv), dq.p, do.p, 2 * hd, 2 * hd, st.p, ln.p, 2, 2 * new, new, 160, 2, scale, 1,
+                                       F32 if dtype == "f32" else BF16, work.p, None))
+        got = values(do.get(), dtype).reshape(2, new, 2, hd)
+        for b in range(2):
+            want, size, lost = kvref.attend(ref, b, lens[b] - new, q64.reshape(2, new, 2, hd)[b], scale, 1)
+            assert (np.abs(got[b] - want) <= kvref.bound(want, size, lost, lens[b], dtype)).all(), (scale, b)
