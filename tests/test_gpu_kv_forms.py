@@ -8,7 +8,7 @@ import pytest
 
 import kvref
 from gpuutil import DBuf, log
-from test_gpu_kv_cache import BF16, F32, OnDevice, as_dtype, spread, starts_of, values
+from test_gpu_kv_cache import BF16, F32, OnDevice, as_dtype, attention_case, spread, starts_of, values
 
 pytestmark = pytest.mark.gpu
 
@@ -246,3 +246,66 @@ def test_score_scales_of_any_size(dev, dtype, hd, new):
         for b in range(2):
             want, size, lost = kvref.attend(ref, b, lens[b] - new, q64.reshape(2, new, 2, hd)[b], scale, 1)
             assert (np.abs(got[b] - want) <= kvref.bound(want, size, lost, lens[b], dtype)).all(), (scale, b)
+
+
+# up to 16 rows a key head: dtype, hd, page, kvh, group, past, new
+FEW = [
+    ("f32", 72, 16, 2, 2, [333, 0, 701], 1),
+    ("bf16", 96, 32, 2, 4, [300, 63], 1),
+    ("bf16", 72, 64, 1, 3, [517, 90], 5),
+    ("f32", 128, 128, 2, 1, [450, 6], 3),
+    ("f32", 160, 64, 1, 2, [619, 127, 0], 1),
+    ("bf16", 192, 16, 2, 1, [411, 255], 2),
+    ("bf16", 136, 32, 1, 16, [290], 1),
+    ("f32", 256, 32, 2, 1, [555, 3], 1),
+    ("bf16", 256, 128, 1, 4, [777, 256], 4),
+    ("f32", 200, 16, 1, 8, [365], 2),
+]
+
+
+@pytest.mark.parametrize("dtype,hd,page,kvh,G,past,new", FEW)
+def test_few_rows_of_every_head(dev, dtype, hd, page, kvh, G, past, new):
+    """Heads of every padded size in the single-token kernel, several steps a wave, lengths
+    that end inside a step; told the true length and one that splits the keys."""
+    B = len(past)
+    for max_len in (None, 20000):
+        assert attention_case(dev, dtype, hd, page, kvh, G, past, [new] * B, 1, max_len=max_len).tolist() == [0] * B
+
+
+@pytest.mark.parametrize("dtype,hd,page,kvh,G,past,new", FEW)
+def test_few_rows_with_missing_pages_and_nan(dev, dtype, hd, page, kvh, G, past, new):
+    B = len(past)
+
+    def missing(ref):
+        ref.table[0, 1], ref.table[0, past[0] // page // 2] = -1, ref.pages + 7
+
+    def nan(ref):
+        for p, h, d, code in ((past[0] // 2, 0, hd - 1, 0x7f), (past[0] + new - 1, kvh - 1, 0, 0xff), (3, 0, hd // 2, 0x7f)):
+            ref.v[ref.table[0, p // page], h, d, p % page] = code
+        p = past[0] + new - 1  # a key that only the last new token sees
+        ref.k[ref.table[0, p // page], 0, p % page, hd - 1] = 0x7f
+
+    for max_len in (None, 9000):
+        assert attention_case(dev, dtype, hd, page, kvh, G, past, [new] * B, 1, max_len=max_len, spoil=missing)[0] == 1
+        attention_case(dev, dtype, hd, page, kvh, G, past, [new] * B, 1, max_len=max_len, spoil=nan)
+
+
+@pytest.mark.parametrize("dtype,hd,page,kvh,G,past,new", [
+    ("f32", 128, 32, 2, 2, [70, 0, 129], [90, 33, 1]), ("f32", 104, 16, 1, 3, [5], [140]), ("bf16", 192, 64, 1, 2, [100, 0], [65, 130]),
+    ("bf16", 136, 32, 2, 1, [40], [77]), ("f32", 256, 64, 1, 1, [200], [70]), ("f32", 160, 128, 1, 5, [9, 300], [40, 17])])
+def test_prompts_of_every_head(dev, dtype, hd, page, kvh, G, past, new):
+    """Heads of every padded size in the prompts' kernel, whole and split along the keys,
+    with missing pages and NaN."""
+    def missing(ref):
+        ref.table[0, 0] = -3
+
+    def nan(ref):
+        p = past[0] + new[0] // 2
+        ref.v[ref.table[0, p // page], 0, hd - 1, p % page] = 0x7f
+        ref.k[ref.table[0, (p + 3) // page], kvh - 1, (p + 3) % page, 1] = 0xff
+
+    for max_len in (None, 3000):
+        for spoil in (None, missing, nan):
+            bad = attention_case(dev, dtype, hd, page, kvh, G, past, new, 1, max_len=max_len, spoil=spoil)
+            assert bad.tolist() == [int(spoil is missing)] + [0] * (len(past) - 1)
+    attention_case(dev, dtype, hd, page, kvh, G, past, new, 0)
