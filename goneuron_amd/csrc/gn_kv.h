@@ -49,13 +49,13 @@ struct Seq {
   int start, n, len;
   bool bad;
 };
-__device__ __forceinline__ Seq kv_seq(const KvArgs &c, int b) {
+__device__ __forceinline__ Seq kv_seq(const KvArgs &c, int b, int limit) {
   Seq s;
   s.start = c.starts[b];
   const int end = c.starts[b + 1];
   s.len = c.lens[b];
   s.bad = s.start < 0 || end < s.start || end > c.N || end - s.start > c.max_new || s.len < 0 ||
-          (int64_t)s.len + (end - s.start) > c.limit;
+          (int64_t)s.len + (end - s.start) > limit;
   s.n = s.bad ? 0 : end - s.start;
   return s;
 }

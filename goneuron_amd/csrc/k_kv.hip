@@ -3,8 +3,8 @@
 // Layout: K pages [page][kv head][token][R], V pages [page][kv head][R][token]
 // in E4M3 with a power-of-two scale per (page, kv head) for each.  V lies
 // transposed so that attention's two products read both caches as their matrix
-// operands lie in registers, 16 bytes a lane, with no pass through LDS; the
-// writer owns a whole block anyway (its scale covers the block).
+// operands lie in registers, 16 bytes a lane (single tokens with no pass through LDS);
+// the writer owns a whole block anyway (its scale covers the block).
 #include "gn_kv.h"
 
 namespace gn {
@@ -78,9 +78,10 @@ constexpr int KV_TURNS = 2;  // groups of four pairs of queries a thread turns
 // block, so its new maximum, the growth of its scale and the bytes of tokens
 // already there need no other workgroup.  New values stay in registers between
 // the maximum and the rounding.  Blocks behind those rotate the queries.
-// Bound by latency for single tokens (a chain of table, row and scale reads, one
-// reduction: 9.5 us for a bfloat16 token of 256 sequences, 32 query heads and 8 key
-// heads of 128, whose 5.9 MB a copy moves in 1.2) and by memory for prompts (six of up to
+// Single tokens: a chain of table, row and scale reads and one reduction, 4.2 us for a
+// token of 4 sequences; a bfloat16 token of 256 sequences, 32 query heads and 8 key heads
+// of 128, takes 9.5 (a copy moves its 5.9 MB in 1.2), most likely for the 262144 bytes of
+// V, each into a line of its own (no counter was read for it).  Prompts: memory (six of up to
 // 2048: 45 us for 163 MB, 3.6 TB/s, where a copy reaches 4.9).  Prompts also wait for the
 // vector unit: indexes without divisions, pairs turned once and bytes rounded two at a
 // time brought them from 60.
@@ -90,10 +91,13 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   const KvArgs &c = a.c;
   const int tid = threadIdx.x, NT = blockDim.x;
   const int items = c.B * a.touch * c.KVH * 2;
+  // no page behind the table, whatever the limit.  (Without the minimum prompts of
+  // bfloat16 rows are given 80 registers, six waves a SIMD, not 72 and seven: 1 us of 39.)
+  const int limit = min(c.limit, c.max_pages * c.P);
   const int half = c.hd >> 1;
   if ((int)blockIdx.x >= items) {  // queries: KV_TURNS groups of four pairs a thread
     const int i = blockIdx.x - items, b = i / a.qtiles, tile = i % a.qtiles;
-    const Seq s = kv_seq(c, b);
+    const Seq s = kv_seq(c, b, limit);
     const T *q = (const T *)a.q;
     T *qo = (T *)a.qo;
     const int per = (half + 3) >> 2, row_groups = a.H * per;  // of a head, of a token
@@ -150,7 +154,7 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   const int h = i % c.KVH;
   i /= c.KVH;
   const int j = i % a.touch, b = i / a.touch;
-  const Seq s = kv_seq(c, b);
+  const Seq s = kv_seq(c, b, limit);
   if (s.bad && c.bad && j == 0 && tid == 0) c.bad[b] = 1;
   const int pi = (s.len >> c.lgP) + j;             // page of the sequence
   const int first = pi << c.lgP;                   // its first position
@@ -340,7 +344,7 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
 // what the other kernels flag, where a call has no row for them
 __global__ __launch_bounds__(256) void kv_check_kernel(KvArgs c) {
   const int b = blockIdx.x * 256 + threadIdx.x;
-  if (b < c.B && kv_seq(c, b).bad) c.bad[b] = 1;
+  if (b < c.B && kv_seq(c, b, c.limit).bad) c.bad[b] = 1;
 }
 
 }  // namespace

@@ -107,7 +107,7 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
   id /= pl.splits;
   const int tile = pl.tiles - 1 - id % pl.tiles;  // the rows that see most first
   x.b = id / pl.tiles;
-  x.s = kv_seq(c, x.b);
+  x.s = kv_seq(c, x.b, c.limit);
   if (x.s.bad && c.bad && threadIdx.x == 0) c.bad[x.b] = 1;
   x.total = x.s.len + x.s.n;
   x.rows = x.s.n * a.G;
@@ -527,9 +527,10 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
 // operands come straight from memory into the lanes that need them: four times
 // the loads in flight for one set of rows, and no barrier until the waves are
 // joined through LDS.
-// Bound by memory: one sequence of 131072 tokens, 8 key heads of 128, in 58 us with its
-// join, 4.6 TB/s of cache (44 us alone: 6.1, as fast as memory is read here); 64
-// sequences of up to 8192 in 122 us, 4.4 TB/s.  A step of 5 us at the least.
+// Bound by memory: one sequence of 131072 tokens, 8 key heads of 128, in 57 us with its
+// join, 4.7 TB/s of cache (43 us alone: 6.2, as fast as memory is read here; float32
+// queries without shared heads 50, 5.4); 64 sequences of up to 8192 in 121 us, 4.4 TB/s.
+// A step of 5 us at the least.
 template <typename T, int R>
 __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void kv_attn_keys_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int NK = R / 32, ND = R / 16;
@@ -709,7 +710,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void kv_join_kernel(
   const int64_t slots = (int64_t)c.B * c.max_new * a.H, slot = WAVES == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x;
   if (slot >= slots) return;
   const int h = (int)(slot % a.H), t = (int)(slot / a.H % c.max_new), b = (int)(slot / a.H / c.max_new);
-  const Seq s = kv_seq(c, b);
+  const Seq s = kv_seq(c, b, c.limit);
   if (t >= s.n) return;
   // what the row's workgroup saw, as it counted it
   const int row = t * a.G + h % a.G, wg0 = row / pl.rows_wg * pl.rows_wg;
