@@ -521,7 +521,8 @@ class Sequential:
 
     def Sample(self, x, u, temperature=None, top_k=None, top_p=None, min_p=None):
         """A prediction of every row of x and a draw from its outputs as logits
-        (gn_model_sample; no counterpart in the reference): int32 indices.  u:
+        (gn_model_sample; no counterpart in the reference): int32 indices of what
+        the model puts out, behind a CLSPooling the pooled position's classes.  u:
         a random number in [0, 1) for each row; each setting a number for all
         rows or one for each."""
         x = _f32(x)

@@ -8,9 +8,9 @@ namespace gn {
 
 // Keys are split until every CU has work to change over to; items: workgroups without a
 // split.  Single tokens: 4096 workgroups for sequences of unlike length (64 of up to 8192
-// tokens, 8 heads: 122 us; 8192 workgroups 137, 2048 128), but 32 splits at most, or 64
+// tokens, 8 heads: 121 us; 8192 workgroups 137, 2048 128), but 32 splits at most, or 64
 // while a workgroup a CU is not reached: the join reads them all (one sequence of 131072,
-// 8 heads: 58 us with 32 splits, 61 with 64; one head: 36 and 27).  Prompts: 512
+// 8 heads: 57 us with 32 splits, 61 with 64; one head: 36 and 27).  Prompts: 512
 // workgroups (24.8 us for the five float32 prompts, 1024: 33.2), 128 keys a split at
 // least.
 static int64_t kv_splits(bool by_rows, int64_t items, int64_t len) {

@@ -20,8 +20,10 @@
 // rows of 8000, every filter, 13.3 us.  Longer ones: the pass over the logits is
 // memory's (128 rows of 131072 float32, 67 MB: 15.5 us, 4.3 TB/s), the cut a chain of
 // waits (22 us there, 16.6 for one row of 50257); 42 us and 20 to 24 us in all.  With
-// top-p alone 114 us, without a cut 49: float64 weights of all 16.8 million logits
-// take 27 to 32 us a pass.
+// top-p alone 105 to 114 us, without a cut 45 to 49: a pass that weighs all 16.8 million
+// logits in float64 takes 27 to 32 us, of which the operations themselves are about 9 at
+// the card's rate; how the rest divides between table reads and LDS atomics was not
+// measured.
 #include "gn_serve.h"
 
 namespace gn {

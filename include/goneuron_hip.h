@@ -240,7 +240,9 @@ int gn_model_predict_device(gn_model *m, const float *x_dev, int32_t B, float *o
 /* gn_model_predict and a draw from each sample's outputs as logits, with
  * gn_sample's settings as host arrays of B (each but u may be NULL); ids: B
  * indices.  No counterpart in the reference.  The last layer must give logits or
- * log-probabilities: a Dense Softmax pointer is GN_ERR_UNSUPPORTED. */
+ * log-probabilities: a Dense Softmax pointer is GN_ERR_UNSUPPORTED.  The draw is from
+ * what the model puts out: behind a CLSPooling that is the pooled position, a next
+ * token only if the model was trained to put one out there. */
 int gn_model_sample(gn_model *m, const float *x, int32_t B, const float *temperature, const int32_t *top_k,
                     const float *top_p, const float *min_p, const float *u, int32_t *ids);
 /* Network.SetTraining (net.go:187-193): sets the flag of every layer.  Layers
@@ -530,7 +532,8 @@ int gn_moe_backward(gn_ctx *ctx, const float *x, const float *params, const floa
  * calls queue work on the context's stream, allocate nothing and do not
  * synchronise (but gn_rope_tables); what lies in device memory (starts, lens,
  * the page table, settings) is read when the work runs.  Calls that may run at
- * the same time (two contexts) need a `work` each.
+ * the same time (two contexts) need a `work` each.  Like the other operators
+ * they may use the context's scratch.
  *
  * Tokens are packed: sequence b's new tokens are the rows starts[b] ..
  * starts[b + 1] - 1 (starts: B + 1 int32) of the inputs and outputs, at the
