@@ -56,6 +56,15 @@ class KVCache(C.Structure):
                 ("head_dim", C.c_int32), ("max_pages", C.c_int32)]
 
 
+class LogitRules(C.Structure):
+    """gn_logit_rules: device pointers and strides of what gn_logits_adjust applies."""
+    _fields_ = [("repetition", C.c_void_p), ("frequency", C.c_void_p), ("presence", C.c_void_p), ("tokens", C.c_void_p),
+                ("token_lens", C.c_void_p), ("prompt_lens", C.c_void_p), ("tokens_stride", C.c_int64),
+                ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("bias_lens", C.c_void_p), ("bias_stride", C.c_int64),
+                ("allowed", C.c_void_p), ("allowed_row", C.c_void_p), ("allowed_stride", C.c_int64),
+                ("allowed_rows", C.c_int32)]
+
+
 class Info(C.Structure):
     _fields_ = [("arch", C.c_char * 64), ("cu_count", C.c_int32), ("hbm_bytes", C.c_int64),
                 ("peak_fp32_mfma_tflops", C.c_double), ("peak_hbm_gbps", C.c_double)]
@@ -168,11 +177,19 @@ SIGNATURES = {
     "gn_kv_attention_workspace": (C.c_int, [C.c_int32] * 6 + [C.POINTER(C.c_int64)]),
     "gn_kv_attention": (C.c_int, [vp, C.POINTER(KVCache), vp, vp, C.c_int64, C.c_int64, vp, vp] + [C.c_int32] * 5
                         + [C.c_float, C.c_int32, C.c_int32, vp, vp]),
+    "gn_kv_attention_window": (C.c_int, [vp, C.POINTER(KVCache), vp, vp, C.c_int64, C.c_int64, vp, vp] + [C.c_int32] * 5
+                               + [C.c_float] + [C.c_int32] * 3 + [vp, vp]),
+    "gn_kv_append_at": (C.c_int, [vp, C.POINTER(KVCache), vp, vp, vp, vp] + [C.c_int64] * 4 + [vp, vp, C.c_int32, vp, vp, vp]
+                        + [C.c_int32] * 5 + [vp]),
+    "gn_kv_attention_tree": (C.c_int, [vp, C.POINTER(KVCache), vp, vp, C.c_int64, C.c_int64, vp, C.c_int64, vp, vp]
+                             + [C.c_int32] * 5 + [C.c_float, C.c_int32, vp, vp]),
+    "gn_kv_keep": (C.c_int, [vp, C.POINTER(KVCache)] + [vp] * 4 + [C.c_int32] * 3 + [vp]),
     "gn_mha_cached_workspace": (C.c_int, [C.c_int32] * 6 + [C.POINTER(C.c_int64)]),
     "gn_mha_cached_forward": (C.c_int, [vp, C.POINTER(KVCache)] + [vp] * 5 + [C.c_int32, vp, vp] + [C.c_int32] * 5
                               + [vp, vp]),
     "gn_sample_workspace": (C.c_int, [C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
     "gn_sample": (C.c_int, [vp, vp, C.c_int64, C.c_int32] + [vp] * 6 + [C.c_int32, C.c_int32, vp]),
+    "gn_logits_adjust": (C.c_int, [vp, vp, C.c_int64, vp, C.c_int64, C.c_int32, C.POINTER(LogitRules), C.c_int32, C.c_int32]),
     "gn_model_sample": (C.c_int, [vp, f32p, C.c_int32, f32p, i32p, f32p, f32p, f32p, i32p]),
     "gn_gemm": (C.c_int, [vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_float, vp,
                           C.c_int32, vp, C.c_int32, vp, C.c_int32]),

@@ -1,6 +1,6 @@
 // Library-private: the operators that answer token by token (paged 8-bit
-// cache, attention over it, sampling), kernels in k_kv.hip and k_sample.hip,
-// entry points in gn_serve.hip.
+// cache, attention over it, rules on logits, sampling), kernels in k_kv*,
+// k_logits.hip and k_sample.hip, entry points in gn_serve.hip.
 #pragma once
 #include "gn_common.h"
 
@@ -31,6 +31,8 @@ struct KvAppendArgs {
   void *qo;
   int64_t qs, xs[2], qos;
   const float *cs, *sn;  // null: no rotation
+  const int32_t *at;     // the rows' positions; null: those of their tokens in the sequence
+  int rope_len;          // positions in cs and sn (looked at with `at`)
   int H;
   int touch;             // pages a sequence's new tokens can lie in
   int qtiles;            // rotation blocks a sequence
@@ -39,7 +41,11 @@ struct KvAppendArgs {
 };
 hipError_t launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s);
 hipError_t launch_kv_check(const KvArgs &c, hipStream_t s);
+hipError_t launch_kv_keep(const KvArgs &c, const int32_t *keep, const int32_t *counts, hipStream_t s);
 
+// Which keys a query sees: those up to itself, or all (causal); of those up to itself the
+// first and the nearest; the cached ones and of the new ones those that its mask names.
+enum KvView { KV_PREFIX, KV_WINDOW, KV_TREE };
 struct KvAttnArgs {
   KvArgs c;
   const void *q;
@@ -50,6 +56,10 @@ struct KvAttnArgs {
   int causal;
   int vec;  // queries and outputs allow 4-value accesses, heads are whole eights
   float *work;
+  int view;
+  int sinks, window;     // KV_WINDOW
+  const uint32_t *mask;  // KV_TREE: a row of bits for each new token, ms words apart
+  int64_t ms;
 };
 // how a call's work is split
 struct KvPlan {
@@ -67,9 +77,13 @@ constexpr int kv_two_tiles(int bytes) { return bytes == 4 ? 64 : 128; }
 // the workspace: (maximum, sum) of every split's rows, then their outputs
 __host__ __device__ inline int64_t kv_part_at(int splits, int64_t slots) { return (splits * slots * 2 + 3) / 4 * 4; }
 int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd);
-bool kv_attn_uses_work(const KvArgs &c, int H, int dtype);  // whether a call of these very sizes does
+bool kv_attn_uses_work(const KvAttnArgs &a, int dtype);  // whether a call of these very sizes does
 hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, float *scratch, int64_t scratch_floats, hipStream_t s);
 hipError_t launch_kv_attn_bf16(const KvAttnArgs &a, const KvPlan &p, hipStream_t s);
+hipError_t launch_kv_window_f32(const KvAttnArgs &a, const KvPlan &p, hipStream_t s);
+hipError_t launch_kv_window_bf16(const KvAttnArgs &a, const KvPlan &p, hipStream_t s);
+hipError_t launch_kv_tree_f32(const KvAttnArgs &a, const KvPlan &p, hipStream_t s);
+hipError_t launch_kv_tree_bf16(const KvAttnArgs &a, const KvPlan &p, hipStream_t s);
 
 struct SampleArgs {
   const void *z;
@@ -83,5 +97,15 @@ struct SampleArgs {
 constexpr int SAMPLE_MAX_V = 1 << 20;
 int64_t sample_work_floats(int B, int V);
 hipError_t launch_sample(const SampleArgs &a, int dtype, hipStream_t s);
+
+struct LogitArgs {
+  const void *z;
+  void *out;
+  int64_t zs, os;
+  gn_logit_rules r;
+  int B, V;
+};
+constexpr int64_t LOGITS_MAX_LIST = (int64_t)1 << 30;  // tokens or biases of a row
+hipError_t launch_logits_adjust(const LogitArgs &a, int dtype, hipStream_t s);
 
 }  // namespace gn

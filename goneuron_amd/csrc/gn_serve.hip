@@ -1,6 +1,6 @@
 // Entry points of the operators that answer token by token: the paged 8-bit
-// cache, attention over it, the MultiHeadAttention layer on such a cache, and
-// sampling.  Arguments are checked here; what lies in device memory (starts,
+// cache, attention over it, the MultiHeadAttention layer on such a cache,
+// rules on logits and sampling.  Arguments are checked here; what lies in device memory (starts,
 // lens, page tables, settings) is checked by the kernels.
 #include <math.h>
 
@@ -87,8 +87,8 @@ bool aligned4(const void *p, int64_t stride, int dtype) {
 }
 
 int append_impl(gn_ctx *c, const KvArgs &kv, const void *q, const void *k, const void *v, void *q_out, int64_t q_stride,
-                int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos, const float *sin, int heads,
-                int dtype) {
+                int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos, const float *sin,
+                const int32_t *positions, int rope_len, int heads, int dtype) {
   KvAppendArgs a{};
   a.c = kv;
   a.c.max_new = std::min(kv.max_new, kv.N);  // no sequence has more, whatever the bound
@@ -102,6 +102,8 @@ int append_impl(gn_ctx *c, const KvArgs &kv, const void *q, const void *k, const
   a.qos = q_out_stride;
   a.cs = cos;
   a.sn = sin;
+  a.at = cos ? positions : nullptr;
+  a.rope_len = rope_len;
   a.H = heads;
   a.vec = kv.hd % 8 == 0 && aligned4(k, k_stride, dtype) && aligned4(v, v_stride, dtype) &&
           (!q || (aligned4(q, q_stride, dtype) && aligned4(q_out, q_out_stride, dtype))) &&
@@ -112,8 +114,8 @@ int append_impl(gn_ctx *c, const KvArgs &kv, const void *q, const void *k, const
   return GN_OK;
 }
 
-int attn_impl(gn_ctx *c, const KvArgs &kv, const void *q, void *out, int64_t qs, int64_t os, int heads, float scale,
-              int causal, int dtype, float *work) {
+KvAttnArgs attn_args(const KvArgs &kv, const void *q, void *out, int64_t qs, int64_t os, int heads, float scale, int causal,
+                     int dtype, float *work) {
   KvAttnArgs a{};
   a.c = kv;
   a.q = q;
@@ -126,10 +128,28 @@ int attn_impl(gn_ctx *c, const KvArgs &kv, const void *q, void *out, int64_t qs,
   a.causal = causal != 0;
   a.vec = kv.hd % 8 == 0 && aligned4(q, qs, dtype) && aligned4(out, os, dtype);
   a.work = work;
+  a.view = KV_PREFIX;
+  return a;
+}
+
+int attn_impl(gn_ctx *c, const KvAttnArgs &a, int dtype) {
+  const KvArgs &kv = a.c;
   // the cache's lengths are on the device: the bound stands for them
-  KTimer kt(c, GN_KCLASS_OTHER, "kv_attention", 2.0 * kv.B * kv.max_len * (double)kv.KVH * kv.hd);
+  const double len = a.view == KV_WINDOW ? std::min((double)kv.max_len, (double)a.sinks + a.window + kv.max_new) : kv.max_len;
+  KTimer kt(c, GN_KCLASS_OTHER, a.view == KV_WINDOW ? "kv_window" : a.view == KV_TREE ? "kv_tree" : "kv_attention",
+            2.0 * kv.B * len * (double)kv.KVH * kv.hd);
   HIP_OK(c, launch_kv_attn(a, dtype, c->scratch, (int64_t)c->scratch_floats, c->stream));
   return GN_OK;
+}
+
+// what the attention calls check alike, and the call
+int attention(gn_ctx *c, KvAttnArgs &a, int dtype, const char *what) {
+  const int64_t w = (int64_t)a.H * a.c.hd;
+  int rc;
+  if ((rc = row_check(c, "q", a.q, a.qs, w, dtype)) || (rc = row_check(c, "out", a.out, a.os, w, dtype))) return rc;
+  if (!a.work && kv_attn_uses_work(a, dtype)) return set_err(c, GN_ERR_INVALID, "%s needs its workspace", what);
+  if ((uintptr_t)a.work & 15) return set_err(c, GN_ERR_INVALID, "%s: work must be 16-byte aligned", what);
+  return attn_impl(c, a, dtype);
 }
 
 }  // namespace
@@ -169,11 +189,11 @@ extern "C" int gn_rope_tables(gn_ctx *c, float *cos, float *sin, int32_t positio
   return GN_OK;
 }
 
-extern "C" int gn_kv_append(gn_ctx *c, const gn_kv_cache *kv, const void *q, const void *k, const void *v, void *q_out,
-                            int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos,
-                            const float *sin, int32_t rope_len, const int32_t *starts, const int32_t *lens, int32_t B,
-                            int32_t N, int32_t max_new, int32_t heads, int32_t dtype, int32_t *bad) {
-  ENTRY(c);
+namespace {
+int append(gn_ctx *c, const gn_kv_cache *kv, const void *q, const void *k, const void *v, void *q_out, int64_t q_stride,
+           int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos, const float *sin, int rope_len,
+           const int32_t *positions, bool by_positions, const int32_t *starts, const int32_t *lens, int B, int N, int max_new,
+           int heads, int dtype, int32_t *bad) {
   KvArgs a{};
   int rc = cache_check(c, kv, a);
   if (rc) return rc;
@@ -181,15 +201,53 @@ extern "C" int gn_kv_append(gn_ctx *c, const gn_kv_cache *kv, const void *q, con
   if (rc) return rc;
   if (!cos != !sin || (cos && rope_len < 0)) return set_err(c, GN_ERR_INVALID, "cos and sin come together");
   if (!q != !q_out) return set_err(c, GN_ERR_INVALID, "q and q_out come together");
-  if (cos) a.limit = std::min(a.limit, rope_len);
+  if (cos && !by_positions) a.limit = std::min(a.limit, rope_len);
   if (B == 0 || N == 0 || max_new == 0) return no_rows(c, a);
+  if (by_positions && cos && (!positions || rope_len < 1))
+    return set_err(c, GN_ERR_INVALID, "rotation needs positions and tables");
   const int64_t kw = (int64_t)a.KVH * a.hd, qw = (int64_t)heads * a.hd;
   if ((rc = row_check(c, "k", k, k_stride, kw, dtype)) || (rc = row_check(c, "v", v, v_stride, kw, dtype))) return rc;
   if (q && ((rc = row_check(c, "q", q, q_stride, qw, dtype)) || (rc = row_check(c, "q_out", q_out, q_out_stride, qw, dtype))))
     return rc;
   if (q == q_out && q && q_stride != q_out_stride)
     return set_err(c, GN_ERR_INVALID, "q_out in place of q needs q's stride");
-  return append_impl(c, a, q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, cos, sin, heads, dtype);
+  return append_impl(c, a, q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, cos, sin, by_positions ? positions : nullptr,
+                     rope_len, heads, dtype);
+}
+}  // namespace
+
+extern "C" int gn_kv_append(gn_ctx *c, const gn_kv_cache *kv, const void *q, const void *k, const void *v, void *q_out,
+                            int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos,
+                            const float *sin, int32_t rope_len, const int32_t *starts, const int32_t *lens, int32_t B,
+                            int32_t N, int32_t max_new, int32_t heads, int32_t dtype, int32_t *bad) {
+  ENTRY(c);
+  return append(c, kv, q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, cos, sin, rope_len, nullptr, false, starts,
+                lens, B, N, max_new, heads, dtype, bad);
+}
+
+extern "C" int gn_kv_append_at(gn_ctx *c, const gn_kv_cache *kv, const void *q, const void *k, const void *v, void *q_out,
+                               int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos,
+                               const float *sin, int32_t rope_len, const int32_t *positions, const int32_t *starts,
+                               const int32_t *lens, int32_t B, int32_t N, int32_t max_new, int32_t heads, int32_t dtype,
+                               int32_t *bad) {
+  ENTRY(c);
+  return append(c, kv, q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, cos, sin, rope_len, positions, true, starts,
+                lens, B, N, max_new, heads, dtype, bad);
+}
+
+extern "C" int gn_kv_keep(gn_ctx *c, const gn_kv_cache *kv, const int32_t *keep, const int32_t *counts, const int32_t *starts,
+                          const int32_t *lens, int32_t B, int32_t N, int32_t max_new, int32_t *bad) {
+  ENTRY(c);
+  KvArgs a{};
+  int rc = cache_check(c, kv, a);
+  if (rc) return rc;
+  rc = batch_check(c, a, starts, lens, B, N, max_new, a.max_pages * a.P, a.KVH, GN_DTYPE_F32, bad);
+  if (rc) return rc;
+  if (B == 0 || N == 0 || max_new == 0) return no_rows(c, a);
+  if (!keep || !counts) return set_err(c, GN_ERR_INVALID, "null pointer");
+  KTimer kt(c, GN_KCLASS_OTHER, "kv_keep", 4.0 * N * (double)a.KVH * a.hd);
+  HIP_OK(c, launch_kv_keep(a, keep, counts, c->stream));
+  return GN_OK;
 }
 
 extern "C" int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max_len, int32_t heads, int32_t kv_heads,
@@ -213,12 +271,51 @@ extern "C" int gn_kv_attention(gn_ctx *c, const gn_kv_cache *kv, const void *q, 
   if (rc) return rc;
   if (!isfinite(scale)) return set_err(c, GN_ERR_INVALID, "scale is not finite");
   if (B == 0 || N == 0 || max_new == 0) return no_rows(c, a);
-  const int64_t w = (int64_t)heads * a.hd;
-  if ((rc = row_check(c, "q", q, q_stride, w, dtype)) || (rc = row_check(c, "out", out, out_stride, w, dtype))) return rc;
-  if (!work && kv_attn_uses_work(a, heads, dtype))
-    return set_err(c, GN_ERR_INVALID, "kv_attention needs its workspace");
-  if ((uintptr_t)work & 15) return set_err(c, GN_ERR_INVALID, "kv_attention: work must be 16-byte aligned");
-  return attn_impl(c, a, q, out, q_stride, out_stride, heads, scale, causal, dtype, work);
+  KvAttnArgs t = attn_args(a, q, out, q_stride, out_stride, heads, scale, causal, dtype, work);
+  return attention(c, t, dtype, "kv_attention");
+}
+
+extern "C" int gn_kv_attention_window(gn_ctx *c, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,
+                                      int64_t out_stride, const int32_t *starts, const int32_t *lens, int32_t B, int32_t N,
+                                      int32_t max_new, int32_t max_len, int32_t heads, float scale, int32_t sinks,
+                                      int32_t window, int32_t dtype, float *work, int32_t *bad) {
+  ENTRY(c);
+  KvArgs a{};
+  int rc = cache_check(c, kv, a);
+  if (rc) return rc;
+  rc = batch_check(c, a, starts, lens, B, N, max_new, max_len, heads, dtype, bad);
+  if (rc) return rc;
+  if (!isfinite(scale)) return set_err(c, GN_ERR_INVALID, "scale is not finite");
+  if (sinks < 0 || window < 0) return set_err(c, GN_ERR_INVALID, "%d first tokens, a window of %d", sinks, window);
+  if (B == 0 || N == 0 || max_new == 0) return no_rows(c, a);
+  KvAttnArgs t = attn_args(a, q, out, q_stride, out_stride, heads, scale, 1, dtype, work);
+  t.view = KV_WINDOW;
+  t.sinks = sinks;
+  t.window = window;
+  return attention(c, t, dtype, "kv_attention_window");
+}
+
+extern "C" int gn_kv_attention_tree(gn_ctx *c, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,
+                                    int64_t out_stride, const uint32_t *mask, int64_t mask_stride, const int32_t *starts,
+                                    const int32_t *lens, int32_t B, int32_t N, int32_t max_new, int32_t max_len, int32_t heads,
+                                    float scale, int32_t dtype, float *work, int32_t *bad) {
+  ENTRY(c);
+  KvArgs a{};
+  int rc = cache_check(c, kv, a);
+  if (rc) return rc;
+  rc = batch_check(c, a, starts, lens, B, N, max_new, max_len, heads, dtype, bad);
+  if (rc) return rc;
+  if (!isfinite(scale)) return set_err(c, GN_ERR_INVALID, "scale is not finite");
+  if (B == 0 || N == 0 || max_new == 0) return no_rows(c, a);
+  if (!mask) return set_err(c, GN_ERR_INVALID, "mask is null");
+  if ((uintptr_t)mask & 3) return set_err(c, GN_ERR_INVALID, "mask is misaligned");
+  if (mask_stride < (std::min(max_new, N) + 31) / 32)
+    return set_err(c, GN_ERR_INVALID, "mask: %lld words do not hold %d bits", (long long)mask_stride, std::min(max_new, N));
+  KvAttnArgs t = attn_args(a, q, out, q_stride, out_stride, heads, scale, 0, dtype, work);
+  t.view = KV_TREE;
+  t.mask = mask;
+  t.ms = mask_stride;
+  return attention(c, t, dtype, "kv_attention_tree");
 }
 
 // ---------------------------------------------------------------------------
@@ -267,13 +364,14 @@ extern "C" int gn_mha_cached_forward(gn_ctx *c, const gn_kv_cache *kv, const flo
     g.bstride_B = nd; g.bstride_bias = nd; g.bstride_C = rows;
     KTimer kt(c, GN_KCLASS_GEMM, "gemm_fwd", gemm_flops(g));
     HIP_OK(c, launch_gemm('N', 'T', EPI_BIAS_ACT, g, c->stream));
-    rc = append_impl(c, a, qkv, qkv + rows, qkv + 2 * rows, qkv, D, D, D, D, cos, sin, a.KVH, GN_DTYPE_F32);
+    rc = append_impl(c, a, qkv, qkv + rows, qkv + 2 * rows, qkv, D, D, D, D, cos, sin, nullptr, rope_len, a.KVH, GN_DTYPE_F32);
     if (rc) return rc;
   }
   // rows outside every sequence are not attention's to write, but wOut reads them
   HIP_OK(c, launch_fill(o, 0.f, (int64_t)N * D, c->stream));
   if (some) {
-    rc = attn_impl(c, a, qkv, o, D, D, a.KVH, (float)(1.0 / sqrt((double)a.hd)), 1, GN_DTYPE_F32, work + 4 * rows);
+    rc = attn_impl(c, attn_args(a, qkv, o, D, D, a.KVH, (float)(1.0 / sqrt((double)a.hd)), 1, GN_DTYPE_F32, work + 4 * rows),
+                   GN_DTYPE_F32);
     if (rc) return rc;
   }
   GemmArgs g{};
@@ -320,5 +418,45 @@ extern "C" int gn_sample(gn_ctx *c, const void *logits, int64_t stride, int32_t 
   a.work = work;
   KTimer kt(c, GN_KCLASS_OTHER, "sample", (double)B * V * (dtype == GN_DTYPE_F32 ? 4 : 2));
   HIP_OK(c, launch_sample(a, dtype, c->stream));
+  return GN_OK;
+}
+
+// ---------------------------------------------------------------- rules on logits
+extern "C" int gn_logits_adjust(gn_ctx *c, const void *logits, int64_t stride, void *out, int64_t out_stride, int32_t dtype,
+                                const gn_logit_rules *rules, int32_t B, int32_t V) {
+  ENTRY(c);
+  if (dtype != GN_DTYPE_F32 && dtype != GN_DTYPE_BF16) return set_err(c, GN_ERR_INVALID, "unknown dtype %d", dtype);
+  if (B < 0 || V < 1) return set_err(c, GN_ERR_INVALID, "B %d, V %d", B, V);
+  if (!rules) return set_err(c, GN_ERR_INVALID, "rules are null");
+  const gn_logit_rules &r = *rules;
+  const bool past = r.repetition || r.frequency || r.presence;
+  if (r.tokens_stride < 0 || r.bias_stride < 0) return set_err(c, GN_ERR_INVALID, "rules: a negative stride");
+  if (past && r.tokens_stride > 0 && !r.tokens) return set_err(c, GN_ERR_INVALID, "penalties need the rows' tokens");
+  if (r.bias_stride > 0 && (!r.bias != !r.bias_ids)) return set_err(c, GN_ERR_INVALID, "bias and bias_ids come together");
+  if (r.allowed && (r.allowed_stride < (V + 31) / 32 || r.allowed_rows < 1 || (!r.allowed_row && r.allowed_rows < B)))
+    return set_err(c, GN_ERR_INVALID, "allowed: %d rows of %lld words for B %d, V %d", r.allowed_rows,
+                   (long long)r.allowed_stride, B, V);
+  if (B > 65535 || V > SAMPLE_MAX_V || r.tokens_stride > LOGITS_MAX_LIST || r.bias_stride > LOGITS_MAX_LIST)
+    return set_err(c, GN_ERR_UNSUPPORTED, "logits_adjust: B %d, V %d or lists beyond 65535 rows of %d", B, V, SAMPLE_MAX_V);
+  if (B == 0) return GN_OK;
+  int rc = row_check(c, "logits", logits, stride, V, dtype);
+  if (rc || (rc = row_check(c, "out", out, out_stride, V, dtype))) return rc;
+  if (((uintptr_t)r.repetition | (uintptr_t)r.frequency | (uintptr_t)r.presence | (uintptr_t)r.tokens | (uintptr_t)r.token_lens |
+       (uintptr_t)r.prompt_lens | (uintptr_t)r.bias_ids | (uintptr_t)r.bias | (uintptr_t)r.bias_lens | (uintptr_t)r.allowed |
+       (uintptr_t)r.allowed_row) & 3)
+    return set_err(c, GN_ERR_INVALID, "rules: a misaligned array");
+  if (logits == out && stride != out_stride) return set_err(c, GN_ERR_INVALID, "out in place of logits needs their stride");
+  LogitArgs a{};
+  a.z = logits;
+  a.out = out;
+  a.zs = stride;
+  a.os = out_stride;
+  a.r = r;
+  if (!past) a.r.tokens_stride = 0;  // a history that nothing is taken from
+  if (!r.bias) a.r.bias_stride = 0;
+  a.B = B;
+  a.V = V;
+  KTimer kt(c, GN_KCLASS_OTHER, "logits_adjust", 2.0 * B * V * (dtype == GN_DTYPE_F32 ? 4 : 2));
+  HIP_OK(c, launch_logits_adjust(a, dtype, c->stream));
   return GN_OK;
 }

@@ -85,7 +85,9 @@ constexpr int KV_TURNS = 2;  // groups of four pairs of queries a thread turns
 // 2048: 45 us for 163 MB, 3.6 TB/s, where a copy reaches 4.9).  Prompts also wait for the
 // vector unit: indexes without divisions, pairs turned once and bytes rounded two at a
 // time brought them from 60.
-template <typename T, int KV_SLOTS>
+// AT: rows turn by positions of their own; one outside the tables makes its query and key
+// NaN.  (A template, so that rows without are given no more registers.)
+template <typename T, int KV_SLOTS, bool AT>
 __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
   const KvArgs &c = a.c;
@@ -117,8 +119,10 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
       const int h = divided(g, a.per_inv, per), d = (g - h * per) * 4;
       const T *row = q + (int64_t)(s.start + t) * a.qs + h * c.hd;
       T *out = qo + (int64_t)(s.start + t) * a.qos + h * c.hd;
-      const float *cs = a.cs ? a.cs + (int64_t)(s.len + t) * half : nullptr;
-      const float *sn = a.cs ? a.sn + (int64_t)(s.len + t) * half : nullptr;
+      const int pos = AT ? a.at[s.start + t] : s.len + t;
+      const bool lost = AT && (unsigned)pos >= (unsigned)a.rope_len;
+      const float *cs = a.cs ? a.cs + (int64_t)(lost ? 0 : pos) * half : nullptr;
+      const float *sn = a.cs ? a.sn + (int64_t)(lost ? 0 : pos) * half : nullptr;
       float lo[4], hi[4];
       if (a.vec) {
         Elem<T>::get4(row + d, lo);
@@ -128,6 +132,10 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
           const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) turn(lo[j], hi[j], cc[j], ss[j]);
+          if (lost) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) lo[j] = hi[j] = __uint_as_float(0x7fc00000u);
+          }
         }
         Elem<T>::put4(out + d, lo);
         Elem<T>::put4(out + d + half, hi);
@@ -135,6 +143,7 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
         for (int j = d; j < min(d + 4, half); ++j) {
           float x = Elem<T>::get(row + j), y = Elem<T>::get(row + j + half);
           if (a.cs) turn(x, y, cs[j], sn[j]);
+          if (lost) x = y = __uint_as_float(0x7fc00000u);
           Elem<T>::put(out + j, x);
           Elem<T>::put(out + j + half, y);
         }
@@ -143,8 +152,9 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
     if (c.hd & 1)  // the last column has no partner; every tile takes its share of the rows
       for (int64_t g = (int64_t)tile * NT + tid; g < (int64_t)s.n * a.H; g += (int64_t)a.qtiles * NT) {
         const int t = (int)(g / a.H), h = (int)(g % a.H);
+        const bool lost = AT && (unsigned)a.at[s.start + t] >= (unsigned)a.rope_len;
         Elem<T>::put(qo + (int64_t)(s.start + t) * a.qos + h * c.hd + c.hd - 1,
-                     Elem<T>::get(q + (int64_t)(s.start + t) * a.qs + h * c.hd + c.hd - 1));
+                     lost ? __uint_as_float(0x7fc00000u) : Elem<T>::get(q + (int64_t)(s.start + t) * a.qs + h * c.hd + c.hd - 1));
       }
     return;
   }
@@ -184,6 +194,13 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
 
   float v[KV_SLOTS][4];
   const T *xs = x + (int64_t)(s.start + first - s.len) * a.xs[which];
+  // the place in the tables of token t of the page, and whether there is none
+  const int32_t *at = AT ? a.at + (s.start + first - s.len) : nullptr;
+  const auto turns = [&](int t) { return AT ? at[t] : first + t; };
+  const auto outside = [&](int p) { return AT && (unsigned)p >= (unsigned)a.rope_len; };
+  if (AT && !which && h == 0 && c.bad)
+    for (int t = lo + tid; t < hi; t += NT)
+      if (outside(at[t])) c.bad[b] = 1;
   // no branch between the loads: all of them under way at once
   if (a.vec) {
 #pragma unroll
@@ -198,9 +215,11 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
       for (int u = 0; u < KV_SLOTS; u += 2) {
         int t, d;
         const bool on = place(u, t, d);
-        const int64_t at = (int64_t)(first + (on ? t : lo)) * half + (on ? d : 0);
-        cs[u / 2] = *reinterpret_cast<const float4 *>(a.cs + at);
-        sn[u / 2] = *reinterpret_cast<const float4 *>(a.sn + at);
+        const int pos = turns(on ? t : lo);
+        const int64_t from = (int64_t)(outside(pos) ? 0 : pos) * half + (on ? d : 0);
+        cs[u / 2] = *reinterpret_cast<const float4 *>(a.cs + from);
+        sn[u / 2] = *reinterpret_cast<const float4 *>(a.sn + from);
+        if (outside(pos)) cs[u / 2] = make_float4(NAN, NAN, NAN, NAN);
       }
 #pragma unroll
       for (int u = 0; u < KV_SLOTS; u += 2) {
@@ -223,9 +242,14 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
     for (int u = 0; u < KV_SLOTS; ++u) {
       int t, d;
       if (!place(u, t, d)) break;
-      const int64_t pos = first + t;
+      const int p = turns(t);
+      const int64_t pos = outside(p) ? 0 : p;
       load_rotated(xs + t * a.xs[which], rot ? a.cs + pos * half : nullptr, rot ? a.sn + pos * half : nullptr, c.hd, d, rot,
                    v[u]);
+      if (rot && outside(p)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[u][k] = d + k < c.hd ? __uint_as_float(0x7fc00000u) : 0.f;
+      }
     }
   }
   const auto largest = [&](auto of) {
@@ -341,6 +365,88 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   }
 }
 
+// ---------------------------------------------------------------- keep
+// Token keep[i] of a sequence's new ones becomes its i-th, i < counts[b].  keep rises, so
+// a token moves to its own place or an earlier one, and from the first that moves on all
+// do.  One workgroup per (sequence, kv head, K or V) takes the pages in rising order: a
+// page's tokens come from it or from later ones, which are as they were then.  The page's
+// scale becomes the largest of its own and those its tokens come from, and all of its
+// bytes are scaled to it; within a page tokens are read before any is written.
+// Latency: a chain of reads (bounds, numbers, pages, scales, bytes), a page after the other.
+__global__ __launch_bounds__(256) void kv_keep_kernel(KvArgs c, const int32_t *keep, const int32_t *counts) {
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int which = blockIdx.x & 1, h = (blockIdx.x >> 1) % c.KVH, b = (blockIdx.x >> 1) / c.KVH, tid = threadIdx.x;
+  const Seq s = kv_seq(c, b, c.limit);
+  const int n = counts[b], R = c.R, P = c.P;
+  if (s.bad || n < 0 || n > s.n) {
+    if (c.bad && tid == 0) c.bad[b] = 1;
+    return;
+  }
+  keep += s.start;
+  const int32_t *table = c.table + (int64_t)b * c.max_pages;
+  const auto missing = [&](int p) { return (unsigned)table[p >> c.lgP] >= (unsigned)c.pages; };
+  int stay = 0;  // tokens that are in their place
+  bool wrong = false;
+  for (int i0 = 0; i0 < n; i0 += 256) {
+    const int i = i0 + tid;
+    bool same = false;
+    if (i < n) {
+      const int k = keep[i], before = i ? keep[i - 1] : -1;
+      same = k == i;
+      wrong |= k < 0 || k <= before || k >= s.n || missing(s.len + k) || missing(s.len + i);
+    }
+    stay += __syncthreads_count(same);
+  }
+  if (__syncthreads_or(wrong)) {
+    if (c.bad && tid == 0) c.bad[b] = 1;
+    return;
+  }
+  uint8_t *cache = which ? c.v : c.k;
+  float *scales = which ? c.vs : c.ks;
+  const auto block = [&](int p) { return (int64_t)table[p >> c.lgP] * c.KVH + h; };
+  for (int at = s.len + stay; at < s.len + n;) {
+    const int first = at >> c.lgP << c.lgP, end = min(s.len + n, first + P), m = end - at;
+    const int64_t blk = block(at);
+    const float own = scales[blk];
+    float scale = own;
+    for (int t = tid; t < m; t += 256) scale = fmaxf(scale, scales[block(s.len + keep[at - s.len + t])]);
+    for (int off = 32; off > 0; off >>= 1) scale = fmaxf(scale, __shfl_xor(scale, off, 64));
+    __shared__ float red[4];
+    if ((tid & 63) == 0) red[tid >> 6] = scale;
+    __syncthreads();
+    scale = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    uint8_t *dst = cache + blk * P * R;
+    if (own < scale) {
+      const float ratio = own / scale;
+      for (int g = tid; g < P * R / 4; g += 256) {
+        uint32_t *w = reinterpret_cast<uint32_t *>(dst) + g;
+        const uint32_t o = *w;
+        *w = rescaled(o & 0xff, ratio) | rescaled(o >> 8 & 0xff, ratio) << 8 | rescaled(o >> 16 & 0xff, ratio) << 16 |
+             rescaled(o >> 24, ratio) << 24;
+      }
+      __syncthreads();
+      if (tid == 0) scales[blk] = scale;
+    }
+    __syncthreads();
+    for (int g = tid; g < m * R; g += 256) {
+      const int t = which ? g % m : g / R, d = which ? g / m : g % R;
+      const int from = s.len + keep[at - s.len + t];
+      const int64_t src = block(from);
+      const int slot = from & (P - 1);
+      const uint32_t byte = cache[src * P * R + (which ? d * P + slot : slot * R + d)];
+      const float had = src == blk ? scale : scales[src];
+      lds[g] = (uint8_t)(had == scale ? byte : rescaled(byte, had / scale));
+    }
+    __syncthreads();
+    for (int g = tid; g < m * R; g += 256) {
+      const int t = which ? g % m : g / R, d = which ? g / m : g % R, slot = at - first + t;
+      dst[which ? d * P + slot : slot * R + d] = lds[g];
+    }
+    __syncthreads();
+    at = end;
+  }
+}
+
 // what the other kernels flag, where a call has no row for them
 __global__ __launch_bounds__(256) void kv_check_kernel(KvArgs c) {
   const int b = blockIdx.x * 256 + threadIdx.x;
@@ -351,6 +457,14 @@ __global__ __launch_bounds__(256) void kv_check_kernel(KvArgs c) {
 
 hipError_t launch_kv_check(const KvArgs &c, hipStream_t s) {
   hipLaunchKernelGGL(kv_check_kernel, dim3((c.B + 255) / 256), dim3(256), 0, s, c);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_keep(const KvArgs &c, const int32_t *keep, const int32_t *counts, hipStream_t s) {
+  const int64_t blocks = (int64_t)c.B * c.KVH * 2;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  const int most = c.max_new < c.P ? c.max_new : c.P;
+  hipLaunchKernelGGL(kv_keep_kernel, dim3((unsigned)blocks), dim3(256), (size_t)most * c.R, s, c, keep, counts);
   return hipGetLastError();
 }
 
@@ -376,8 +490,12 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   // single tokens fill two groups of a thread at most: loads of eight took 6.1 us where
   // theirs take 4 (a token of 4 sequences, 8 heads of 32)
   const bool one = c.max_new == 1;
-  auto fn = one ? kv_append_kernel<float, KV_ONE> : kv_append_kernel<float, KV_MANY>;
-  if (dtype != GN_DTYPE_F32) fn = one ? kv_append_kernel<uint16_t, KV_ONE> : kv_append_kernel<uint16_t, KV_MANY>;
+  auto fn = one ? kv_append_kernel<float, KV_ONE, false> : kv_append_kernel<float, KV_MANY, false>;
+  if (dtype != GN_DTYPE_F32) fn = one ? kv_append_kernel<uint16_t, KV_ONE, false> : kv_append_kernel<uint16_t, KV_MANY, false>;
+  if (a.at) {
+    fn = one ? kv_append_kernel<float, KV_ONE, true> : kv_append_kernel<float, KV_MANY, true>;
+    if (dtype != GN_DTYPE_F32) fn = one ? kv_append_kernel<uint16_t, KV_ONE, true> : kv_append_kernel<uint16_t, KV_MANY, true>;
+  }
   hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(nt), sh, s, a);
   return hipGetLastError();
 }

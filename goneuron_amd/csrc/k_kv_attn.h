@@ -88,15 +88,44 @@ struct Int {
   static constexpr int value = V;
 };
 
+// The first n of 16 bits.
+__device__ __forceinline__ uint32_t first_bits(int n) { return (1u << min(max(n, 0), 16)) - 1u; }
+
+// The keys that the rows row0 .. last of a sequence see, walked without what lies between
+// a window and the first tokens: the i-th of them is key i, from `at` on (a whole step of
+// 64 and so a start of the walk's steps) key i + gap.
+struct Span {
+  int at, gap, end;  // end: how many
+  template <int VIEW>
+  __device__ __forceinline__ int key(int i) const {
+    return VIEW == KV_WINDOW && i >= at ? i + gap : i;
+  }
+};
+template <int VIEW>
+__device__ __forceinline__ Span kv_span(const KvAttnArgs &a, const Seq &s, int row0, int last) {
+  Span p{0, 0, s.len + s.n};
+  if constexpr (VIEW == KV_PREFIX) {
+    if (a.causal) p.end = s.len + last / a.G + 1;
+  } else if constexpr (VIEW == KV_WINDOW) {
+    const int near = max(s.len + row0 / a.G - a.window + 1, 0) & ~63;
+    p.at = (min(a.sinks, near) + 63) & ~63;
+    p.gap = near - p.at;
+    p.end = s.len + last / a.G + 1 - p.gap;
+  }
+  return p;
+}
+
 // The work of one workgroup: a sequence's tile of rows of one key head, over one
 // split of its keys.
 struct Work {
   Seq s;
+  Span span;
   int b, kvh, split;
   int total, rows, row0;  // keys of the sequence, its rows, the workgroup's first
-  int end, k0, k1;        // the last key its rows see + 1, the split's keys
+  int end, k0, k1;        // what its rows see, the split's part of it
   bool any;
 };
+template <int VIEW>
 __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
   const KvArgs &c = a.c;
   Work x;
@@ -112,8 +141,9 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
   x.total = x.s.len + x.s.n;
   x.rows = x.s.n * a.G;
   x.row0 = tile * pl.rows_wg;
-  const int last = min(x.rows, x.row0 + pl.rows_wg) - 1;
-  x.end = a.causal ? x.s.len + max(last, 0) / a.G + 1 : x.total;
+  const int last = max(min(x.rows, x.row0 + pl.rows_wg) - 1, 0);
+  x.span = kv_span<VIEW>(a, x.s, min(x.row0, last), last);
+  x.end = x.span.end;
   x.k0 = x.split * pl.chunk;
   x.k1 = x.end - x.k0 < pl.chunk ? x.end : x.k0 + pl.chunk;  // the sum alone could pass 32 bits
   x.any = x.row0 < x.rows && (x.split == 0 || x.k0 < x.end);
@@ -123,7 +153,7 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
 // A wave's 16 RT rows.  Lane n + 16 g holds, for row n of a tile: the queries'
 // columns of its k slots, sixteen keys' scores of a step, and columns 4 g + i of
 // each 16 of the output.
-template <typename T, int R, int RT>
+template <typename T, int R, int RT, int VIEW>
 struct Rows {
   // bf16 numbers that a query and a weight are cut into
   static constexpr int PARTS = sizeof(T) == 4 ? 3 : 1, WPARTS = sizeof(T) == 4 ? 3 : 2;
@@ -131,7 +161,9 @@ struct Rows {
   bf16x8 q[RT][NK][PARTS];
   f32x4 O[RT][ND], L[RT];  // outputs; sums, as a product with ones (four equal rows)
   float m[RT];             // the reference maxima, in powers of two
-  int lim[RT], lo_lim;     // the last key of each row, of any row
+  int lim[RT], lo_lim;     // the last key of each row (KV_TREE: the last that all rows see), of any row
+  int low[RT], hi_low;     // KV_WINDOW: the first key of each row's window, the last of those
+  const uint32_t *bits[RT];  // KV_TREE: which of the new keys each row sees
   bool seen[RT], every;    // whether a masked step, or any other, held a key of the row
 
   // col(k): the first of this lane's eight columns in the k-th product
@@ -140,14 +172,20 @@ struct Rows {
     // maxima are taken before the factor, which is above 0
     const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
     lo_lim = x.total - 1;
+    hi_low = 0;
     every = false;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int row = row0 + r * 16 + n;
       const bool on = row < x.rows;
       const int t = on ? row / a.G : 0;
-      lim[r] = on && a.causal ? x.s.len + t : x.total - 1;
+      lim[r] = VIEW == KV_TREE ? x.s.len - 1 : on && (VIEW == KV_WINDOW || a.causal) ? x.s.len + t : x.total - 1;
       lo_lim = min(lo_lim, lim[r]);
+      if constexpr (VIEW == KV_WINDOW) {
+        low[r] = on ? max(lim[r] - a.window + 1, 0) : 0;
+        hi_low = max(hi_low, low[r]);
+      }
+      if constexpr (VIEW == KV_TREE) bits[r] = a.mask + (int64_t)(x.s.start + t) * a.ms;
       const T *p = (const T *)a.q + (int64_t)(x.s.start + t) * a.qs + (int64_t)(x.kvh * a.G + (on ? row % a.G : 0)) * a.c.hd;
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
@@ -174,14 +212,39 @@ struct Rows {
     }
     for (int o = 8; o > 0; o >>= 1) lo_lim = min(lo_lim, __shfl_xor(lo_lim, o, 64));
     lo_lim = __builtin_amdgcn_readfirstlane(lo_lim);
+    if constexpr (VIEW == KV_WINDOW) {
+      for (int o = 8; o > 0; o >>= 1) hi_low = max(hi_low, __shfl_xor(hi_low, o, 64));
+      hi_low = __builtin_amdgcn_readfirstlane(hi_low);
+    }
   }
+  // whether every row sees the 64 keys from j on
+  __device__ __forceinline__ bool clear(const KvAttnArgs &a, int j) const {
+    return j + 63 <= lo_lim && (VIEW != KV_WINDOW || j >= hi_low || j + 63 < a.sinks);
+  }
+  // Which of the sixteen keys from `first` on row r sees: how many (KV_PREFIX), else a
+  // bit each.
+  static constexpr int ALL = VIEW == KV_PREFIX ? 16 : 0xffff;
+  __device__ __forceinline__ int sees(const KvAttnArgs &a, const Work &x, int r, int first) const {
+    if constexpr (VIEW == KV_PREFIX) return max(0, min(16, lim[r] - first + 1));
+    if constexpr (VIEW == KV_WINDOW)
+      return (int)(first_bits(lim[r] - first + 1) & (~first_bits(low[r] - first) | first_bits(a.sinks - first)));
+    const int at = first - x.s.len;  // the number of the first as a new token
+    uint32_t w = first_bits(-at);
+    if (at > -16 && at < x.s.n) {
+      const int i = max(at, 0) >> 5;
+      const uint32_t lo = bits[r][i], hi = i * 32 + 32 < x.s.n ? bits[r][i + 1] : 0;
+      w |= at < 0 ? lo << -at : (uint32_t)((((uint64_t)hi << 32) | lo) >> (at & 31));
+    }
+    return (int)(w & first_bits(x.total - first));
+  }
+  static __device__ __forceinline__ bool in_sight(int see, int k) { return VIEW == KV_PREFIX ? k < see : see >> k & 1; }
 
   // the lane's sixteen keys that the row does not see leave the scores
   __device__ __forceinline__ void mask(int r, f32x4 (&S)[4], int see) {
     asm volatile("" : "+v"(see));  // keeps the comparisons out of steps without a mask
     seen[r] |= see > 0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) S[k >> 2][k & 3] = k < see ? S[k >> 2][k & 3] : -INFINITY;
+    for (int k = 0; k < 16; ++k) S[k >> 2][k & 3] = in_sight(see, k) ? S[k >> 2][k & 3] : -INFINITY;
   }
   // scores S (before the factor sf > 0) of tile r to weights, as the second
   // product's operands
@@ -225,7 +288,7 @@ struct Rows {
       u32x4 on;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        on[k] = (8 * h + 2 * k < see ? 0x3f80u : 0u) | (8 * h + 2 * k + 1 < see ? 0x3f800000u : 0u);
+        on[k] = (in_sight(see, 8 * h + 2 * k) ? 0x3f80u : 0u) | (in_sight(see, 8 * h + 2 * k + 1) ? 0x3f800000u : 0u);
       hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(is[h], as_bf16x8(on), hit, 0, 0, 0);
     }
 #pragma unroll
@@ -317,20 +380,24 @@ __device__ __forceinline__ int v_place(int row, int chunk) { return chunk ^ ((ro
 // 2048, 32 heads of 128 over 8, bfloat16, in 307 us, 206 GFLOP at 672 TFLOP/s of the
 // definition's products and, the weights' second part among them, 1007 of the units' (a
 // product of 16384^3 reaches 1369 here); the waves wait for LDS and the barrier.
-template <typename T, int R, int RT>
+template <typename T, int R, int RT, int VIEW>
 __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int NK = R / 32, ND = R / 16;
   extern __shared__ __align__(16) uint8_t lds[];
   const KvArgs &c = a.c;
-  const Work x = kv_work(a, pl);
+  const Work x = kv_work<VIEW>(a, pl);
   if (!x.any) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, g = lane >> 4;
   const int row0 = x.row0 + w * 16 * RT;
   // the last key that this wave's rows see
   const int my_last = min(x.rows, row0 + 16 * RT) - 1;
-  const int my_end = row0 >= x.rows ? 0 : a.causal ? x.s.len + my_last / a.G + 1 : x.total;
+  const int my_end = row0 >= x.rows                                       ? 0
+                     : VIEW == KV_WINDOW || (VIEW == KV_PREFIX && a.causal) ? x.s.len + my_last / a.G + 1
+                                                                            : x.total;
+  // where this wave's windows begin
+  const int my_low = VIEW == KV_WINDOW ? x.s.len + row0 / a.G - a.window + 1 : 0;
   const float sf = kv_factor(a.scale);
-  Rows<T, R, RT> A;
+  Rows<T, R, RT, VIEW> A;
   A.init(a, x, row0, n, [&](int k) { return k * 32 + g * 8; });
 
   const int32_t *table = c.table + (int64_t)x.b * c.max_pages;
@@ -352,12 +419,16 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
   const auto in = [&](int q) { return CH % 256 == 0 || q < CH; };
   const auto chunk = [&](int i) { return in(tid + i * 256) ? tid + i * 256 : 0; };
   const int gv = tid & 3;
+  // whether some row may see one of the 16 keys from j on: pages that none does need not be
+  // there, nor hold a scale
+  const int reach = VIEW == KV_WINDOW ? x.s.len + x.row0 / a.G - a.window + 1 : 0;
+  const auto in_reach = [&](int j) { return VIEW != KV_WINDOW || j + 15 >= reach || j < a.sinks; };
   const auto pages = [&](int j) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) pk[i] = SAME && i ? pk[0] : page_at(j + ((chunk(i) / KC & 15) >> 2) * 16);
     pv = page_at(j + gv * 16);
   };
-  const auto load = [&](int j) {
+  const auto load = [&](int j, int next) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int q = chunk(i), row = q / KC, tok = ((row & 15) >> 2) * 16 + (row >> 4) * 4 + (row & 3);
@@ -367,7 +438,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
       if (!(SAME && i)) ksc[i] = c.ks[(int64_t)p * c.KVH + x.kvh];
       ksc[i] = SAME && i ? ksc[0] : on ? ksc[i] : 1.f;
     }
-    const bool on = (unsigned)pv < (unsigned)c.pages;
+    const bool near = in_reach(j + gv * 16), on = near && (unsigned)pv < (unsigned)c.pages;
     const int p = on ? pv : 0;
     const uint8_t *v = vb + p * page_bytes + ((j + gv * 16) & (c.P - 1));
 #pragma unroll
@@ -376,12 +447,19 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
     vsc = on ? vsc : 1.f;
     have = on ? x.total - (j + gv * 16) : 0;
     there = __ballot(on);
-    if (!on && j + gv * 16 < x.total && c.bad) c.bad[x.b] = 1;
-    pages(j + 64);
+    if (!on && j + gv * 16 < x.total && near && c.bad) c.bad[x.b] = 1;
+    pages(next);
   };
   // the first key that some row of the workgroup does not see
-  const int wg_lim = a.causal ? x.s.len + x.row0 / a.G + 1 : x.total;
-  int *first_nan = reinterpret_cast<int *>(lds + 512 * R);
+  const int wg_lim = VIEW == KV_TREE ? x.s.len : VIEW == KV_WINDOW || a.causal ? x.s.len + x.row0 / a.G + 1 : x.total;
+  // the first that all windows hold
+  const int wg_low = VIEW == KV_WINDOW ? x.s.len + (min(x.rows, x.row0 + pl.rows_wg) - 1) / a.G - a.window + 1 : 0;
+  const auto masked = [&](int j) { return j + 64 > wg_lim || (VIEW == KV_WINDOW && j < wg_low && j + 63 >= a.sinks); };
+  int *first_nan = reinterpret_cast<int *>(lds + 512 * R);  // KV_PREFIX
+  // other views: a bit for each of a step's 64 keys that holds NaN in a column, for two
+  // steps; the step (key + 1) whose bits hold any
+  uint16_t *nan_bits = reinterpret_cast<uint16_t *>(lds + 512 * R);
+  int *nan_step = reinterpret_cast<int *>(lds + 528 * R);
   const auto spread = [&](int buf, int j) {
     uint8_t *kl = lds + buf * (256 * R), *vl = kl + 128 * R;
     if (have < 16) {  // keys behind the sequence, or of a page that is not there: 0
@@ -395,17 +473,27 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
         }
       }
     }
-    if (j + 64 > wg_lim) {
+    if (masked(j)) {
       // masked weights are 0, but 0 * NaN is not: NaN leaves V, and the first key that
-      // has it in a column is noted (a row sees it if it sees that key)
+      // has it in a column is noted (a row sees it if it sees that key), or every one
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         uint32_t *v = reinterpret_cast<uint32_t *>(&vr[i]);
-        if (!has_nan(v[0]) && !has_nan(v[1]) && !has_nan(v[2]) && !has_nan(v[3])) continue;
+        const bool any = has_nan(v[0]) || has_nan(v[1]) || has_nan(v[2]) || has_nan(v[3]);
+        if (VIEW != KV_PREFIX && in(tid + i * 256)) nan_bits[(buf * R + (chunk(i) >> 2)) * 4 + gv] = 0;
+        if (!any) continue;
+        uint32_t found = 0;
         for (int k = 15; k >= 0; --k) {
           const int at = k >> 2, sh = 8 * (k & 3);
           const uint32_t word = at == 0 ? v[0] : at == 1 ? v[1] : at == 2 ? v[2] : v[3];
-          if ((word >> sh & 0x7f) == 0x7f) atomicMin(&first_nan[chunk(i) >> 2], j + gv * 16 + k);
+          if ((word >> sh & 0x7f) == 0x7f) {
+            if constexpr (VIEW == KV_PREFIX) atomicMin(&first_nan[chunk(i) >> 2], j + gv * 16 + k);
+            else found |= 1u << k;
+          }
+        }
+        if (VIEW != KV_PREFIX && in(tid + i * 256)) {
+          nan_bits[(buf * R + (chunk(i) >> 2)) * 4 + gv] = (uint16_t)found;
+          nan_step[buf] = j + 1;
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -466,12 +554,33 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
       vf[d][0] = v_at(d, 0);
       vf[d][1] = v_at(d, 1);
     }
-    if (j + 63 > A.lo_lim || groups != 15) {
+    int see[RT];
+    if (!A.clear(a, j) || groups != 15) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
-        A.mask(r, S[r], groups >> g & 1 ? max(0, min(16, A.lim[r] - (j + 16 * g) + 1)) : 0);
+      for (int r = 0; r < RT; ++r) {
+        see[r] = groups >> g & 1 ? A.sees(a, x, r, j + 16 * g) : 0;
+        A.mask(r, S[r], see[r]);
+      }
     } else {
       A.every = true;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) see[r] = A.ALL;
+    }
+    if constexpr (VIEW != KV_PREFIX) {
+      if (nan_step[buf] == j + 1) {  // NaN that left V, for the rows that see it
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          uint64_t row = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) row |= (uint64_t)(uint32_t)__shfl(see[r], n + 16 * k, 64) << (16 * k);
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (reinterpret_cast<const uint64_t *>(nan_bits)[buf * R + d * 16 + 4 * g + i] & row)
+                A.O[r][d][i] = __uint_as_float(0x7fc00000u);
+        }
+      }
     }
     bf16x8 pf[RT][2][A.WPARTS];
 #pragma unroll
@@ -492,33 +601,41 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
     }
   };
 
-  for (int d = tid; d < R; d += 256) first_nan[d] = 0x7fffffff;
+  const auto key = [&](int i) { return x.span.key<VIEW>(i); };
+  if constexpr (VIEW == KV_PREFIX) {
+    for (int d = tid; d < R; d += 256) first_nan[d] = 0x7fffffff;
+  } else if (tid < 2) {
+    nan_step[tid] = 0;
+  }
   if (x.k0 < x.k1) {
-    pages(x.k0);
-    load(x.k0);
+    pages(key(x.k0));
+    load(key(x.k0), key(x.k0 + 64));
     __syncthreads();
-    spread(0, x.k0);
+    spread(0, key(x.k0));
     __syncthreads();
   }
-  for (int j = x.k0; j < x.k1; j += 64) {
-    const bool more = j + 64 < x.k1;
+  for (int i = x.k0; i < x.k1; i += 64) {
+    const bool more = i + 64 < x.k1;
+    const int j = key(i), then = key(i + 64);
     groups = there & 15;
-    if (more) load(j + 64);
-    if (j < my_end) step(j);
-    if (more) spread(buf ^ 1, j + 64);
+    if (more) load(then, key(i + 128));
+    if (j < my_end && (VIEW != KV_WINDOW || j + 63 >= my_low || j < a.sinks)) step(j);
+    if (more) spread(buf ^ 1, then);
     __syncthreads();
     buf ^= 1;
   }
   A.finish();
+  if constexpr (VIEW == KV_PREFIX) {
 #pragma unroll
-  for (int d = 0; d < ND; ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int nan = first_nan[d * 16 + 4 * g + i];
+      for (int i = 0; i < 4; ++i) {
+        const int nan = first_nan[d * 16 + 4 * g + i];
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
-        if (A.lim[r] >= nan) A.O[r][d][i] = __uint_as_float(0x7fc00000u);
-    }
+        for (int r = 0; r < RT; ++r)
+          if (A.lim[r] >= nan) A.O[r][d][i] = __uint_as_float(0x7fc00000u);
+      }
+  }
   A.store(a, pl, x, row0, n, g);
 }
 
@@ -531,17 +648,17 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
 // join, 4.7 TB/s of cache (43 us alone: 6.2, as fast as memory is read here; float32
 // queries without shared heads 50, 5.4); 64 sequences of up to 8192 in 121 us, 4.4 TB/s.
 // A step of 5 us at the least.
-template <typename T, int R>
+template <typename T, int R, int VIEW>
 __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void kv_attn_keys_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int NK = R / 32, ND = R / 16;
   constexpr bool LEAN = R >= 192;  // registers hold K or V, not both
   extern __shared__ __align__(16) float join[];
   const KvArgs &c = a.c;
-  const Work x = kv_work(a, pl);
+  const Work x = kv_work<VIEW>(a, pl);
   if (!x.any) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, g = lane >> 4;
   const float sf = kv_factor(a.scale);
-  Rows<T, R, 1> A;
+  Rows<T, R, 1, VIEW> A;
   A.init(a, x, x.row0, n, [&](int k) { return k < R / 64 * 2 ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 : R / 64 * 64 + g * 8; });
 
   const int32_t *table = c.table + (int64_t)x.b * c.max_pages;
@@ -583,15 +700,19 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
     }
   };
 
-  int j = x.k0 + w * 64, page = 0, next = 0;
+  const auto key = [&](int i) { return x.span.key<VIEW>(i); };
+  // pages that no row sees need not be there, nor hold a scale
+  const int reach = VIEW == KV_WINDOW ? x.s.len + x.row0 / a.G - a.window + 1 : 0;
+  const auto in_reach = [&](int at) { return VIEW != KV_WINDOW || at + 15 >= reach || at < a.sinks; };
+  int j = 0, page = 0, next = 0;
   bool ok = false;
   // a step's page (0 where there is none), K and scales, and the page after it
-  const auto advance = [&](int at, int p) {
-    ok = (unsigned)p < (unsigned)c.pages;
+  const auto advance = [&](int i, int p) {
+    ok = (unsigned)p < (unsigned)c.pages && in_reach(key(i) + 16 * g);
     page = ok ? p : 0;
-    load_k(at, page);
+    load_k(key(i), page);
     vsc = c.vs[(int64_t)page * c.KVH + x.kvh];
-    next = page_at(at + STEP);
+    next = page_at(key(i + STEP));
   };
 
   const auto step = [&](auto clean_, auto &&between) {
@@ -608,7 +729,7 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
     }
     between();  // K's registers are free
     bf16x8 pf[2][A.WPARTS];
-    const int see = CLEAN ? 16 : was_ok ? max(0, min(16, A.lim[0] - first + 1)) : 0;
+    const int see = CLEAN ? A.ALL : was_ok ? A.sees(a, x, 0, first) : 0;
     if constexpr (CLEAN) A.every = true;
     else A.mask(0, S, see);
     A.weights(0, S, sf, pf);
@@ -649,19 +770,21 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
     }
   };
 
-  if (j < x.k1) advance(j, page_at(j));
-  for (; j < x.k1; j += STEP) {
-    const bool more = j + STEP < x.k1, here = ok;
-    if (!here && j + 16 * g < x.total && c.bad) c.bad[x.b] = 1;
+  int i = x.k0 + w * 64;
+  if (i < x.k1) advance(i, page_at(key(i)));
+  for (; i < x.k1; i += STEP) {
+    j = key(i);
+    const bool more = i + STEP < x.k1, here = ok;
+    if (!here && j + 16 * g < x.total && in_reach(j + 16 * g) && c.bad) c.bad[x.b] = 1;
     if constexpr (!LEAN) load_v(j, page);  // on its way while the scores are computed
     const auto between = [&]() {
       if constexpr (LEAN) load_v(j, page);
-      else if (more) advance(j + STEP, next);
+      else if (more) advance(i + STEP, next);
     };
-    if (j + 63 <= A.lo_lim && __all(here)) step(Int<1>(), between);
+    if (A.clear(a, j) && __all(here)) step(Int<1>(), between);
     else step(Int<0>(), between);
     if constexpr (LEAN)
-      if (more) advance(j + STEP, next);
+      if (more) advance(i + STEP, next);
   }
   A.finish();
 
@@ -702,7 +825,7 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
 // where few rows have few splits (2048 rows of 8: 7 us, 12 with one), 16 where they
 // have many (32 rows of 64: 8 us; one wave alone waits for a load per split, 150 us
 // at 128).
-template <typename T, int WAVES>
+template <typename T, int WAVES, int VIEW>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void kv_join_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int U = KV_MAX_HEAD / 64;
   const KvArgs &c = a.c;
@@ -714,8 +837,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void kv_join_kernel(
   if (t >= s.n) return;
   // what the row's workgroup saw, as it counted it
   const int row = t * a.G + h % a.G, wg0 = row / pl.rows_wg * pl.rows_wg;
-  const int wg_last = min(s.n * a.G, wg0 + pl.rows_wg) - 1;
-  const int wg_end = a.causal ? s.len + wg_last / a.G + 1 : s.len + s.n;
+  const int wg_end = kv_span<VIEW>(a, s, wg0, min(s.n * a.G, wg0 + pl.rows_wg) - 1).end;
   if (wg_end <= pl.chunk) return;
   const int n = (wg_end - 1) / pl.chunk + 1;
   const float *ml = a.work + slot * 2;
@@ -775,36 +897,37 @@ hipError_t kv_attn_run(F fn, std::atomic<int> (&set)[kAttrDevices], int lds, con
   hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), lds, s, a, p);
   return hipGetLastError();
 }
-template <typename T, int R>
+template <typename T, int R, int VIEW>
 hipError_t kv_attn_rows(const KvAttnArgs &a, const KvPlan &p, hipStream_t s) {
   static std::atomic<int> set[3][kAttrDevices];
   if (!p.by_rows)  // two waves' outputs
-    return kv_attn_run(kv_attn_keys_kernel<T, R>, set[0], 2 * (R / 16 * 4 + 3) * 64 * 4, a, p, s);
-  const int lds = 516 * R;  // two steps' K and V, and where V holds NaN
+    return kv_attn_run(kv_attn_keys_kernel<T, R, VIEW>, set[0], 2 * (R / 16 * 4 + 3) * 64 * 4, a, p, s);
+  // two steps' K and V, and where V holds NaN
+  constexpr int lds = VIEW == KV_PREFIX ? 516 * R : 528 * R + 16;
   if constexpr (R <= kv_two_tiles(sizeof(T)))
-    if (p.rt == 2) return kv_attn_run(kv_attn_rows_kernel<T, R, 2>, set[1], lds, a, p, s);
-  return kv_attn_run(kv_attn_rows_kernel<T, R, 1>, set[2], lds, a, p, s);
+    if (p.rt == 2) return kv_attn_run(kv_attn_rows_kernel<T, R, 2, VIEW>, set[1], lds, a, p, s);
+  return kv_attn_run(kv_attn_rows_kernel<T, R, 1, VIEW>, set[2], lds, a, p, s);
 }
-template <typename T>
+template <typename T, int VIEW>
 hipError_t kv_attn_typed(const KvAttnArgs &a, const KvPlan &p, hipStream_t s) {
   const KvArgs &c = a.c;
   hipError_t e = hipErrorInvalidValue;
   switch (c.R) {
-    case 32: e = kv_attn_rows<T, 32>(a, p, s); break;
-    case 64: e = kv_attn_rows<T, 64>(a, p, s); break;
-    case 96: e = kv_attn_rows<T, 96>(a, p, s); break;
-    case 128: e = kv_attn_rows<T, 128>(a, p, s); break;
-    case 192: e = kv_attn_rows<T, 192>(a, p, s); break;
-    case 256: e = kv_attn_rows<T, 256>(a, p, s); break;
+    case 32: e = kv_attn_rows<T, 32, VIEW>(a, p, s); break;
+    case 64: e = kv_attn_rows<T, 64, VIEW>(a, p, s); break;
+    case 96: e = kv_attn_rows<T, 96, VIEW>(a, p, s); break;
+    case 128: e = kv_attn_rows<T, 128, VIEW>(a, p, s); break;
+    case 192: e = kv_attn_rows<T, 192, VIEW>(a, p, s); break;
+    case 256: e = kv_attn_rows<T, 256, VIEW>(a, p, s); break;
   }
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t slots = (int64_t)c.B * c.max_new * a.H;
   if (slots >= 16384)
-    hipLaunchKernelGGL((kv_join_kernel<T, 1>), dim3((unsigned)((slots + 3) / 4)), dim3(256), 0, s, a, p);
+    hipLaunchKernelGGL((kv_join_kernel<T, 1, VIEW>), dim3((unsigned)((slots + 3) / 4)), dim3(256), 0, s, a, p);
   else if (p.splits <= 16)
-    hipLaunchKernelGGL((kv_join_kernel<T, 4>), dim3((unsigned)slots), dim3(256), 0, s, a, p);
+    hipLaunchKernelGGL((kv_join_kernel<T, 4, VIEW>), dim3((unsigned)slots), dim3(256), 0, s, a, p);
   else
-    hipLaunchKernelGGL((kv_join_kernel<T, 16>), dim3((unsigned)slots), dim3(1024), 0, s, a, p);
+    hipLaunchKernelGGL((kv_join_kernel<T, 16, VIEW>), dim3((unsigned)slots), dim3(1024), 0, s, a, p);
   return hipGetLastError();
 }
 

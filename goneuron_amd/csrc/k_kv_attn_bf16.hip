@@ -3,6 +3,6 @@
 
 namespace gn {
 hipError_t launch_kv_attn_bf16(const KvAttnArgs &a, const KvPlan &p, hipStream_t s) {
-  return kv_attn_typed<uint16_t>(a, p, s);
+  return kv_attn_typed<uint16_t, KV_PREFIX>(a, p, s);
 }
 }  // namespace gn

@@ -19,7 +19,9 @@ static int64_t kv_splits(bool by_rows, int64_t items, int64_t len) {
   return std::max<int64_t>(splits, 1);
 }
 
-static KvPlan kv_plan(int B, int max_new, int max_len, int H, int KVH, int R, int bytes) {
+static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
+  const int B = a.c.B, max_new = a.c.max_new, H = a.H, KVH = a.c.KVH, R = a.c.R;
+  const int bytes = dtype == GN_DTYPE_F32 ? 4 : 2;
   KvPlan p{};
   const int64_t rows = (int64_t)max_new * (H / KVH);
   // up to one tile of rows the waves share it and split the keys; beyond, every
@@ -31,7 +33,13 @@ static KvPlan kv_plan(int B, int max_new, int max_len, int H, int KVH, int R, in
   p.rows_wg = 16 * p.rt * (p.by_rows ? 4 : 1);
   p.tiles = (int)((rows + p.rows_wg - 1) / p.rows_wg);
   const int64_t items = (int64_t)B * KVH * p.tiles, unit = p.by_rows ? 64 : 256;
-  const int64_t len = std::min(std::max(max_len, 1), KV_MAX_TOKENS);  // no table holds more
+  int64_t len = std::min(std::max(a.c.max_len, 1), KV_MAX_TOKENS);  // no table holds more
+  if (a.view == KV_WINDOW) {
+    // what the rows of a workgroup see at most: whole steps of the first tokens, and from
+    // its first row's window, rounded to a step, to its last row
+    const int64_t tokens = std::min<int64_t>(max_new, (p.rows_wg - 1) / a.G + 2);
+    len = std::min(len, ((int64_t)a.sinks + 63) / 64 * 64 + a.window + tokens + 63);
+  }
   const int64_t splits = kv_splits(p.by_rows, items, len), chunk = (len + splits - 1) / splits;
   p.chunk = (int)((chunk + unit - 1) / unit * unit);
   p.splits = (int)((len + p.chunk - 1) / p.chunk);  // no more than kv_splits: chunks only grow
@@ -67,14 +75,12 @@ int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int
   return most ? kv_part_floats(most, R) : 0;
 }
 
-bool kv_attn_uses_work(const KvArgs &c, int H, int dtype) {
-  return kv_plan(c.B, c.max_new, c.max_len, H, c.KVH, c.R, dtype == GN_DTYPE_F32 ? 4 : 2).work;
-}
+bool kv_attn_uses_work(const KvAttnArgs &a, int dtype) { return kv_plan(a, dtype).work; }
 
 hipError_t launch_kv_attn(const KvAttnArgs &a0, int dtype, float *scratch, int64_t scratch_floats, hipStream_t s) {
   KvAttnArgs a = a0;
   const KvArgs &c = a.c;
-  KvPlan p = kv_plan(c.B, c.max_new, c.max_len, a.H, c.KVH, c.R, dtype == GN_DTYPE_F32 ? 4 : 2);
+  KvPlan p = kv_plan(a, dtype);
   if (p.splits > 1 && !p.work) {
     a.work = scratch;
     if (kv_part_floats((int64_t)p.splits * c.B * c.max_new * a.H, c.R) > scratch_floats) {
@@ -82,7 +88,10 @@ hipError_t launch_kv_attn(const KvAttnArgs &a0, int dtype, float *scratch, int64
       p.chunk = c.max_len;
     }
   }
-  return dtype == GN_DTYPE_F32 ? kv_attn_typed<float>(a, p, s) : launch_kv_attn_bf16(a, p, s);
+  const bool f32 = dtype == GN_DTYPE_F32;
+  if (a.view == KV_WINDOW) return f32 ? launch_kv_window_f32(a, p, s) : launch_kv_window_bf16(a, p, s);
+  if (a.view == KV_TREE) return f32 ? launch_kv_tree_f32(a, p, s) : launch_kv_tree_bf16(a, p, s);
+  return f32 ? kv_attn_typed<float, KV_PREFIX>(a, p, s) : launch_kv_attn_bf16(a, p, s);
 }
 
 }  // namespace gn

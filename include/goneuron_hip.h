@@ -613,6 +613,47 @@ int gn_kv_attention(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out
                     int64_t out_stride, const int32_t *starts, const int32_t *lens, int32_t B, int32_t N,
                     int32_t max_new, int32_t max_len, int32_t heads, float scale, int32_t causal, int32_t dtype,
                     float *work, int32_t *bad);
+/* gn_kv_attention for long streams: a query at position p sees the first `sinks` tokens
+ * and the last `window` up to its own, p - window + 1 .. p.  Of both 0 a query sees
+ * nothing and gives 0.  Pages that no query of the call sees may be gone: their entries
+ * in the table may hold anything.  work: gn_kv_attention_workspace floats, as
+ * gn_kv_attention's. */
+int gn_kv_attention_window(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,
+                           int64_t out_stride, const int32_t *starts, const int32_t *lens, int32_t B, int32_t N,
+                           int32_t max_new, int32_t max_len, int32_t heads, float scale, int32_t sinks, int32_t window,
+                           int32_t dtype, float *work, int32_t *bad);
+
+/* Drafted tokens: a tree of guesses is appended, attended to and drawn for in one
+ * step, and the path that turns out right is kept.
+ * gn_kv_append for rows whose positions are not those of their places: the token of row r
+ * is stored as its sequence's next one as gn_kv_append stores it, and it and its query turn
+ * by (cos, sin)[positions[r]] (positions: N int32 on the device; two guesses for one place
+ * have one position).  A position outside [0, rope_len) makes the row's query and key NaN
+ * and flags its sequence.  Without cos and sin positions may be null. */
+int gn_kv_append_at(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, const void *k, const void *v, void *q_out,
+                    int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t q_out_stride, const float *cos,
+                    const float *sin, int32_t rope_len, const int32_t *positions, const int32_t *starts,
+                    const int32_t *lens, int32_t B, int32_t N, int32_t max_new, int32_t heads, int32_t dtype,
+                    int32_t *bad);
+/* gn_kv_attention of new tokens that see all lens[b] cached ones and, of their sequence's
+ * new ones, those that a mask names: bit j % 32 of word j / 32 of row r (mask: N rows,
+ * mask_stride words apart, of a bit for each of up to max_new tokens) says that the token
+ * of row r sees its sequence's j-th new token.  Its own bit is like any other; bits behind
+ * the sequence's new tokens are not looked at.  work: gn_kv_attention_workspace floats. */
+int gn_kv_attention_tree(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,
+                         int64_t out_stride, const uint32_t *mask, int64_t mask_stride, const int32_t *starts,
+                         const int32_t *lens, int32_t B, int32_t N, int32_t max_new, int32_t max_len, int32_t heads,
+                         float scale, int32_t dtype, float *work, int32_t *bad);
+/* Keeps counts[b] (B int32) of a sequence's new tokens: the keep[starts[b] + i]-th
+ * becomes the i-th, i < counts[b]; their numbers rise (keep: N int32, those behind the
+ * counts are not looked at).  The caller advances lens[b] by counts[b].  Where tokens
+ * move into a block (one page, one head, K or V apart), its scale becomes the largest of its
+ * own and those of the blocks they come from, and all bytes of the block are scaled to it
+ * (exact but for what falls below the smallest E4M3 step).  The pages of the new tokens
+ * belong to one sequence.  bad as above: set for a sequence that is skipped whole because
+ * its bounds, counts or numbers are wrong or a page is outside [0, pages). */
+int gn_kv_keep(gn_ctx *ctx, const gn_kv_cache *kv, const int32_t *keep, const int32_t *counts, const int32_t *starts,
+               const int32_t *lens, int32_t B, int32_t N, int32_t max_new, int32_t *bad);
 /* MultiHeadAttention (transformer.go:405-529) for new tokens of B sequences
  * over such a cache: x and out are N rows of D floats, params as
  * gn_mha_forward's; Q, K, V of the new tokens, rotated where cos and sin are
@@ -628,6 +669,35 @@ int gn_mha_cached_forward(gn_ctx *ctx, const gn_kv_cache *kv, const float *x, co
                           const float *cos, const float *sin, int32_t rope_len, const int32_t *starts,
                           const int32_t *lens, int32_t B, int32_t N, int32_t max_new, int32_t max_len, int32_t D,
                           float *work, int32_t *bad);
+/* Rules for B rows of V logits, all arrays on the device; a null pointer leaves its rule
+ * out.  Row b's text is the first token_lens[b] of tokens[b * tokens_stride ..] (null: all
+ * tokens_stride), the first prompt_lens[b] of them (null: none) the prompt; its biases the
+ * first bias_lens[b] (null: all) of bias_ids and bias [b * bias_stride ..].  Lengths below 0
+ * count as 0, above the stride as the stride, ids outside [0, V) as none.  Row
+ * allowed_row[b] (null: b) of `allowed`, allowed_stride words of 32 tokens, lowest bit
+ * first, names the tokens that may follow; a number outside [0, allowed_rows): all may. */
+typedef struct gn_logit_rules {
+  const float *repetition, *frequency, *presence; /* B each */
+  const int32_t *tokens, *token_lens, *prompt_lens;
+  int64_t tokens_stride;
+  const int32_t *bias_ids;
+  const float *bias;
+  const int32_t *bias_lens;
+  int64_t bias_stride;
+  const uint32_t *allowed;
+  const int32_t *allowed_row;
+  int64_t allowed_stride;
+  int32_t allowed_rows;
+} gn_logit_rules;
+/* out (may be logits itself, with their stride) = the logits under the rules, for
+ * gn_sample.  In this order, in float32: a token of the text has a logit above 0 divided by
+ * repetition[b], any other multiplied by it (a repetition that is not above 0 counts as 1);
+ * one that stands n > 0 times behind the prompt loses frequency[b] n and then presence[b];
+ * one with a bias gains it (of several the last entry's); one that may not follow becomes
+ * -inf, whatever it was.  Rows may be anything that gn_sample takes.  V <= 2^20, lists of a
+ * row <= 2^30. */
+int gn_logits_adjust(gn_ctx *ctx, const void *logits, int64_t stride, void *out, int64_t out_stride, int32_t dtype,
+                     const gn_logit_rules *rules, int32_t B, int32_t V);
 /* Draws one index of each of B rows of V logits (row stride in elements, dtype)
  * with the given random number u[b] in [0, 1).  With m the row's largest logit,
  * w_i = exp((z_i - m) / temperature[b]); NaN and -inf logits are left out.  Kept
