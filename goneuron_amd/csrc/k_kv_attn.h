@@ -161,9 +161,8 @@ struct Rows {
   bf16x8 q[RT][NK][PARTS];
   f32x4 O[RT][ND], L[RT];  // outputs; sums, as a product with ones (four equal rows)
   float m[RT];             // the reference maxima, in powers of two
-  int lim[RT], lo_lim;     // the last key of each row (KV_TREE: the last that all rows see), of any row
-  int low[RT], hi_low;     // KV_WINDOW: the first key of each row's window, the last of those
-  const uint32_t *bits[RT];  // KV_TREE: which of the new keys each row sees
+  int lim[RT], lo_lim;     // the last key of each row (KV_TREE: its token's number), that all rows see
+  int hi_low;              // KV_WINDOW: the first key of the last row's window
   bool seen[RT], every;    // whether a masked step, or any other, held a key of the row
 
   // col(k): the first of this lane's eight columns in the k-th product
@@ -179,13 +178,9 @@ struct Rows {
       const int row = row0 + r * 16 + n;
       const bool on = row < x.rows;
       const int t = on ? row / a.G : 0;
-      lim[r] = VIEW == KV_TREE ? x.s.len - 1 : on && (VIEW == KV_WINDOW || a.causal) ? x.s.len + t : x.total - 1;
-      lo_lim = min(lo_lim, lim[r]);
-      if constexpr (VIEW == KV_WINDOW) {
-        low[r] = on ? max(lim[r] - a.window + 1, 0) : 0;
-        hi_low = max(hi_low, low[r]);
-      }
-      if constexpr (VIEW == KV_TREE) bits[r] = a.mask + (int64_t)(x.s.start + t) * a.ms;
+      lim[r] = VIEW == KV_TREE ? t : on && (VIEW == KV_WINDOW || a.causal) ? x.s.len + t : x.total - 1;
+      lo_lim = VIEW == KV_TREE ? x.s.len - 1 : min(lo_lim, lim[r]);
+      if (VIEW == KV_WINDOW && on) hi_low = max(hi_low, lim[r] - a.window + 1);
       const T *p = (const T *)a.q + (int64_t)(x.s.start + t) * a.qs + (int64_t)(x.kvh * a.G + (on ? row % a.G : 0)) * a.c.hd;
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
@@ -210,7 +205,8 @@ struct Rows {
 #pragma unroll
       for (int d = 0; d < ND; ++d) O[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int o = 8; o > 0; o >>= 1) lo_lim = min(lo_lim, __shfl_xor(lo_lim, o, 64));
+    if constexpr (VIEW != KV_TREE)
+      for (int o = 8; o > 0; o >>= 1) lo_lim = min(lo_lim, __shfl_xor(lo_lim, o, 64));
     lo_lim = __builtin_amdgcn_readfirstlane(lo_lim);
     if constexpr (VIEW == KV_WINDOW) {
       for (int o = 8; o > 0; o >>= 1) hi_low = max(hi_low, __shfl_xor(hi_low, o, 64));
@@ -227,12 +223,14 @@ struct Rows {
   __device__ __forceinline__ int sees(const KvAttnArgs &a, const Work &x, int r, int first) const {
     if constexpr (VIEW == KV_PREFIX) return max(0, min(16, lim[r] - first + 1));
     if constexpr (VIEW == KV_WINDOW)
-      return (int)(first_bits(lim[r] - first + 1) & (~first_bits(low[r] - first) | first_bits(a.sinks - first)));
+      return (int)(first_bits(lim[r] - first + 1) &
+                   (~first_bits(max(lim[r] - a.window + 1, 0) - first) | first_bits(a.sinks - first)));
     const int at = first - x.s.len;  // the number of the first as a new token
+    const uint32_t *bits = a.mask + (int64_t)(x.s.start + lim[r]) * a.ms;
     uint32_t w = first_bits(-at);
     if (at > -16 && at < x.s.n) {
       const int i = max(at, 0) >> 5;
-      const uint32_t lo = bits[r][i], hi = i * 32 + 32 < x.s.n ? bits[r][i + 1] : 0;
+      const uint32_t lo = bits[i], hi = i * 32 + 32 < x.s.n ? bits[i + 1] : 0;
       w |= at < 0 ? lo << -at : (uint32_t)((((uint64_t)hi << 32) | lo) >> (at & 31));
     }
     return (int)(w & first_bits(x.total - first));
@@ -528,6 +526,25 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
       const int row = d * 16 + n;
       return *reinterpret_cast<const bf16x8 *>(vl + row * 128 + v_place(row, 4 * h + g) * 16);
     };
+    if constexpr (VIEW != KV_PREFIX) {
+      if (nan_step[buf] == j + 1) {  // NaN that left V, for the rows that see it: rare, and few registers
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const int see = groups >> g & 1 ? A.sees(a, x, r, j + 16 * g) : 0;
+          uint64_t row = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) row |= (uint64_t)(uint32_t)__shfl(see, n + 16 * k, 64) << (16 * k);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (reinterpret_cast<const uint64_t *>(nan_bits)[buf * R + d * 16 + 4 * g + i] & row)
+                A.O[r][d][i] = __uint_as_float(0x7fc00000u);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    }
     // operands are read one tile ahead of their products
     f32x4 S[RT][4];
     bf16x8 kf[2][NK];
@@ -554,33 +571,11 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
       vf[d][0] = v_at(d, 0);
       vf[d][1] = v_at(d, 1);
     }
-    int see[RT];
     if (!A.clear(a, j) || groups != 15) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        see[r] = groups >> g & 1 ? A.sees(a, x, r, j + 16 * g) : 0;
-        A.mask(r, S[r], see[r]);
-      }
+      for (int r = 0; r < RT; ++r) A.mask(r, S[r], groups >> g & 1 ? A.sees(a, x, r, j + 16 * g) : 0);
     } else {
       A.every = true;
-#pragma unroll
-      for (int r = 0; r < RT; ++r) see[r] = A.ALL;
-    }
-    if constexpr (VIEW != KV_PREFIX) {
-      if (nan_step[buf] == j + 1) {  // NaN that left V, for the rows that see it
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          uint64_t row = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) row |= (uint64_t)(uint32_t)__shfl(see[r], n + 16 * k, 64) << (16 * k);
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (reinterpret_cast<const uint64_t *>(nan_bits)[buf * R + d * 16 + 4 * g + i] & row)
-                A.O[r][d][i] = __uint_as_float(0x7fc00000u);
-        }
-      }
     }
     bf16x8 pf[RT][2][A.WPARTS];
 #pragma unroll
@@ -656,7 +651,8 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
   const KvArgs &c = a.c;
   const Work x = kv_work<VIEW>(a, pl);
   if (!x.any) return;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int w = VIEW == KV_PREFIX ? tid >> 6 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const float sf = kv_factor(a.scale);
   Rows<T, R, 1, VIEW> A;
   A.init(a, x, x.row0, n, [&](int k) { return k < R / 64 * 2 ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 : R / 64 * 64 + g * 8; });
@@ -772,8 +768,8 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
 
   int i = x.k0 + w * 64;
   if (i < x.k1) advance(i, page_at(key(i)));
-  for (; i < x.k1; i += STEP) {
-    j = key(i);
+  const auto clean = [&]() { return A.clear(a, j) && __all(ok); };
+  const auto walk = [&](auto clean_) {
     const bool more = i + STEP < x.k1, here = ok;
     if (!here && j + 16 * g < x.total && in_reach(j + 16 * g) && c.bad) c.bad[x.b] = 1;
     if constexpr (!LEAN) load_v(j, page);  // on its way while the scores are computed
@@ -781,10 +777,18 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
       if constexpr (LEAN) load_v(j, page);
       else if (more) advance(i + STEP, next);
     };
-    if (A.clear(a, j) && __all(here)) step(Int<1>(), between);
-    else step(Int<0>(), between);
+    step(clean_, between);
     if constexpr (LEAN)
       if (more) advance(i + STEP, next);
+    i += STEP;
+    j = key(i);
+  };
+  j = key(i);
+  while (i < x.k1) {
+    // steps without a mask in a loop of their own: both kinds in one loop leave a window's
+    // walk, which has them in any order, without registers (heads of 128: 131 in memory)
+    while (i < x.k1 && clean()) walk(Int<1>());
+    if (i < x.k1) walk(Int<0>());
   }
   A.finish();
 
