@@ -73,6 +73,64 @@ inline uint32_t inverse(int n) { return n > 1 ? (uint32_t)(((1ull << 32) + n - 1
 constexpr int KV_MANY = 8;  // four-value groups of new tokens a thread holds, of single tokens
 constexpr int KV_ONE = 2;
 constexpr int KV_TURNS = 2;  // groups of four pairs of queries a thread turns
+constexpr int KV_TURNS_AT = 3;  // of those with positions of their own, all under way at once
+
+// Queries that turn by positions of their own, whole groups of four pairs: rows and
+// positions are asked for together and the angles as soon as the positions are there.
+template <typename T>
+__device__ __forceinline__ void turn_queries_at(const KvAppendArgs &a, const Seq &s, int tile) {
+  constexpr int U = KV_TURNS_AT;
+  const int hd = a.c.hd, half = hd >> 1, per = half >> 2, row_groups = a.H * per, NT = blockDim.x, tid = threadIdx.x;
+  const int64_t g0 = (int64_t)tile * U * NT;
+  if (g0 >= (int64_t)s.n * row_groups) return;
+  const int t0 = (int)(g0 / row_groups), first = (int)(g0 % row_groups);
+  int t[U], at[U], col[U], pos[U];
+  float lo[U][4], hi[U][4];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    int g = first + u * NT + tid;
+    t[u] = t0;
+    if (row_groups >= U * NT) {  // one token's end at most lies between
+      t[u] += g >= row_groups;
+      g -= g >= row_groups ? row_groups : 0;
+    } else {
+      t[u] += g / row_groups;
+      g %= row_groups;
+    }
+    const int h = divided(g, a.per_inv, per);
+    col[u] = (g - h * per) * 4;
+    at[u] = h * hd + col[u];
+    pos[u] = a.at[s.start + min(t[u], s.n - 1)];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const T *row = (const T *)a.q + (int64_t)(s.start + min(t[u], s.n - 1)) * a.qs + at[u];
+    Elem<T>::get4(row, lo[u]);
+    Elem<T>::get4(row + half, hi[u]);
+  }
+  float4 cs[U], sn[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t from = (int64_t)((unsigned)pos[u] < (unsigned)a.rope_len ? pos[u] : 0) * half + col[u];
+    cs[u] = *reinterpret_cast<const float4 *>(a.cs + from);
+    sn[u] = *reinterpret_cast<const float4 *>(a.sn + from);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    turn(lo[u][0], hi[u][0], cs[u].x, sn[u].x);
+    turn(lo[u][1], hi[u][1], cs[u].y, sn[u].y);
+    turn(lo[u][2], hi[u][2], cs[u].z, sn[u].z);
+    turn(lo[u][3], hi[u][3], cs[u].w, sn[u].w);
+    if ((unsigned)pos[u] >= (unsigned)a.rope_len) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) lo[u][j] = hi[u][j] = __uint_as_float(0x7fc00000u);
+    }
+    if (t[u] >= s.n) continue;
+    T *out = (T *)a.qo + (int64_t)(s.start + t[u]) * a.qos + at[u];
+    Elem<T>::put4(out, lo[u]);
+    Elem<T>::put4(out + half, hi[u]);
+  }
+}
 
 // One workgroup per (sequence, touched page, kv head, K or V): it owns that
 // block, so its new maximum, the growth of its scale and the bytes of tokens
@@ -100,6 +158,10 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   if ((int)blockIdx.x >= items) {  // queries: KV_TURNS groups of four pairs a thread
     const int i = blockIdx.x - items, b = i / a.qtiles, tile = i % a.qtiles;
     const Seq s = kv_seq(c, b, limit);
+    if (AT && a.vec) {
+      turn_queries_at<T>(a, s, tile);
+      return;
+    }
     const T *q = (const T *)a.q;
     T *qo = (T *)a.qo;
     const int per = (half + 3) >> 2, row_groups = a.H * per;  // of a head, of a token
@@ -203,6 +265,14 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
       if (outside(at[t])) c.bad[b] = 1;
   // no branch between the loads: all of them under way at once
   if (a.vec) {
+    int pos[KV_SLOTS / 2];  // asked for before the rows, so that the angles need not wait for those
+    if (AT && rot) {
+#pragma unroll
+      for (int u = 0; u < KV_SLOTS; u += 2) {
+        int t, d;
+        pos[u / 2] = at[place(u, t, d) ? t : lo];
+      }
+    }
 #pragma unroll
     for (int u = 0; u < KV_SLOTS; ++u) {
       int t, d;
@@ -215,15 +285,14 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
       for (int u = 0; u < KV_SLOTS; u += 2) {
         int t, d;
         const bool on = place(u, t, d);
-        const int pos = turns(on ? t : lo);
-        const int64_t from = (int64_t)(outside(pos) ? 0 : pos) * half + (on ? d : 0);
+        const int p = AT ? pos[u / 2] : first + (on ? t : lo);
+        const int64_t from = (int64_t)(outside(p) ? 0 : p) * half + (on ? d : 0);
         cs[u / 2] = *reinterpret_cast<const float4 *>(a.cs + from);
         sn[u / 2] = *reinterpret_cast<const float4 *>(a.sn + from);
-        if (outside(pos)) cs[u / 2] = make_float4(NAN, NAN, NAN, NAN);
       }
 #pragma unroll
       for (int u = 0; u < KV_SLOTS; u += 2) {
-        const float4 c4 = cs[u / 2], s4 = sn[u / 2];
+        const float4 c4 = AT && outside(pos[u / 2]) ? make_float4(NAN, NAN, NAN, NAN) : cs[u / 2], s4 = sn[u / 2];
         turn(v[u][0], v[u + 1][0], c4.x, s4.x);
         turn(v[u][1], v[u + 1][1], c4.y, s4.y);
         turn(v[u][2], v[u + 1][2], c4.z, s4.z);
@@ -479,7 +548,8 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   // a thread with eight groups waits eight times for memory: 17 us for 256 tokens of
   // 32 heads of 128, where two take 9.5
   const int64_t turns = (int64_t)c.max_new * a.H * ((c.hd / 2 + 3) / 4);
-  const int64_t qtiles = (turns + KV_TURNS * nt - 1) / (KV_TURNS * nt);  // below 2^31: rows are
+  const int per_thread = a.at && a.vec ? KV_TURNS_AT : KV_TURNS;
+  const int64_t qtiles = (turns + per_thread * nt - 1) / (per_thread * nt);  // below 2^31: rows are
   a.qtiles = qtiles < 1 ? 1 : (int)qtiles;
   a.per_inv = inverse((c.hd / 2 + 3) / 4);
   a.group_inv = inverse(c.R / 4);
