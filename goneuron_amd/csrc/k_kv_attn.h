@@ -132,10 +132,18 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
   int id = blockIdx.x;  // heads fastest: with 8 of them a head's tiles share an XCD's L2
   x.kvh = id % c.KVH;
   id /= c.KVH;
-  x.split = id % pl.splits;
-  id /= pl.splits;
-  const int tile = pl.tiles - 1 - id % pl.tiles;  // the rows that see most first
-  x.b = id / pl.tiles;
+  int tile;
+  if (VIEW == KV_TREE && !pl.by_rows) {  // tiles of a split together: they read the same keys
+    tile = id % pl.tiles;
+    id /= pl.tiles;
+    x.split = id % pl.splits;
+    x.b = id / pl.splits;
+  } else {
+    x.split = id % pl.splits;
+    id /= pl.splits;
+    tile = pl.tiles - 1 - id % pl.tiles;  // the rows that see most first
+    x.b = id / pl.tiles;
+  }
   x.s = kv_seq(c, x.b, c.limit);
   if (x.s.bad && c.bad && threadIdx.x == 0) c.bad[x.b] = 1;
   x.total = x.s.len + x.s.n;
@@ -926,9 +934,13 @@ hipError_t kv_attn_typed(const KvAttnArgs &a, const KvPlan &p, hipStream_t s) {
   }
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t slots = (int64_t)c.B * c.max_new * a.H;
-  if (slots >= 16384)
+  // windows and trees: a wave a row from 4096 rows on (8 x 40 x 32 rows of 5 splits: 44 us
+  // with the attention, 51 with four), four from 512 (2048 rows of 32 splits: 77 us, 86
+  // with sixteen)
+  const bool few = VIEW == KV_PREFIX || slots < 512;
+  if (slots >= (VIEW == KV_PREFIX ? 16384 : 4096))
     hipLaunchKernelGGL((kv_join_kernel<T, 1, VIEW>), dim3((unsigned)((slots + 3) / 4)), dim3(256), 0, s, a, p);
-  else if (p.splits <= 16)
+  else if (!few || p.splits <= 16)
     hipLaunchKernelGGL((kv_join_kernel<T, 4, VIEW>), dim3((unsigned)slots), dim3(256), 0, s, a, p);
   else
     hipLaunchKernelGGL((kv_join_kernel<T, 16, VIEW>), dim3((unsigned)slots), dim3(1024), 0, s, a, p);

@@ -12,11 +12,36 @@ namespace gn {
 // while a workgroup a CU is not reached: the join reads them all (one sequence of 131072,
 // 8 heads: 57 us with 32 splits, 61 with 64; one head: 36 and 27).  Prompts: 512
 // workgroups (24.8 us for the five float32 prompts, 1024: 33.2), 128 keys a split at
-// least.
-static int64_t kv_splits(bool by_rows, int64_t items, int64_t len) {
-  int64_t splits = by_rows ? 512 / items : std::min<int64_t>(4096 / items, std::clamp<int64_t>(256 / items, 32, 64));
-  splits = std::min(splits, len / (by_rows ? 128 : 512));
+// least.  Trees whose waves take rows of their own have few tiles of sequences of unlike
+// length: up to 2048 workgroups as long as a split has 1024 keys (16 trees of up to 64
+// tokens behind up to 8000, 32 heads of 128 over 8, bfloat16: 140 us; 512 workgroups: 215),
+// or 1024 of 512 keys (16 trees of 24 behind up to 3000, 8 heads of 128: 32 us, 36 without;
+// two trees of 40 behind 8000, 48 workgroups a split, float32: 54, with 1024 63).
+static int64_t kv_splits(bool by_rows, bool tree, int64_t items, int64_t len) {
+  if (!by_rows) {
+    const int64_t splits = std::min<int64_t>(4096 / items, std::clamp<int64_t>(256 / items, 32, 64));
+    return std::max<int64_t>(std::min(splits, len / 512), 1);
+  }
+  int64_t splits = std::min<int64_t>(512 / items, len / 128);
+  if (tree) splits = std::max({splits, items >= 64 ? std::min(1024 / items, len / 512) : 0, std::min(2048 / items, len / 1024)});
   return std::max<int64_t>(splits, 1);
+}
+
+// Whether the waves of a tree's workgroup take rows of their own, through LDS, or else the
+// same 16 rows and every fourth step of keys, which other tiles read again.  The second is
+// faster where the tree is small against its history, as long as a row is short (12 heads
+// of 80 over 4, float32, three trees of 37 behind up to 33333: 39 us, 47; 32 heads of 64
+// over 8, bfloat16, 16 trees of 40 behind 500: 11 us, 24).  Longer rows cost more to turn
+// into bf16 again for every tile: there it pays while the history is short (heads of 128,
+// the same 16 trees: 21 us, 34; 16 trees of 16 behind 3000: 48, 40), and where registers
+// hold a wave a SIMD (float32 from 128 on, bfloat16 above) for up to four tiles.  With
+// enough workgroups for the card rows of their own are as fast or faster (64 trees of 32
+// behind 100, 8 heads of 64, float32: 9 us, 12).  items: sequences times key heads.
+constexpr int TREE_ROWS = 512;
+static bool tree_by_rows(int64_t items, int64_t rows, int64_t len, int R, int bytes) {
+  if (rows <= 16) return false;
+  const bool wide = R > 96;
+  return items * ((rows + 127) / 128) >= 512 || (wide && len > 1536) || rows > (wide && R * bytes > 256 ? 64 : TREE_ROWS);
 }
 
 static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
@@ -26,24 +51,24 @@ static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
   const int64_t rows = (int64_t)max_new * (H / KVH);
   // up to one tile of rows the waves share it and split the keys; beyond, every
   // further tile would read all keys again
-  p.by_rows = rows > 16;
+  int64_t len = std::min(std::max(a.c.max_len, 1), KV_MAX_TOKENS);  // no table holds more
+  p.by_rows = a.view == KV_TREE ? tree_by_rows((int64_t)B * KVH, rows, len, R, bytes) : rows > 16;
   // two tiles a wave use a K or V operand twice: 310 us for two prompts of 2048 tokens
   // behind 2048, one tile 376; larger heads and float32's parts leave no registers
-  p.rt = rows > 64 && R <= kv_two_tiles(bytes) ? 2 : 1;
+  p.rt = p.by_rows && rows > 64 && R <= kv_two_tiles(bytes) ? 2 : 1;
   p.rows_wg = 16 * p.rt * (p.by_rows ? 4 : 1);
   p.tiles = (int)((rows + p.rows_wg - 1) / p.rows_wg);
   const int64_t items = (int64_t)B * KVH * p.tiles, unit = p.by_rows ? 64 : 256;
-  int64_t len = std::min(std::max(a.c.max_len, 1), KV_MAX_TOKENS);  // no table holds more
   if (a.view == KV_WINDOW) {
     // what the rows of a workgroup see at most: whole steps of the first tokens, and from
     // its first row's window, rounded to a step, to its last row
     const int64_t tokens = std::min<int64_t>(max_new, (p.rows_wg - 1) / a.G + 2);
     len = std::min(len, ((int64_t)a.sinks + 63) / 64 * 64 + a.window + tokens + 63);
   }
-  const int64_t splits = kv_splits(p.by_rows, items, len), chunk = (len + splits - 1) / splits;
+  const int64_t splits = kv_splits(p.by_rows, a.view == KV_TREE, items, len), chunk = (len + splits - 1) / splits;
   p.chunk = (int)((chunk + unit - 1) / unit * unit);
   p.splits = (int)((len + p.chunk - 1) / p.chunk);  // no more than kv_splits: chunks only grow
-  p.work = p.splits > 1 && (p.by_rows || len > KV_SHORT);
+  p.work = p.splits > 1 && (rows > 16 || len > KV_SHORT);
   return p;
 }
 
@@ -61,17 +86,19 @@ int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int
   int64_t most = 0;
   const auto look = [&](bool by_rows, int64_t tiles, int64_t rows) {  // rows: of a key head
     const int64_t n = std::min<int64_t>(max_new, rows / G);
-    if (n == 0 || (n * G > 16) != by_rows) return;
-    for (int64_t b = 1; b <= B && b * KVH * tiles <= (by_rows ? 256 : 2048); ++b) {
-      const int64_t s = kv_splits(by_rows, b * KVH * tiles, len);
+    if (n == 0 || (by_rows && n * G <= 16)) return;
+    for (int64_t b = 1; b <= B && b * KVH * tiles <= (by_rows ? 1024 : 2048); ++b) {
+      const int64_t s = kv_splits(by_rows, true, b * KVH * tiles, len);
       if (s > 1) most = std::max(most, s * b * n * H);
     }
   };
   if (len > KV_SHORT) look(false, 1, 16);
-  for (int64_t tiles = 1; tiles * KVH <= 256; ++tiles) {  // of one 16-row tile a wave, of two
+  for (int64_t tiles = 1; tiles * KVH <= 1024; ++tiles) {  // of one 16-row tile a wave, of two
     look(true, tiles, tiles * 64);
     look(true, tiles, tiles * 128);
   }
+  if (max_new * (int64_t)G > 16)  // trees whose rows all waves share
+    for (int64_t tiles = 1; tiles * KVH <= 2048 && tiles * 16 <= TREE_ROWS; ++tiles) look(false, tiles, tiles * 16);
   return most ? kv_part_floats(most, R) : 0;
 }
 

@@ -232,9 +232,12 @@ def test_a_chain_is_causal_attention(dev):
                                        code, work.p, None))
         check(dev.h, L.gn_kv_attention_tree(dev.h, C.byref(on.kv), dq.p, b.p, H * hd, H * hd, m.p, 3, st.p, ln.p, 1, new, new, total,
                                             H, 0.125, code, work.p, None))
-        va, vb = values(a.get(), dtype), values(b.get(), dtype)
-        # one step of the type where a row's work is cut elsewhere
-        assert (np.abs(va - vb) <= np.maximum(np.abs(va), 1e-3) * (2.0 ** -20 if dtype == "f32" else 2.0 ** -7)).all()
+        va, vb = (values(y.get(), dtype).reshape(new, H, hd) for y in (a, b))
+        # each is within the bound of the exact value, so within twice it of the other: the
+        # two walk the keys in different orders and round elsewhere
+        want, size, lost = kvref.attend(ref, 0, past, values(q, dtype).reshape(new, H, hd), 0.125, 1)
+        lim = kvref.bound(want, size, lost, total, dtype)
+        assert (np.abs(vb - want) <= lim).all() and (np.abs(va - vb) <= 2 * lim).all()
 
 
 # ---------------------------------------------------------------- both
