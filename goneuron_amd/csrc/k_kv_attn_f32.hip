@@ -12,18 +12,31 @@ namespace gn {
 // while a workgroup a CU is not reached: the join reads them all (one sequence of 131072,
 // 8 heads: 57 us with 32 splits, 61 with 64; one head: 36 and 27).  Prompts: 512
 // workgroups (24.8 us for the five float32 prompts, 1024: 33.2), 128 keys a split at
-// least.  Trees whose waves take rows of their own have few tiles of sequences of unlike
-// length: up to 2048 workgroups as long as a split has 1024 keys (16 trees of up to 64
-// tokens behind up to 8000, 32 heads of 128 over 8, bfloat16: 140 us; 512 workgroups: 215),
-// or 1024 of 512 keys (16 trees of 24 behind up to 3000, 8 heads of 128: 32 us, 36 without;
-// two trees of 40 behind 8000, 48 workgroups a split, float32: 54, with 1024 63).
-static int64_t kv_splits(bool by_rows, bool tree, int64_t items, int64_t len) {
+// least.
+// Windows make sequences alike: a workgroup a CU and no more (64 tokens with windows of 4096,
+// 32 heads of 128 over 8, bfloat16: 91 us, 512 workgroups 102, 4096 111; 16 of them: 31
+// us, 34 with 384; 24: 39, 48).
+// Trees whose waves share their rows: 512 workgroups (64 trees of four tokens behind 8000,
+// 32 heads of 64 over 8: 60 us, 69 with 1024 or 4096), or 1024 of 2048 keys at least while
+// there are few without a split (three trees of 37 behind up to 33333, 12 heads of 80 over
+// 4, float32: 35 us, 54 with 512).
+// Trees whose waves take rows of their own have few tiles of sequences of unlike length: up
+// to 2048 workgroups as long as a split has 1024 keys (16 trees of up to 64 tokens behind up
+// to 8000, 32 heads of 128 over 8, bfloat16: 140 us; 512 workgroups: 215), or 1024 of 512
+// keys (16 trees of 24 behind up to 3000, 8 heads of 128: 32 us, 36 without; two trees of
+// 40 behind 8000, 48 workgroups a split, float32: 54, with 1024 63).
+static int64_t kv_splits(bool by_rows, int view, int64_t items, int64_t len) {
+  int64_t splits;
   if (!by_rows) {
-    const int64_t splits = std::min<int64_t>(4096 / items, std::clamp<int64_t>(256 / items, 32, 64));
+    splits = std::min<int64_t>(4096 / items, std::clamp<int64_t>(256 / items, 32, 64));
+    if (view == KV_WINDOW) splits = 256 / items;
+    if (view == KV_TREE)
+      splits = std::min(splits, std::max(512 / items, items < 256 ? std::min(1024 / items, len / 2048) : 0));
     return std::max<int64_t>(std::min(splits, len / 512), 1);
   }
-  int64_t splits = std::min<int64_t>(512 / items, len / 128);
-  if (tree) splits = std::max({splits, items >= 64 ? std::min(1024 / items, len / 512) : 0, std::min(2048 / items, len / 1024)});
+  splits = std::min<int64_t>(512 / items, len / 128);
+  if (view == KV_TREE)
+    splits = std::max({splits, items >= 64 ? std::min(1024 / items, len / 512) : 0, std::min(2048 / items, len / 1024)});
   return std::max<int64_t>(splits, 1);
 }
 
@@ -65,7 +78,7 @@ static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
     const int64_t tokens = std::min<int64_t>(max_new, (p.rows_wg - 1) / a.G + 2);
     len = std::min(len, ((int64_t)a.sinks + 63) / 64 * 64 + a.window + tokens + 63);
   }
-  const int64_t splits = kv_splits(p.by_rows, a.view == KV_TREE, items, len), chunk = (len + splits - 1) / splits;
+  const int64_t splits = kv_splits(p.by_rows, a.view, items, len), chunk = (len + splits - 1) / splits;
   p.chunk = (int)((chunk + unit - 1) / unit * unit);
   p.splits = (int)((len + p.chunk - 1) / p.chunk);  // no more than kv_splits: chunks only grow
   p.work = p.splits > 1 && (rows > 16 || len > KV_SHORT);
@@ -88,7 +101,7 @@ int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int
     const int64_t n = std::min<int64_t>(max_new, rows / G);
     if (n == 0 || (by_rows && n * G <= 16)) return;
     for (int64_t b = 1; b <= B && b * KVH * tiles <= (by_rows ? 1024 : 2048); ++b) {
-      const int64_t s = kv_splits(by_rows, true, b * KVH * tiles, len);
+      const int64_t s = kv_splits(by_rows, by_rows ? KV_TREE : KV_PREFIX, b * KVH * tiles, len);
       if (s > 1) most = std::max(most, s * b * n * H);
     }
   };
