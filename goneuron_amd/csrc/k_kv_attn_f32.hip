@@ -41,20 +41,18 @@ static int64_t kv_splits(bool by_rows, int view, int64_t items, int64_t len) {
 }
 
 // Whether the waves of a tree's workgroup take rows of their own, through LDS, or else the
-// same 16 rows and every fourth step of keys, which other tiles read again.  The second is
-// faster where the tree is small against its history, as long as a row is short (12 heads
-// of 80 over 4, float32, three trees of 37 behind up to 33333: 39 us, 47; 32 heads of 64
-// over 8, bfloat16, 16 trees of 40 behind 500: 11 us, 24).  Longer rows cost more to turn
-// into bf16 again for every tile: there it pays while the history is short (heads of 128,
-// the same 16 trees: 21 us, 34; 16 trees of 16 behind 3000: 48, 40), and where registers
-// hold a wave a SIMD (float32 from 128 on, bfloat16 above) for up to four tiles.  With
-// enough workgroups for the card rows of their own are as fast or faster (64 trees of 32
-// behind 100, 8 heads of 64, float32: 9 us, 12).  items: sequences times key heads.
-constexpr int TREE_ROWS = 512;
-static bool tree_by_rows(int64_t items, int64_t rows, int64_t len, int R, int bytes) {
+// same 16 rows and every fourth step of keys, which other tiles read again.  The second
+// needs no barrier and has no idle waves: three trees of 37 behind up to 33333, 12 heads of
+// 80 over 4, float32: 35 us, 47; 16 trees of 40 behind 500, 32 heads of 64 over 8, bfloat16:
+// 11, 24; 32 trees of 32 behind 8000, 32 heads of 256 over 8: 369, 561.  With heads of 128
+// in bfloat16 the first is at its best (two tiles a wave) and takes over from 160 rows on (8
+// trees of 40 behind 3000, 32 heads over 8: 33, 49; one of 64 behind 32000: 100, 75).  With
+// enough workgroups for the card it is as fast or faster (64 trees of 32 behind 100, 8 heads
+// of 64, float32: 12, 9).  items: sequences times key heads.
+constexpr int TREE_ROWS = 512, TREE_ROWS_128 = 160;
+static bool tree_by_rows(int64_t items, int64_t rows, int R, int bytes) {
   if (rows <= 16) return false;
-  const bool wide = R > 96;
-  return items * ((rows + 127) / 128) >= 512 || (wide && len > 1536) || rows > (wide && R * bytes > 256 ? 64 : TREE_ROWS);
+  return rows > (R == 128 && bytes == 2 ? TREE_ROWS_128 : TREE_ROWS) || items * ((rows + 127) / 128) >= 512;
 }
 
 static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
@@ -64,14 +62,14 @@ static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
   const int64_t rows = (int64_t)max_new * (H / KVH);
   // up to one tile of rows the waves share it and split the keys; beyond, every
   // further tile would read all keys again
-  int64_t len = std::min(std::max(a.c.max_len, 1), KV_MAX_TOKENS);  // no table holds more
-  p.by_rows = a.view == KV_TREE ? tree_by_rows((int64_t)B * KVH, rows, len, R, bytes) : rows > 16;
+  p.by_rows = a.view == KV_TREE ? tree_by_rows((int64_t)B * KVH, rows, R, bytes) : rows > 16;
   // two tiles a wave use a K or V operand twice: 310 us for two prompts of 2048 tokens
   // behind 2048, one tile 376; larger heads and float32's parts leave no registers
   p.rt = p.by_rows && rows > 64 && R <= kv_two_tiles(bytes) ? 2 : 1;
   p.rows_wg = 16 * p.rt * (p.by_rows ? 4 : 1);
   p.tiles = (int)((rows + p.rows_wg - 1) / p.rows_wg);
   const int64_t items = (int64_t)B * KVH * p.tiles, unit = p.by_rows ? 64 : 256;
+  int64_t len = std::min(std::max(a.c.max_len, 1), KV_MAX_TOKENS);  // no table holds more
   if (a.view == KV_WINDOW) {
     // what the rows of a workgroup see at most: whole steps of the first tokens, and from
     // its first row's window, rounded to a step, to its last row
