@@ -40,6 +40,7 @@ struct KvAppendArgs {
   int vec;               // rows, tables and halves allow 4-value accesses
 };
 hipError_t launch_kv_append(const KvAppendArgs &a, int dtype, hipStream_t s);
+hipError_t launch_kv_append_at(const KvAppendArgs &a, int dtype, hipStream_t s);
 hipError_t launch_kv_check(const KvArgs &c, hipStream_t s);
 hipError_t launch_kv_keep(const KvArgs &c, const int32_t *keep, const int32_t *counts, hipStream_t s);
 

@@ -110,7 +110,7 @@ int append_impl(gn_ctx *c, const KvArgs &kv, const void *q, const void *k, const
           (!cos || (((uintptr_t)cos | (uintptr_t)sin) & 15) == 0);
   const double e = dtype == GN_DTYPE_F32 ? 4 : 2;
   KTimer kt(c, GN_KCLASS_OTHER, "kv_append", kv.N * (double)kv.hd * (kv.KVH * 2 * (e + 1) + (q ? 2 * e * heads : 0)));
-  HIP_OK(c, launch_kv_append(a, dtype, c->stream));
+  HIP_OK(c, a.at ? launch_kv_append_at(a, dtype, c->stream) : launch_kv_append(a, dtype, c->stream));
   return GN_OK;
 }
 

@@ -11,126 +11,9 @@ namespace gn {
 namespace {
 
 // ---------------------------------------------------------------- append
-// x * 2^-e rounded to E4M3 (|x| <= 448 2^e by the choice of e); what is not
-// finite becomes NaN (0x7f)
-__device__ __forceinline__ uint32_t to_e4m3(float x, float inv) {
-  const uint32_t b = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x * inv, 0.f, 0, false) & 0xff;
-  return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? 0x7fu : b;
-}
-// four of them
-__device__ __forceinline__ uint32_t to_e4m3(float x, float y, float z, float w, float inv) {
-  const uint32_t most = max(max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu),
-                            max(__float_as_uint(z) & 0x7fffffffu, __float_as_uint(w) & 0x7fffffffu));
-  if (most >= 0x7f800000u) return to_e4m3(x, inv) | to_e4m3(y, inv) << 8 | to_e4m3(z, inv) << 16 | to_e4m3(w, inv) << 24;
-  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x * inv, y * inv, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z * inv, w * inv, lo, true);
-}
-// a stored byte under a larger scale; NaN stays
-__device__ __forceinline__ uint32_t rescaled(uint32_t byte, float ratio) {
-  if ((byte & 0x7f) == 0x7f) return byte;
-  const float x = __builtin_amdgcn_cvt_f32_fp8((int)byte, 0);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x * ratio, 0.f, 0, false) & 0xff;
-}
-// smallest power of two s >= 2^-100 with amax / s <= 448
-__device__ __forceinline__ float block_scale(float amax) {
-  const uint32_t u = __float_as_uint(amax / 448.f);
-  int e = (int)(u >> 23) - 127 + ((u & 0x7fffffu) ? 1 : 0);
-  e = max(e, KV_MAX_SCALE_EXP);
-  return __uint_as_float((uint32_t)(e + 127) << 23);
-}
-
-// a pair turned by an angle, in float64 and rounded once
-__device__ __forceinline__ void turn(float &x, float &y, float c, float s) {
-  const double a = (double)x * (double)c - (double)y * (double)s, b = (double)x * (double)s + (double)y * (double)c;
-  x = (float)a;
-  y = (float)b;
-}
-// four values of one token's head from column d on, rotated (rot) in float64 and
-// rounded once: products of two float32 are exact there, so every reader of
-// the definition gets the same float32.  Columns beyond hd are 0.
-template <typename T>
-__device__ __forceinline__ void load_rotated(const T *row, const float *cs, const float *sn, int hd, int d, bool rot,
-                                             float (&o)[4]) {
-  const int half = hd >> 1;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = d + i;
-    o[i] = j < hd ? Elem<T>::get(row + j) : 0.f;
-    if (rot && j < 2 * half) {  // the last column of an odd head does not turn
-      const bool up = j >= half;
-      const int t = up ? j - half : j;
-      const float p = Elem<T>::get(row + (up ? t : j + half));
-      const double a = (double)o[i] * (double)cs[t], b = (double)p * (double)sn[t];
-      o[i] = (float)(up ? b + a : a - b);
-    }
-  }
-}
-
-// g / n by ceil(2^32 / n), exact while g n < 2^32: a division takes twenty times as long
-__device__ __forceinline__ int divided(int g, uint32_t inv, int n) { return n == 1 ? g : (int)__umulhi((uint32_t)g, inv); }
-inline uint32_t inverse(int n) { return n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / n) : 0; }
-
 constexpr int KV_MANY = 8;  // four-value groups of new tokens a thread holds, of single tokens
 constexpr int KV_ONE = 2;
 constexpr int KV_TURNS = 2;  // groups of four pairs of queries a thread turns
-constexpr int KV_TURNS_AT = 3;  // of those with positions of their own, all under way at once
-
-// Queries that turn by positions of their own, whole groups of four pairs: rows and
-// positions are asked for together and the angles as soon as the positions are there.
-template <typename T>
-__device__ __forceinline__ void turn_queries_at(const KvAppendArgs &a, const Seq &s, int tile) {
-  constexpr int U = KV_TURNS_AT;
-  const int hd = a.c.hd, half = hd >> 1, per = half >> 2, row_groups = a.H * per, NT = blockDim.x, tid = threadIdx.x;
-  const int64_t g0 = (int64_t)tile * U * NT;
-  if (g0 >= (int64_t)s.n * row_groups) return;
-  const int t0 = (int)(g0 / row_groups), first = (int)(g0 % row_groups);
-  int t[U], at[U], col[U], pos[U];
-  float lo[U][4], hi[U][4];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    int g = first + u * NT + tid;
-    t[u] = t0;
-    if (row_groups >= U * NT) {  // one token's end at most lies between
-      t[u] += g >= row_groups;
-      g -= g >= row_groups ? row_groups : 0;
-    } else {
-      t[u] += g / row_groups;
-      g %= row_groups;
-    }
-    const int h = divided(g, a.per_inv, per);
-    col[u] = (g - h * per) * 4;
-    at[u] = h * hd + col[u];
-    pos[u] = a.at[s.start + min(t[u], s.n - 1)];
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const T *row = (const T *)a.q + (int64_t)(s.start + min(t[u], s.n - 1)) * a.qs + at[u];
-    Elem<T>::get4(row, lo[u]);
-    Elem<T>::get4(row + half, hi[u]);
-  }
-  float4 cs[U], sn[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t from = (int64_t)((unsigned)pos[u] < (unsigned)a.rope_len ? pos[u] : 0) * half + col[u];
-    cs[u] = *reinterpret_cast<const float4 *>(a.cs + from);
-    sn[u] = *reinterpret_cast<const float4 *>(a.sn + from);
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    turn(lo[u][0], hi[u][0], cs[u].x, sn[u].x);
-    turn(lo[u][1], hi[u][1], cs[u].y, sn[u].y);
-    turn(lo[u][2], hi[u][2], cs[u].z, sn[u].z);
-    turn(lo[u][3], hi[u][3], cs[u].w, sn[u].w);
-    if ((unsigned)pos[u] >= (unsigned)a.rope_len) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) lo[u][j] = hi[u][j] = __uint_as_float(0x7fc00000u);
-    }
-    if (t[u] >= s.n) continue;
-    T *out = (T *)a.qo + (int64_t)(s.start + t[u]) * a.qos + at[u];
-    Elem<T>::put4(out, lo[u]);
-    Elem<T>::put4(out + half, hi[u]);
-  }
-}
 
 // One workgroup per (sequence, touched page, kv head, K or V): it owns that
 // block, so its new maximum, the growth of its scale and the bytes of tokens
@@ -143,9 +26,7 @@ __device__ __forceinline__ void turn_queries_at(const KvAppendArgs &a, const Seq
 // 2048: 45 us for 163 MB, 3.6 TB/s, where a copy reaches 4.9).  Prompts also wait for the
 // vector unit: indexes without divisions, pairs turned once and bytes rounded two at a
 // time brought them from 60.
-// AT: rows turn by positions of their own; one outside the tables makes its query and key
-// NaN.  (A template, so that rows without are given no more registers.)
-template <typename T, int KV_SLOTS, bool AT>
+template <typename T, int KV_SLOTS>
 __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
   const KvArgs &c = a.c;
@@ -158,10 +39,6 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
   if ((int)blockIdx.x >= items) {  // queries: KV_TURNS groups of four pairs a thread
     const int i = blockIdx.x - items, b = i / a.qtiles, tile = i % a.qtiles;
     const Seq s = kv_seq(c, b, limit);
-    if (AT && a.vec) {
-      turn_queries_at<T>(a, s, tile);
-      return;
-    }
     const T *q = (const T *)a.q;
     T *qo = (T *)a.qo;
     const int per = (half + 3) >> 2, row_groups = a.H * per;  // of a head, of a token
@@ -181,10 +58,8 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
       const int h = divided(g, a.per_inv, per), d = (g - h * per) * 4;
       const T *row = q + (int64_t)(s.start + t) * a.qs + h * c.hd;
       T *out = qo + (int64_t)(s.start + t) * a.qos + h * c.hd;
-      const int pos = AT ? a.at[s.start + t] : s.len + t;
-      const bool lost = AT && (unsigned)pos >= (unsigned)a.rope_len;
-      const float *cs = a.cs ? a.cs + (int64_t)(lost ? 0 : pos) * half : nullptr;
-      const float *sn = a.cs ? a.sn + (int64_t)(lost ? 0 : pos) * half : nullptr;
+      const float *cs = a.cs ? a.cs + (int64_t)(s.len + t) * half : nullptr;
+      const float *sn = a.cs ? a.sn + (int64_t)(s.len + t) * half : nullptr;
       float lo[4], hi[4];
       if (a.vec) {
         Elem<T>::get4(row + d, lo);
@@ -194,10 +69,6 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
           const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) turn(lo[j], hi[j], cc[j], ss[j]);
-          if (lost) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) lo[j] = hi[j] = __uint_as_float(0x7fc00000u);
-          }
         }
         Elem<T>::put4(out + d, lo);
         Elem<T>::put4(out + d + half, hi);
@@ -205,7 +76,6 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
         for (int j = d; j < min(d + 4, half); ++j) {
           float x = Elem<T>::get(row + j), y = Elem<T>::get(row + j + half);
           if (a.cs) turn(x, y, cs[j], sn[j]);
-          if (lost) x = y = __uint_as_float(0x7fc00000u);
           Elem<T>::put(out + j, x);
           Elem<T>::put(out + j + half, y);
         }
@@ -214,9 +84,8 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
     if (c.hd & 1)  // the last column has no partner; every tile takes its share of the rows
       for (int64_t g = (int64_t)tile * NT + tid; g < (int64_t)s.n * a.H; g += (int64_t)a.qtiles * NT) {
         const int t = (int)(g / a.H), h = (int)(g % a.H);
-        const bool lost = AT && (unsigned)a.at[s.start + t] >= (unsigned)a.rope_len;
         Elem<T>::put(qo + (int64_t)(s.start + t) * a.qos + h * c.hd + c.hd - 1,
-                     lost ? __uint_as_float(0x7fc00000u) : Elem<T>::get(q + (int64_t)(s.start + t) * a.qs + h * c.hd + c.hd - 1));
+                     Elem<T>::get(q + (int64_t)(s.start + t) * a.qs + h * c.hd + c.hd - 1));
       }
     return;
   }
@@ -256,23 +125,8 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
 
   float v[KV_SLOTS][4];
   const T *xs = x + (int64_t)(s.start + first - s.len) * a.xs[which];
-  // the place in the tables of token t of the page, and whether there is none
-  const int32_t *at = AT ? a.at + (s.start + first - s.len) : nullptr;
-  const auto turns = [&](int t) { return AT ? at[t] : first + t; };
-  const auto outside = [&](int p) { return AT && (unsigned)p >= (unsigned)a.rope_len; };
-  if (AT && !which && h == 0 && c.bad)
-    for (int t = lo + tid; t < hi; t += NT)
-      if (outside(at[t])) c.bad[b] = 1;
   // no branch between the loads: all of them under way at once
   if (a.vec) {
-    int pos[KV_SLOTS / 2];  // asked for before the rows, so that the angles need not wait for those
-    if (AT && rot) {
-#pragma unroll
-      for (int u = 0; u < KV_SLOTS; u += 2) {
-        int t, d;
-        pos[u / 2] = at[place(u, t, d) ? t : lo];
-      }
-    }
 #pragma unroll
     for (int u = 0; u < KV_SLOTS; ++u) {
       int t, d;
@@ -285,14 +139,13 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
       for (int u = 0; u < KV_SLOTS; u += 2) {
         int t, d;
         const bool on = place(u, t, d);
-        const int p = AT ? pos[u / 2] : first + (on ? t : lo);
-        const int64_t from = (int64_t)(outside(p) ? 0 : p) * half + (on ? d : 0);
-        cs[u / 2] = *reinterpret_cast<const float4 *>(a.cs + from);
-        sn[u / 2] = *reinterpret_cast<const float4 *>(a.sn + from);
+        const int64_t at = (int64_t)(first + (on ? t : lo)) * half + (on ? d : 0);
+        cs[u / 2] = *reinterpret_cast<const float4 *>(a.cs + at);
+        sn[u / 2] = *reinterpret_cast<const float4 *>(a.sn + at);
       }
 #pragma unroll
       for (int u = 0; u < KV_SLOTS; u += 2) {
-        const float4 c4 = AT && outside(pos[u / 2]) ? make_float4(NAN, NAN, NAN, NAN) : cs[u / 2], s4 = sn[u / 2];
+        const float4 c4 = cs[u / 2], s4 = sn[u / 2];
         turn(v[u][0], v[u + 1][0], c4.x, s4.x);
         turn(v[u][1], v[u + 1][1], c4.y, s4.y);
         turn(v[u][2], v[u + 1][2], c4.z, s4.z);
@@ -311,14 +164,9 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(KvAppendArgs a) {
     for (int u = 0; u < KV_SLOTS; ++u) {
       int t, d;
       if (!place(u, t, d)) break;
-      const int p = turns(t);
-      const int64_t pos = outside(p) ? 0 : p;
+      const int64_t pos = first + t;
       load_rotated(xs + t * a.xs[which], rot ? a.cs + pos * half : nullptr, rot ? a.sn + pos * half : nullptr, c.hd, d, rot,
                    v[u]);
-      if (rot && outside(p)) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[u][k] = d + k < c.hd ? __uint_as_float(0x7fc00000u) : 0.f;
-      }
     }
   }
   const auto largest = [&](auto of) {
@@ -548,8 +396,7 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   // a thread with eight groups waits eight times for memory: 17 us for 256 tokens of
   // 32 heads of 128, where two take 9.5
   const int64_t turns = (int64_t)c.max_new * a.H * ((c.hd / 2 + 3) / 4);
-  const int per_thread = a.at && a.vec ? KV_TURNS_AT : KV_TURNS;
-  const int64_t qtiles = (turns + per_thread * nt - 1) / (per_thread * nt);  // below 2^31: rows are
+  const int64_t qtiles = (turns + KV_TURNS * nt - 1) / (KV_TURNS * nt);  // below 2^31: rows are
   a.qtiles = qtiles < 1 ? 1 : (int)qtiles;
   a.per_inv = inverse((c.hd / 2 + 3) / 4);
   a.group_inv = inverse(c.R / 4);
@@ -560,12 +407,8 @@ hipError_t launch_kv_append(const KvAppendArgs &a0, int dtype, hipStream_t s) {
   // single tokens fill two groups of a thread at most: loads of eight took 6.1 us where
   // theirs take 4 (a token of 4 sequences, 8 heads of 32)
   const bool one = c.max_new == 1;
-  auto fn = one ? kv_append_kernel<float, KV_ONE, false> : kv_append_kernel<float, KV_MANY, false>;
-  if (dtype != GN_DTYPE_F32) fn = one ? kv_append_kernel<uint16_t, KV_ONE, false> : kv_append_kernel<uint16_t, KV_MANY, false>;
-  if (a.at) {
-    fn = one ? kv_append_kernel<float, KV_ONE, true> : kv_append_kernel<float, KV_MANY, true>;
-    if (dtype != GN_DTYPE_F32) fn = one ? kv_append_kernel<uint16_t, KV_ONE, true> : kv_append_kernel<uint16_t, KV_MANY, true>;
-  }
+  auto fn = one ? kv_append_kernel<float, KV_ONE> : kv_append_kernel<float, KV_MANY>;
+  if (dtype != GN_DTYPE_F32) fn = one ? kv_append_kernel<uint16_t, KV_ONE> : kv_append_kernel<uint16_t, KV_MANY>;
   hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(nt), sh, s, a);
   return hipGetLastError();
 }
