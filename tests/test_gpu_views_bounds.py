@@ -1,0 +1,165 @@
+"""GPU tests of windows, trees, appends at positions and moves at the bounds of what they
+take: loose bounds of new tokens, caches whose offsets pass 32 bits, histories of nothing."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import kvref
+import viewref
+from gpuutil import DBuf, log
+from test_gpu_drafts import append_at
+from test_gpu_kv_cache import BF16, F32, OnDevice, as_dtype, spread, starts_of, values
+from test_gpu_kv_views import case, floats, tree
+
+pytestmark = pytest.mark.gpu
+
+
+def _lib():
+    from goneuron_amd._lib import check, lib
+    return lib(), check
+
+
+@pytest.mark.parametrize("dtype,hd", [("f32", 64), ("bf16", 128), ("bf16", 256), ("f32", 80)])
+@pytest.mark.parametrize("view", ["window", "tree"])
+def test_loose_bounds_of_new_tokens(dev, view, dtype, hd):
+    """Single tokens and short sequences in calls made for many more."""
+    rng = np.random.default_rng(hd)
+    for new, bound in (([1, 1], 17), ([1, 3], 200), ([5, 1], 700)):
+        kw = dict(masks=[tree(rng, n) for n in new]) if view == "tree" else dict(sinks=3, window=40)
+        case(dev, dtype, hd, 16, 2, 2, [90, 0], new, max_new=bound, max_len=1000, **kw)
+
+
+@pytest.mark.parametrize("dtype,G,hd", [("f32", 1, 64), ("f32", 4, 96), ("bf16", 4, 64), ("bf16", 8, 128), ("bf16", 2, 256), ("f32", 3, 128),
+                                        ("bf16", 5, 128), ("f32", 8, 192)])
+def test_trees_of_every_plan(dev, dtype, G, hd):
+    """Rows that a workgroup's waves share, over one tile and many, and rows of their own;
+    with and without splits."""
+    rng = np.random.default_rng(G + hd)
+    for past, new in (([20], [4]), ([700, 40], [24, 7]), ([2300], [40]), ([30, 5, 0], [130, 1, 66]), ([5000], [33])):
+        if sum(new) * G * (sum(past) + sum(new)) > 700000:
+            continue
+        case(dev, dtype, hd, 32, 1, G, past, new, masks=[tree(rng, n) for n in new], seed=len(past))
+
+
+def test_many_short_trees(dev):
+    """So many that no split pays: the plan for a full card."""
+    rng = np.random.default_rng(1)
+    new = [int(x) for x in rng.integers(0, 9, 300)]
+    new[0] = 8
+    past = [int(x) for x in rng.integers(0, 40, 300)]
+    case(dev, "bf16", 32, 16, 2, 4, past, new, masks=[tree(rng, n) for n in new])
+    case(dev, "f32", 32, 16, 2, 4, past, new, sinks=2, window=11)
+
+
+@pytest.mark.parametrize("dtype,hd,page", [("f32", 32, 16), ("bf16", 128, 64), ("f32", 7, 16), ("bf16", 80, 128)])
+def test_append_at_and_keep_with_loose_bounds(dev, dtype, hd, page):
+    L, check = _lib()
+    rng = np.random.default_rng(hd)
+    kvh, heads, past, new = 2, 4, [page - 1, 0, 7], [3, 0, 20]
+    N = sum(new)
+    pages, table = spread(rng, 3, 3)
+    ref = kvref.Cache(pages, page, kvh, hd, table, rng)
+    for b in range(3):
+        x = rng.normal(size=(2, past[b], kvh, hd))
+        ref.append(b, 0, x[0], x[1])
+    on = OnDevice(dev, ref)
+    cos, sin = kvref.tables(64, hd)
+    (q, q64), (k, k64), (v, v64) = (as_dtype(rng.normal(size=(N, n * hd)), dtype) for n in (heads, kvh, kvh))
+    at = rng.integers(0, 64, N).astype(np.int32)
+    w = [n * hd for n in (heads, kvh, kvh)]
+    bufs = [DBuf(dev, a) for a in (q, k, v, q * 0, cos, sin, at, starts_of(new), np.asarray(past, np.int32), np.zeros(3, np.int32))]
+    dq, dk, dv, do, dc, ds, da, st, ln, bad = bufs
+    check(dev.h, L.gn_kv_append_at(dev.h, C.byref(on.kv), dq.p, dk.p, dv.p, do.p, w[0], w[1], w[2], w[0], dc.p, ds.p, 64, da.p, st.p,
+                                   ln.p, 3, N, 500, heads, F32 if dtype == "f32" else BF16, bad.p))
+    s, want = starts_of(new), np.zeros((N, heads, hd))
+    for b in range(3):
+        r = slice(s[b], s[b + 1])
+        c, sn = cos[at[r]][:, None], sin[at[r]][:, None]
+        want[r] = kvref.rotate(q64[r].reshape(-1, heads, hd), c, sn)
+        ref.append(b, past[b], kvref.rotate(k64[r].reshape(-1, kvh, hd), c, sn), v64[r].reshape(-1, kvh, hd))
+    on.same()
+    assert np.array_equal(do.get(), as_dtype(want.reshape(N, -1), dtype)[0]) and not bad.get().any()
+    paths = [[1, 2], [], [0, 4, 9, 18, 19]]
+    keep, counts = np.zeros(N, np.int32), np.array([2, 0, 5], np.int32)
+    for b in range(3):
+        keep[s[b]:s[b] + counts[b]] = paths[b]
+        viewref.keep(ref, b, past[b], new[b], paths[b])
+    dk, dn = DBuf(dev, keep), DBuf(dev, counts)
+    check(dev.h, L.gn_kv_keep(dev.h, C.byref(on.kv), dk.p, dn.p, st.p, ln.p, 3, N, 1000, bad.p))
+    on.same()
+    assert not bad.get().any()
+
+
+def test_offsets_beyond_32_bits(dev):
+    """K and V of 6.4 GB each, the pages in use at their end."""
+    from goneuron_amd._lib import KVCache
+    L, check = _lib()
+    rng = np.random.default_rng(4)
+    kvh, hd, P, heads, R = 8, 128, 128, 8, 128
+    block = kvh * P * R
+    pages, used = 49152, 4
+    past, new, total = 150, 40, 190
+    table = np.arange(pages - used, pages, dtype=np.int32)[[2, 0, 3, 1]].reshape(1, 4)
+    small = kvref.Cache(used, P, kvh, hd, table - (pages - used), rng)
+    size = pages * block
+    assert size > 2 ** 32
+    p = [C.c_void_p(), C.c_void_p()]
+    for x in p:
+        check(dev.h, L.gn_malloc(dev.h, size, C.byref(x)))
+    try:
+        scales = [DBuf(dev, np.full((pages, kvh), np.nan, np.float32)) for _ in range(2)]
+        dt = DBuf(dev, table)
+        kv = KVCache(k=p[0], v=p[1], k_scale=scales[0].p, v_scale=scales[1].p, table=dt.p, pages=pages, page_size=P, kv_heads=kvh,
+                     head_dim=hd, max_pages=4)
+        end = (pages - used) * block
+        for x, a in zip(p, (small.k, small.v)):
+            check(dev.h, L.gn_memcpy_h2d(dev.h, C.c_void_p(x.value + end), a.ctypes.data, a.nbytes))
+
+        def same():
+            for x, a in zip(p, (small.k, small.v)):
+                got = np.empty_like(a)
+                check(dev.h, L.gn_memcpy_d2h(dev.h, got.ctypes.data, C.c_void_p(x.value + end), got.nbytes))
+                assert np.array_equal(got, a)
+            for d, a in zip(scales, (small.ks, small.vs)):
+                assert np.array_equal(d.get()[pages - used:], a, equal_nan=True)
+
+        cos, sin = kvref.tables(256, hd)
+        dc, ds = DBuf(dev, cos), DBuf(dev, sin)
+        bad = DBuf(dev, np.zeros(1, np.int32))
+        for at0, n in ((0, past), (past, new)):
+            (k, k64), (v, v64), (q, q64) = (as_dtype(rng.normal(size=(n, kvh * hd)), "f32") for _ in range(3))
+            at = rng.integers(0, 256, n).astype(np.int32)
+            bufs = [DBuf(dev, a) for a in (q, k, v, q * 0, at, starts_of([n]), np.array([at0], np.int32))]
+            w = kvh * hd
+            check(dev.h, L.gn_kv_append_at(dev.h, C.byref(kv), bufs[0].p, bufs[1].p, bufs[2].p, bufs[3].p, w, w, w, w, dc.p, ds.p, 256,
+                                           bufs[4].p, bufs[5].p, bufs[6].p, 1, n, n, heads, F32, bad.p))
+            c, s = cos[at][:, None], sin[at][:, None]
+            small.append(0, at0, kvref.rotate(k64.reshape(n, kvh, hd), c, s), v64.reshape(n, kvh, hd))
+        same()
+        q64 = values(bufs[3].get(), "f32").reshape(new, heads, hd)
+        work = DBuf(dev, np.zeros(max(1, floats(1, new, total, heads, kvh, hd)), np.float32))
+        mask = tree(rng, new)
+        dm, do = DBuf(dev, viewref.words([mask], 2).view(np.int32)), DBuf(dev, np.zeros((new, w), np.float32))
+        for view in ("window", "tree"):
+            log(f"{view} at offsets beyond 32 bits")
+            if view == "window":
+                check(dev.h, L.gn_kv_attention_window(dev.h, C.byref(kv), bufs[3].p, do.p, w, w, bufs[5].p, bufs[6].p, 1, new, new, total,
+                                                      heads, 0.1, 5, 90, F32, work.p, bad.p))
+                sight = viewref.window_sight(past, new, 5, 90)
+            else:
+                check(dev.h, L.gn_kv_attention_tree(dev.h, C.byref(kv), bufs[3].p, do.p, w, w, dm.p, 2, bufs[5].p, bufs[6].p, 1, new, new,
+                                                    total, heads, 0.1, F32, work.p, bad.p))
+                sight = viewref.tree_sight(past, mask)
+            want, size_, lost = viewref.attend(small, 0, past, q64, float(np.float32(0.1)), sight)
+            got = do.get().astype(np.float64).reshape(new, heads, hd)
+            assert (np.abs(got - want) <= kvref.bound(want, size_, lost, total, "f32")).all()
+        path = np.flatnonzero(mask[new - 1])
+        dk, dn = DBuf(dev, np.pad(path, (0, new - len(path))).astype(np.int32)), DBuf(dev, np.array([len(path)], np.int32))
+        check(dev.h, L.gn_kv_keep(dev.h, C.byref(kv), dk.p, dn.p, bufs[5].p, bufs[6].p, 1, new, new, bad.p))
+        viewref.keep(small, 0, past, new, path)
+        same()
+        assert not bad.get().any()
+    finally:
+        for x in p:
+            L.gn_free(dev.h, x)
