@@ -572,6 +572,10 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
         for (int r = 0; r < RT; ++r) A.scores(kf[t & 1][k], k, r, S[r][t]);
       __builtin_amdgcn_sched_barrier(0);  // else all tiles' reads move up and registers run out
     }
+    // The wave that weighs goes before the SIMD's other, whose products can wait for the
+    // matrix unit: a window of 8192 of two prompts of 2048 tokens 843 -> 805 us, of 1024 139
+    // -> 136.
+    if constexpr (VIEW != KV_PREFIX) __builtin_amdgcn_s_setprio(1);
     constexpr int AHEAD = 2;
     bf16x8 vf[AHEAD + 1][2];
 #pragma unroll
@@ -588,6 +592,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
     bf16x8 pf[RT][2][A.WPARTS];
 #pragma unroll
     for (int r = 0; r < RT; ++r) A.weights(r, S[r], sf, pf[r]);
+    if constexpr (VIEW != KV_PREFIX) __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
