@@ -1,5 +1,5 @@
 // Attention over the paged 8-bit cache: the kernels, compiled once for each type
-// of queries (k_kv_attn_f32.hip, k_kv_attn_bf16.hip).
+// of queries and each view of theirs (k_kv_attn_*.hip, k_kv_window_*.hip, k_kv_tree_*.hip).
 #pragma once
 #include "gn_kv.h"
 
@@ -386,6 +386,10 @@ __device__ __forceinline__ int v_place(int row, int chunk) { return chunk ^ ((ro
 // 2048, 32 heads of 128 over 8, bfloat16, in 307 us, 206 GFLOP at 672 TFLOP/s of the
 // definition's products and, the weights' second part among them, 1007 of the units' (a
 // product of 16384^3 reaches 1369 here); the waves wait for LDS and the barrier.
+// Windows of 1024 of the same prompts: 136 us, 69 GFLOP in 19 steps a workgroup, two of them
+// masked and one for four first tokens; the vector units are busy 52 % of the time, the
+// matrix units 37 %.  Trees of up to 64 tokens of 16 sequences of up to 8000: 122 us and
+// 19 for the join, 3.3 us a step whether one or two workgroups share a CU.
 template <typename T, int R, int RT, int VIEW>
 __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int NK = R / 32, ND = R / 16;
@@ -654,8 +658,8 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
 // joined through LDS.
 // Bound by memory: one sequence of 131072 tokens, 8 key heads of 128, in 57 us with its
 // join, 4.7 TB/s of cache (43 us alone: 6.2, as fast as memory is read here; float32
-// queries without shared heads 50, 5.4); 64 sequences of up to 8192 in 121 us, 4.4 TB/s.
-// A step of 5 us at the least.
+// queries without shared heads 50, 5.4); 64 sequences of up to 8192 in 121 us, 4.4 TB/s;
+// 64 windows of 4096 in 91, 5.3 TB/s.  A step of 5 us at the least.
 template <typename T, int R, int VIEW>
 __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void kv_attn_keys_kernel(KvAttnArgs a, KvPlan pl) {
   constexpr int NK = R / 32, ND = R / 16;

@@ -606,7 +606,7 @@ int gn_kv_append(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, const void *
  * is nothing to it.  bad as above.  work: gn_kv_attention_workspace floats, 16-byte
  * aligned (may be 0: then work may be null).  What it asks for serves every call with the
  * same heads whose B, max_new and max_len are no larger, so that a program asks once for
- * its largest sizes. */
+ * its largest sizes, and gn_kv_attention_window's and gn_kv_attention_tree's as well. */
 int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max_len, int32_t heads, int32_t kv_heads,
                               int32_t head_dim, int64_t *floats);
 int gn_kv_attention(gn_ctx *ctx, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,
