@@ -163,3 +163,92 @@ def test_offsets_beyond_32_bits(dev):
     finally:
         for x in p:
             L.gn_free(dev.h, x)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_stream_in_a_few_pages(dev, dtype):
+    """Two streams that never end: their pages go back to a pool once they have left the
+    window, and come again for later tokens.  The answers are those of a cache that holds
+    everything, seen through the window; each step's logits come under rules and are drawn
+    from, and the draws are the next step's tokens."""
+    from test_gpu_drafts import bits, rules
+    L, check = _lib()
+    rng = np.random.default_rng(15)
+    code = F32 if dtype == "f32" else BF16
+    heads, kvh, hd, P, B, V, sinks, window, steps = 4, 2, 32, 16, 2, 61, 4, 40, 60
+    D, KW = heads * hd, kvh * hd
+    E = [rng.normal(size=(V, n)).astype(np.float32) for n in (D, KW, KW)]
+    Wo = rng.normal(size=(V, D)).astype(np.float32) * 2
+    max_pages = 40
+    shadow = kvref.Cache(B * max_pages, P, kvh, hd, np.arange(B * max_pages).reshape(B, max_pages), rng)
+    small = kvref.Cache(12, P, kvh, hd, np.full((B, max_pages), -1), rng)
+    on = OnDevice(dev, small)
+    free = list(range(12))
+    table = np.full((B, max_pages), -1, np.int32)
+    cos, sin = kvref.tables(max_pages * P, hd)
+    dc, ds, dW = DBuf(dev, cos), DBuf(dev, sin), DBuf(dev, Wo)
+    past, tokens = [0, 0], [list(rng.integers(0, V, 23)), list(rng.integers(0, V, 3))]
+    text, recycled = [[], []], 0
+    n = C.c_int64()
+    check(None, L.gn_sample_workspace(B, V, C.byref(n)))
+    draw = DBuf(dev, np.zeros(n.value, np.float32))
+    for step in range(steps):
+        new = [len(t) for t in tokens]
+        for b in range(B):
+            for j in range(max_pages):  # what the coming queries do not see goes back
+                if table[b, j] >= 0 and j * P >= sinks and (j + 1) * P <= past[b] - window + 1:
+                    free.append(int(table[b, j]))
+                    table[b, j] = rng.choice([-1, 99, table[b, j]])
+                    if table[b, j] == free[-1]:
+                        table[b, j] = -5
+            for j in range(past[b] // P, (past[b] + new[b] - 1) // P + 1):
+                if table[b, j] < 0 or j * P >= past[b]:
+                    if j * P >= past[b]:
+                        recycled += step > 0
+                        table[b, j] = free.pop(0)
+        dt = DBuf(dev, table)
+        on.kv.table = dt.p
+        ids = np.concatenate(tokens)
+        N, mx = len(ids), max(new)
+        (q, q64), (k, k64), (v, v64) = (as_dtype(e[ids], dtype) for e in E)
+        bufs = [DBuf(dev, a) for a in (q, k, v, q * 0, q * 0, starts_of(new), np.asarray(past, np.int32), np.zeros(B, np.int32))]
+        dq, dk, dv, dqo, do, st, ln, bad = bufs
+        check(dev.h, L.gn_kv_append(dev.h, C.byref(on.kv), dq.p, dk.p, dv.p, dqo.p, D, KW, KW, D, dc.p, ds.p, max_pages * P, st.p, ln.p,
+                                    B, N, mx, heads, code, bad.p))
+        check(dev.h, L.gn_kv_attention_window(dev.h, C.byref(on.kv), dqo.p, do.p, D, D, st.p, ln.p, B, N, mx, max_pages * P, heads, 0.2,
+                                              sinks, window, code, None, bad.p))
+        assert not bad.get().any()
+        s, turned, got = starts_of(new), values(dqo.get(), dtype), values(do.get(), dtype)
+        for b in range(B):
+            r, pos = slice(s[b], s[b + 1]), np.arange(past[b], past[b] + new[b])
+            shadow.append(b, past[b], kvref.rotate(k64[r].reshape(-1, kvh, hd), cos[pos][:, None], sin[pos][:, None]),
+                          v64[r].reshape(-1, kvh, hd))
+            want, size, lost = viewref.attend(shadow, b, past[b], turned[r].reshape(-1, heads, hd), float(np.float32(0.2)),
+                                              viewref.window_sight(past[b], new[b], sinks, window))
+            lim = kvref.bound(want, size, lost, past[b] + new[b], dtype)
+            assert (np.abs(got[r].reshape(-1, heads, hd) - want) <= lim).all(), (step, b)
+            text[b] += [int(x) for x in tokens[b]]
+        dh, dl = DBuf(dev, got[[s[1] - 1, s[2] - 1]].astype(np.float32)), DBuf(dev, np.zeros((B, V), np.float32))
+        check(dev.h, L.gn_gemm(dev.h, 0, 1, B, V, D, 1.0, dh.p, D, dW.p, D, dl.p, V))
+        z = dl.get()
+        rows = np.zeros((B, 700), np.int32)
+        for b in range(B):
+            rows[b, :len(text[b])] = text[b]
+        ok = rng.random((1, V)) < 0.7
+        R, held = rules(dev, tokens=rows, token_lens=np.array([len(t) for t in text], np.int32), repetition=np.full(B, 1.1, np.float32),
+                        presence=np.full(B, 0.3, np.float32), allowed=bits(ok), allowed_row=np.array([0, -1], np.int32))
+        check(dev.h, L.gn_logits_adjust(dev.h, dl.p, V, dl.p, V, F32, C.byref(R), B, V))
+        y = dl.get()
+        u = rng.random(B).astype(np.float32)
+        du, di = DBuf(dev, u), DBuf(dev, np.zeros(B, np.int32))
+        check(dev.h, L.gn_sample(dev.h, dl.p, V, F32, None, None, None, None, du.p, di.p, B, V, draw.p))
+        drawn = di.get()
+        for b in range(B):
+            w, off = viewref.adjust(z[b], text[b], 0, np.float32(1.1), None, np.float32(0.3), allowed=ok[0] if b == 0 else None)
+            fine = np.isfinite(w)
+            assert np.array_equal(np.isfinite(y[b]), fine) and (np.abs(y[b][fine] - w[fine]) <= off[fine]).all()
+            assert drawn[b] == kvref.sample(y[b].astype(np.float64), u[b])
+        past = [a + x for a, x in zip(past, new)]
+        # a drawn token, and now and then some that a user adds
+        tokens = [[int(drawn[b])] + list(rng.integers(0, V, int(rng.integers(0, 12)) if rng.random() < 0.2 else 0)) for b in range(B)]
+    assert recycled > 6 and max(past) > 60
