@@ -133,7 +133,7 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
   x.kvh = id % c.KVH;
   id /= c.KVH;
   int tile;
-  if (VIEW == KV_TREE && !pl.by_rows) {  // tiles of a split together: they read the same keys
+  if (VIEW != KV_PREFIX && !pl.by_rows) {  // tiles of a split together: they read the same keys
     tile = id % pl.tiles;
     id /= pl.tiles;
     x.split = id % pl.splits;

@@ -15,7 +15,7 @@ namespace gn {
 // least.
 // Windows make sequences alike: a workgroup a CU and no more (64 tokens with windows of 4096,
 // 32 heads of 128 over 8, bfloat16: 91 us, 512 workgroups 102, 4096 111; 16 of them: 31
-// us, 34 with 384; 24: 39, 48).
+// us, 34 with 384; 24: 39, 48; one of 40 with 8192, 8 heads, float32: 21, 29 with 512).
 // Trees whose waves share their rows: 512 workgroups (64 trees of four tokens behind 8000,
 // 32 heads of 64 over 8: 60 us, 69 with 1024 or 4096), or 1024 of 2048 keys at least while
 // there are few without a split (three trees of 37 behind up to 33333, 12 heads of 80 over
@@ -40,19 +40,26 @@ static int64_t kv_splits(bool by_rows, int view, int64_t items, int64_t len) {
   return std::max<int64_t>(splits, 1);
 }
 
-// Whether the waves of a tree's workgroup take rows of their own, through LDS, or else the
-// same 16 rows and every fourth step of keys, which other tiles read again.  The second
-// needs no barrier and has no idle waves: three trees of 37 behind up to 33333, 12 heads of
-// 80 over 4, float32: 35 us, 47; 16 trees of 40 behind 500, 32 heads of 64 over 8, bfloat16:
-// 11, 24; 32 trees of 32 behind 8000, 32 heads of 256 over 8: 369, 561.  With heads of 128
-// in bfloat16 the first is at its best (two tiles a wave) and takes over from 160 rows on (8
-// trees of 40 behind 3000, 32 heads over 8: 33, 49; one of 64 behind 32000: 100, 75).  With
-// enough workgroups for the card it is as fast or faster (64 trees of 32 behind 100, 8 heads
-// of 64, float32: 12, 9).  items: sequences times key heads.
-constexpr int TREE_ROWS = 512, TREE_ROWS_128 = 160;
-static bool tree_by_rows(int64_t items, int64_t rows, int R, int bytes) {
-  if (rows <= 16) return false;
-  return rows > (R == 128 && bytes == 2 ? TREE_ROWS_128 : TREE_ROWS) || items * ((rows + 127) / 128) >= 512;
+// Whether a workgroup's waves take rows of their own, through LDS, or else the same 16 rows
+// and every fourth step of keys, which other tiles read again.  For windows and trees the
+// second has no barrier and no idle waves:
+//   three trees of 37 behind up to 33333, 12 heads of 80 over 4, float32: 35 us, 47;
+//   two trees of 2000 behind 2000, 8 heads of 96, float32: 166, 213;
+//   32 trees of 32 behind 8000, 32 heads of 256 over 8, bfloat16: 369, 561;
+//   4 prompts of up to 128, a window of 512, 32 heads of 64 over 8, bfloat16: 13, 23;
+//   8 of up to 20, a window of 4096, 32 heads of 128 over 8, float32: 35, 62.
+// Longer rows cost more to turn into bf16 again for every tile: float32 heads of 128 change
+// over at 1024 rows (2048: 236, 220; prompts of 2048 with a window of 1024: 120, 59), and
+// bfloat16 ones, of which waves hold two tiles, at 160 with a long history (8 trees of 40
+// behind 3000: 33, 49; one of 64 behind 32000: 100, 75) and 512 in a window (4 of up to
+// 128, a window of 512: 16, 32).  With enough workgroups for the card rows of their own are
+// as fast or faster (64 trees of 32 behind 100, 8 heads of 64, float32: 12, 9; 64 of up to
+// 17, a window of 256, 8 heads of 128, float32: 42, 24).  items: sequences times key heads.
+constexpr int SHARED_ROWS = 8192;  // at most
+static bool by_rows(int view, int64_t items, int64_t rows, int R, int bytes) {
+  if (rows <= 16 || view == KV_PREFIX) return rows > 16;
+  const int most = R <= 96 ? SHARED_ROWS : R > 128 || bytes == 4 ? 1024 : view == KV_TREE ? 160 : 512;
+  return rows > most || items * ((rows + 127) / 128) >= 512;
 }
 
 static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
@@ -60,9 +67,9 @@ static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
   const int bytes = dtype == GN_DTYPE_F32 ? 4 : 2;
   KvPlan p{};
   const int64_t rows = (int64_t)max_new * (H / KVH);
-  // up to one tile of rows the waves share it and split the keys; beyond, every
-  // further tile would read all keys again
-  p.by_rows = a.view == KV_TREE ? tree_by_rows((int64_t)B * KVH, rows, R, bytes) : rows > 16;
+  // up to one tile of rows the waves share it and split the keys; beyond, every further
+  // tile would read all keys again, which windows and trees often still gain by
+  p.by_rows = by_rows(a.view, (int64_t)B * KVH, rows, R, bytes);
   // two tiles a wave use a K or V operand twice: 310 us for two prompts of 2048 tokens
   // behind 2048, one tile 376; larger heads and float32's parts leave no registers
   p.rt = p.by_rows && rows > 64 && R <= kv_two_tiles(bytes) ? 2 : 1;
@@ -108,8 +115,8 @@ int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int
     look(true, tiles, tiles * 64);
     look(true, tiles, tiles * 128);
   }
-  if (max_new * (int64_t)G > 16)  // trees whose rows all waves share
-    for (int64_t tiles = 1; tiles * KVH <= 2048 && tiles * 16 <= TREE_ROWS; ++tiles) look(false, tiles, tiles * 16);
+  if (max_new * (int64_t)G > 16)  // windows and trees whose rows all waves share
+    for (int64_t tiles = 1; tiles * KVH <= 2048 && tiles * 16 <= SHARED_ROWS; ++tiles) look(false, tiles, tiles * 16);
   return most ? kv_part_floats(most, R) : 0;
 }
 

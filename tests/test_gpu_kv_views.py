@@ -134,7 +134,8 @@ def test_window_split_along_the_keys(dev, dtype, G, new, past, window):
 
 
 def test_window_that_holds_all_is_attention_without(dev):
-    """The same numbers as gn_kv_attention's, bit for bit: the walk is the same."""
+    """gn_kv_attention's answers.  Each call is within the bound of the exact value, so they are
+    within twice it of each other; they may walk the keys in different orders."""
     L, check = _lib()
     rng = np.random.default_rng(3)
     for dtype, new, past in (("f32", 1, 700), ("bf16", 90, 200), ("f32", 40, 0), ("bf16", 1, 5000)):
@@ -154,7 +155,10 @@ def test_window_that_holds_all_is_attention_without(dev):
                                        code, work.p, None))
         check(dev.h, L.gn_kv_attention_window(dev.h, C.byref(on.kv), dq.p, b.p, H * hd, H * hd, st.p, ln.p, 1, new, new, total, H,
                                               0.125, 3, total, code, work.p, None))
-        assert np.array_equal(a.get(), b.get()) and np.abs(values(a.get(), dtype)).max() > 0
+        va, vb = (values(y.get(), dtype).reshape(new, H, hd) for y in (a, b))
+        want, size, lost = kvref.attend(ref, 0, past, values(q, dtype).reshape(new, H, hd), 0.125, 1)
+        lim = kvref.bound(want, size, lost, total, dtype)
+        assert (np.abs(vb - want) <= lim).all() and (np.abs(va - vb) <= 2 * lim).all() and np.abs(va).max() > 0
 
 
 # ---------------------------------------------------------------- trees
