@@ -252,3 +252,38 @@ def test_a_stream_in_a_few_pages(dev, dtype):
         # a drawn token, and now and then some that a user adds
         tokens = [[int(drawn[b])] + list(rng.integers(0, V, int(rng.integers(0, 12)) if rng.random() < 0.2 else 0)) for b in range(B)]
     assert recycled > 6 and max(past) > 60
+
+
+@pytest.mark.parametrize("dtype,hd,G,new0", [("f32", 64, 2, 45), ("bf16", 128, 4, 30), ("f32", 192, 2, 20), ("bf16", 96, 2, 70),
+                                             ("bf16", 32, 5, 6), ("f32", 128, 3, 33), ("bf16", 256, 2, 12), ("f32", 32, 1, 90)])
+@pytest.mark.parametrize("view", ["window", "tree"])
+@pytest.mark.parametrize("kind", ["plain", "nan", "missing"])
+def test_a_card_full_of_sequences(dev, view, kind, dtype, hd, G, new0):
+    """Enough sequences that waves take rows of their own: a few longer ones among many of a
+    token or two, with NaN in and out of sight, pages that are not there, and pages that have
+    left the windows."""
+    rng = np.random.default_rng(hd + new0)
+    B, kvh, P = 258, 2, 16
+    past, new = [int(x) for x in rng.integers(0, 30, B)], [int(x) for x in rng.integers(0, 3, B)]
+    for b, (a, n) in zip((0, 7, 100, 257), ((190, new0), (0, new0), (333, new0 // 2 + 1), (64, 1))):
+        past[b], new[b] = a, n
+
+    def spoil(ref):
+        if kind == "nan":
+            for b in (0, 7, 100):
+                for p in {3, 50, past[b] // 2, past[b], past[b] + new[b] - 1}:
+                    if p >= past[b] + new[b]:
+                        continue
+                    page, t = ref.table[b, p // P], p % P
+                    ref.v[page, 0, (p * 5) % hd, t] = 0x7f
+                    ref.v[page, 1, 2, t] = 0xff
+                    if p % 2:
+                        ref.k[page, 1, t, 5] = 0x7f
+        if kind == "missing":
+            ref.table[0, 11] = -1
+            ref.table[7, 0] = ref.pages
+            ref.table[100, 20] = 2 ** 31 - 1
+
+    kw = dict(masks=[tree(rng, n) for n in new]) if view == "tree" else dict(sinks=5, window=41, gone=kind != "missing")
+    bad = case(dev, dtype, hd, P, kvh, G, past, new, spoil=None if kind == "plain" else spoil, **kw)
+    assert sorted(np.flatnonzero(bad)) == ([0, 7, 100] if kind == "missing" else [])
