@@ -656,6 +656,8 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
 // operands come straight from memory into the lanes that need them: four times
 // the loads in flight for one set of rows, and no barrier until the waves are
 // joined through LDS.
+// Windows and trees of several tokens take tiles of 16 rows so too where that is faster
+// than rows of their own.
 // Bound by memory: one sequence of 131072 tokens, 8 key heads of 128, in 57 us with its
 // join, 4.7 TB/s of cache (43 us alone: 6.2, as fast as memory is read here; float32
 // queries without shared heads 50, 5.4); 64 sequences of up to 8192 in 121 us, 4.4 TB/s;
