@@ -147,7 +147,7 @@ int attention(gn_ctx *c, KvAttnArgs &a, int dtype, const char *what) {
   const int64_t w = (int64_t)a.H * a.c.hd;
   int rc;
   if ((rc = row_check(c, "q", a.q, a.qs, w, dtype)) || (rc = row_check(c, "out", a.out, a.os, w, dtype))) return rc;
-  if (!a.work && kv_attn_uses_work(a, dtype)) return set_err(c, GN_ERR_INVALID, "%s needs its workspace", what);
+  if (!a.work && kv_attn_need_floats(a, dtype) > 0) return set_err(c, GN_ERR_INVALID, "%s needs its workspace", what);
   if ((uintptr_t)a.work & 15) return set_err(c, GN_ERR_INVALID, "%s: work must be 16-byte aligned", what);
   return attn_impl(c, a, dtype);
 }
@@ -257,6 +257,24 @@ extern "C" int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max
     return GN_ERR_INVALID;
   *floats = kv_attn_work_floats(B, max_new, max_len, heads, kv_heads, head_dim);
   return GN_OK;
+}
+
+// Not of the public interface: what a call of these sizes would take of its workspace
+// (view: KvView), for the test that holds it against gn_kv_attention_workspace.
+extern "C" int64_t gn_kv_attention_need(int32_t view, int32_t B, int32_t max_new, int32_t max_len, int32_t heads,
+                                        int32_t kv_heads, int32_t head_dim, int32_t sinks, int32_t window, int32_t dtype) {
+  KvAttnArgs a{};
+  a.c.B = B;
+  a.c.max_new = max_new;
+  a.c.max_len = max_len;
+  a.c.KVH = kv_heads;
+  a.c.R = kv_row(head_dim);
+  a.H = heads;
+  a.G = heads / kv_heads;
+  a.view = view;
+  a.sinks = sinks;
+  a.window = window;
+  return kv_attn_need_floats(a, dtype);
 }
 
 extern "C" int gn_kv_attention(gn_ctx *c, const gn_kv_cache *kv, const void *q, void *out, int64_t q_stride,

@@ -15,7 +15,9 @@ namespace gn {
 // least.
 // Windows make sequences alike: a workgroup a CU and no more (64 tokens with windows of 4096,
 // 32 heads of 128 over 8, bfloat16: 91 us, 512 workgroups 102, 4096 111; 16 of them: 31
-// us, 34 with 384; 24: 39, 48; one of 40 with 8192, 8 heads, float32: 21, 29 with 512).
+// us, 34 with 384; 24: 39, 48; one of 40 with 8192, 8 heads, float32: 21, 29 with 512), and
+// 64 splits at most as well (a window of 131072, 8 heads of 128 over one, bfloat16: 27
+// us, 31 with 256; of 65536: 21.6, 20.8 with 128; float32: 29, 32 and 23.4, 22.3).
 // Trees whose waves share their rows: 512 workgroups (64 trees of four tokens behind 8000,
 // 32 heads of 64 over 8: 60 us, 69 with 1024 or 4096), or 1024 of 2048 keys at least while
 // there are few without a split (three trees of 37 behind up to 33333, 12 heads of 80 over
@@ -29,7 +31,7 @@ static int64_t kv_splits(bool by_rows, int view, int64_t items, int64_t len) {
   int64_t splits;
   if (!by_rows) {
     splits = std::min<int64_t>(4096 / items, std::clamp<int64_t>(256 / items, 32, 64));
-    if (view == KV_WINDOW) splits = 256 / items;
+    if (view == KV_WINDOW) splits = std::min(splits, 256 / items);
     if (view == KV_TREE)
       splits = std::min(splits, std::max(512 / items, items < 256 ? std::min(1024 / items, len / 2048) : 0));
     return std::max<int64_t>(std::min(splits, len / 512), 1);
@@ -93,10 +95,10 @@ static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
 // what `rows` (split, token, head) rows of outputs take
 static int64_t kv_part_floats(int64_t rows, int R) { return kv_part_at(1, rows) + rows * R; }
 
-// Enough for every call with no more sequences, new tokens or tokens.  One with fewer of
-// the first two is split further, and a shorter bound may round to more splits, so the
-// most that splits x rows reaches is looked for over all numbers of workgroups that are
-// split at all, with as many rows as their tiles hold.
+// Enough for every call of every view with no more sequences, new tokens or tokens.  One
+// with fewer of the first two is split further, and a shorter bound may round to more
+// splits, so the most that splits x rows reaches is looked for over all numbers of
+// workgroups that any view splits at all, with as many rows as their tiles hold.
 int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd) {
   if (B == 0 || max_new == 0 || max_len == 0) return 0;
   const int R = kv_row(hd), G = H / KVH;
@@ -106,7 +108,8 @@ int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int
     const int64_t n = std::min<int64_t>(max_new, rows / G);
     if (n == 0 || (by_rows && n * G <= 16)) return;
     for (int64_t b = 1; b <= B && b * KVH * tiles <= (by_rows ? 1024 : 2048); ++b) {
-      const int64_t s = kv_splits(by_rows, by_rows ? KV_TREE : KV_PREFIX, b * KVH * tiles, len);
+      int64_t s = 0;
+      for (int view : {KV_PREFIX, KV_WINDOW, KV_TREE}) s = std::max(s, kv_splits(by_rows, view, b * KVH * tiles, len));
       if (s > 1) most = std::max(most, s * b * n * H);
     }
   };
@@ -120,7 +123,10 @@ int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int
   return most ? kv_part_floats(most, R) : 0;
 }
 
-bool kv_attn_uses_work(const KvAttnArgs &a, int dtype) { return kv_plan(a, dtype).work; }
+int64_t kv_attn_need_floats(const KvAttnArgs &a, int dtype) {
+  const KvPlan p = kv_plan(a, dtype);
+  return p.work ? kv_part_floats((int64_t)p.splits * a.c.B * a.c.max_new * a.H, a.c.R) : 0;
+}
 
 hipError_t launch_kv_attn(const KvAttnArgs &a0, int dtype, float *scratch, int64_t scratch_floats, hipStream_t s) {
   KvAttnArgs a = a0;
