@@ -158,6 +158,13 @@ __device__ __forceinline__ Work kv_work(const KvAttnArgs &a, const KvPlan &pl) {
   return x;
 }
 
+// The first key of any of the workgroup's windows; without a window, behind all keys.
+template <int VIEW>
+__device__ __forceinline__ int kv_reach(const KvAttnArgs &a, const Work &x) {
+  if constexpr (VIEW != KV_WINDOW) return 0;
+  return a.window > 0 ? x.s.len + x.row0 / a.G - a.window + 1 : 0x7fffffff;
+}
+
 // A wave's 16 RT rows.  Lane n + 16 g holds, for row n of a tile: the queries'
 // columns of its k slots, sixteen keys' scores of a step, and columns 4 g + i of
 // each 16 of the output.
@@ -431,7 +438,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
   const int gv = tid & 3;
   // whether some row may see one of the 16 keys from j on: pages that none does need not be
   // there, nor hold a scale
-  const int reach = VIEW == KV_WINDOW ? x.s.len + x.row0 / a.G - a.window + 1 : 0;
+  const int reach = kv_reach<VIEW>(a, x);
   const auto in_reach = [&](int j) { return VIEW != KV_WINDOW || j + 15 >= reach || j < a.sinks; };
   const auto pages = [&](int j) {
 #pragma unroll
@@ -717,7 +724,7 @@ __global__ __launch_bounds__(256, R <= (sizeof(T) == 4 ? 96 : 128) ? 2 : 1) void
 
   const auto key = [&](int i) { return x.span.key<VIEW>(i); };
   // pages that no row sees need not be there, nor hold a scale
-  const int reach = VIEW == KV_WINDOW ? x.s.len + x.row0 / a.G - a.window + 1 : 0;
+  const int reach = kv_reach<VIEW>(a, x);
   const auto in_reach = [&](int at) { return VIEW != KV_WINDOW || at + 15 >= reach || at < a.sinks; };
   int j = 0, page = 0, next = 0;
   bool ok = false;
