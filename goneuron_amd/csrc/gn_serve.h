@@ -77,7 +77,7 @@ constexpr int KV_SHORT = 4096;
 constexpr int kv_two_tiles(int bytes) { return bytes == 4 ? 64 : 128; }
 // the workspace: (maximum, sum) of every split's rows, then their outputs
 __host__ __device__ inline int64_t kv_part_at(int splits, int64_t slots) { return (splits * slots * 2 + 3) / 4 * 4; }
-int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd);
+int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd, bool every_view);
 int64_t kv_attn_need_floats(const KvAttnArgs &a, int dtype);  // what a call of these very sizes takes of it
 hipError_t launch_kv_attn(const KvAttnArgs &a, int dtype, float *scratch, int64_t scratch_floats, hipStream_t s);
 hipError_t launch_kv_attn_bf16(const KvAttnArgs &a, const KvPlan &p, hipStream_t s);

@@ -255,7 +255,7 @@ extern "C" int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max
   if (!floats || B < 0 || max_new < 0 || max_len < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 ||
       head_dim > KV_MAX_HEAD || too_many_rows(B, max_new, heads))
     return GN_ERR_INVALID;
-  *floats = kv_attn_work_floats(B, max_new, max_len, heads, kv_heads, head_dim);
+  *floats = kv_attn_work_floats(B, max_new, max_len, heads, kv_heads, head_dim, true);
   return GN_OK;
 }
 
@@ -347,7 +347,7 @@ extern "C" int gn_mha_cached_workspace(int32_t B, int32_t N, int32_t max_new, in
       D / heads > KV_MAX_HEAD || too_many_rows(B, max_new, heads))
     return GN_ERR_INVALID;
   *floats = 4 * (((int64_t)N * D + 63) / 64 * 64) +
-            kv_attn_work_floats(B, max_new, max_len, heads, heads, D / heads);
+            kv_attn_work_floats(B, max_new, max_len, heads, heads, D / heads, false);  // it calls no other view
   return GN_OK;
 }
 

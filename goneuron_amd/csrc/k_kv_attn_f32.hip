@@ -95,11 +95,11 @@ static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
 // what `rows` (split, token, head) rows of outputs take
 static int64_t kv_part_floats(int64_t rows, int R) { return kv_part_at(1, rows) + rows * R; }
 
-// Enough for every call of every view with no more sequences, new tokens or tokens.  One
-// with fewer of the first two is split further, and a shorter bound may round to more
-// splits, so the most that splits x rows reaches is looked for over all numbers of
-// workgroups that any view splits at all, with as many rows as their tiles hold.
-int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd) {
+// Enough for every call of every view, or of prefixes alone, with no more sequences, new
+// tokens or tokens.  One with fewer of the first two is split further, and a shorter bound
+// may round to more splits, so the most that splits x rows reaches is looked for over all
+// numbers of workgroups that a view splits at all, with as many rows as their tiles hold.
+int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int hd, bool every_view) {
   if (B == 0 || max_new == 0 || max_len == 0) return 0;
   const int R = kv_row(hd), G = H / KVH;
   const int64_t len = std::min(max_len, KV_MAX_TOKENS);
@@ -109,7 +109,8 @@ int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int
     if (n == 0 || (by_rows && n * G <= 16)) return;
     for (int64_t b = 1; b <= B && b * KVH * tiles <= (by_rows ? 1024 : 2048); ++b) {
       int64_t s = 0;
-      for (int view : {KV_PREFIX, KV_WINDOW, KV_TREE}) s = std::max(s, kv_splits(by_rows, view, b * KVH * tiles, len));
+      for (int view = KV_PREFIX; view <= (every_view ? KV_TREE : KV_PREFIX); ++view)
+        s = std::max(s, kv_splits(by_rows, view, b * KVH * tiles, len));
       if (s > 1) most = std::max(most, s * b * n * H);
     }
   };
@@ -118,7 +119,7 @@ int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int
     look(true, tiles, tiles * 64);
     look(true, tiles, tiles * 128);
   }
-  if (max_new * (int64_t)G > 16)  // windows and trees whose rows all waves share
+  if (every_view && max_new * (int64_t)G > 16)  // windows and trees whose rows all waves share
     for (int64_t tiles = 1; tiles * KVH <= 2048 && tiles * 16 <= SHARED_ROWS; ++tiles) look(false, tiles, tiles * 16);
   return most ? kv_part_floats(most, R) : 0;
 }

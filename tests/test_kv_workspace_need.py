@@ -74,3 +74,31 @@ def test_sizes_at_random(L, heads):
         have = [grant(L, *m, heads) for m in more]
         for need, *what in needs(L, B, new, length, heads, [(log(1, length) - 1, log(1, ALL)) for _ in range(3)]):
             assert need <= min(have), (more, have, need, what)
+
+
+# ---------------------------------------------------------------- the layer, which sees prefixes alone
+def layer(L, B, rows, new, length, D, heads):
+    """Floats that it asks for beside its own rows."""
+    n = C.c_int64()
+    assert L.gn_mha_cached_workspace(B, rows, new, length, D, heads, C.byref(n)) == 0
+    return n.value - 4 * ((rows * D + 63) // 64 * 64)
+
+
+@pytest.mark.parametrize("B,new,length,D,heads,floats", [
+    # 65536 (split, token, head) rows at most, of 128 floats and two
+    (2, 2048, 4096, 4096, 32, 65536 * 130), (1, 8192, 8192, 512, 4, 65536 * 130), (4, 16, 8192, 256, 8, 278528)])
+def test_the_layer_does_not_pay_for_trees(L, B, new, length, D, heads, floats):
+    assert layer(L, B, B * new, new, length, D, heads) == floats
+
+
+@pytest.mark.parametrize("D,heads", [(256, 8), (256, 1), (64, 4), (960, 12), (4096, 32), (1024, 8)])
+def test_the_layer_at_random(L, D, heads):
+    rng = random.Random(D + heads)
+    for _ in range(3000):
+        B, new = int(3000 ** rng.random()), int(5000 ** rng.random())
+        length = int((2 ** 31 - 1) ** rng.random())
+        if B * new * heads > 2 ** 28:
+            continue
+        need = L.gn_kv_attention_need(PREFIX, B, new, length, heads, heads, D // heads, 0, 0, 0)
+        more = (B + rng.randrange(3), new * rng.choice([1, 2]) + rng.randrange(3), min(length + rng.randrange(5000), ALL))
+        assert need <= layer(L, B, B, new, length, D, heads) and need <= layer(L, more[0], B, *more[1:], D, heads)
