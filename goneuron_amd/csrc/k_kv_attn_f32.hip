@@ -44,24 +44,37 @@ static int64_t kv_splits(bool by_rows, int view, int64_t items, int64_t len) {
 
 // Whether a workgroup's waves take rows of their own, through LDS, or else the same 16 rows
 // and every fourth step of keys, which other tiles read again.  For windows and trees the
-// second has no barrier and no idle waves:
-//   three trees of 37 behind up to 33333, 12 heads of 80 over 4, float32: 35 us, 47;
-//   two trees of 2000 behind 2000, 8 heads of 96, float32: 166, 213;
-//   32 trees of 32 behind 8000, 32 heads of 256 over 8, bfloat16: 369, 561;
-//   4 prompts of up to 128, a window of 512, 32 heads of 64 over 8, bfloat16: 13, 23;
-//   8 of up to 20, a window of 4096, 32 heads of 128 over 8, float32: 35, 62.
-// Longer rows cost more to turn into bf16 again for every tile: float32 heads of 128 change
-// over at 1024 rows (2048: 236, 220; prompts of 2048 with a window of 1024: 120, 59), and
-// bfloat16 ones, of which waves hold two tiles, at 160 with a long history (8 trees of 40
-// behind 3000: 33, 49; one of 64 behind 32000: 100, 75) and 512 in a window (4 of up to
-// 128, a window of 512: 16, 32).  With enough workgroups for the card rows of their own are
-// as fast or faster (64 trees of 32 behind 100, 8 heads of 64, float32: 12, 9; 64 of up to
-// 17, a window of 256, 8 heads of 128, float32: 42, 24).  items: sequences times key heads.
+// second has no barrier and no idle waves; it loses where its workgroups (`shared`) are many
+// and, for long rows, which every tile turns into bf16 again, the rows.  Both sides, shared
+// rows first, in us (32 query heads over 8; B trees of n tokens behind a history, or windows):
+//   heads of up to 96 share: of 64, bfloat16, 1 of 50 behind 200: 6.1, 12.9; 4 of 250 behind
+//     12000: 228, 271; of 96, float32, 1 of 2000 (8 heads) behind 12000: 250, 305 (but 4 of
+//     250 behind 200: 40, 29);
+//   more than 128, and 128 in float32, share up to 1024 rows, but for many of a short history:
+//     of 256, bfloat16, 4 of 128 behind 3000: 183, 204; 4 of 250 behind 200: 138, 67; 128,
+//     float32, 4 of 50 behind 3000: 51, 68; 4 of 250 behind 200: 85, 33 (3000: 217, 182);
+//     4 of 250, a window of 1000: 119, 58;
+//   128 in bfloat16, of which waves hold two tiles of their own: 1 of 60 behind 700: 11, 23; 4
+//     of 128 behind 3000: 77, 90; but 1 of 60 behind 12000: 52, 43; 4 of 100 behind 6000:
+//     137, 118; 12 of 60 behind 1: 23, 13; 12 of 128 behind 700: 80, 54; a window of 512, 1
+//     of 128: 12, 26, 12 of 128: 75, 46.  Histories are bounds of unlike lengths, for which
+//     rows of their own take more splits than for windows (of 8192, 1 of 128: 53, 59; not
+//     for all the best, 4 of 128: 183, 143).
+// With enough workgroups for the card rows of their own are as fast or faster (64 trees of 32
+// behind 100, 8 heads of 64, float32: 12, 9).  On 110 sizes at random where limits on the
+// rows alone (1024; for the last kind 160 in trees, 512 in windows) say otherwise this takes 0.61
+// of their time, 1.09 at worst.  items: sequences times key heads; keys: that a tile sees.
 constexpr int SHARED_ROWS = 8192;  // at most
-static bool by_rows(int view, int64_t items, int64_t rows, int R, int bytes) {
+static bool by_rows(int view, int64_t items, int64_t rows, int64_t keys, int R, int bytes) {
   if (rows <= 16 || view == KV_PREFIX) return rows > 16;
-  const int most = R <= 96 ? SHARED_ROWS : R > 128 || bytes == 4 ? 1024 : view == KV_TREE ? 160 : 512;
-  return rows > most || items * ((rows + 127) / 128) >= 512;
+  if (rows > SHARED_ROWS || items * ((rows + 127) / 128) >= 512) return true;
+  const int64_t shared = items * ((rows + 15) / 16);
+  if (R <= 96) return false;
+  if (rows > 1024) return true;
+  if (R > 128 || bytes == 4) return shared > 1024 && keys < (view == KV_TREE ? 768 : 1280);
+  if (rows <= 160) return false;
+  if (rows > 512 || (shared > 1536 && keys < 1024) || (shared > 1024 && keys < 256) || (shared > 768 && keys < 128)) return true;
+  return view == KV_TREE && (shared > 1536 || keys > 4096 || shared * keys > 4000000);
 }
 
 static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
@@ -69,22 +82,24 @@ static KvPlan kv_plan(const KvAttnArgs &a, int dtype) {
   const int bytes = dtype == GN_DTYPE_F32 ? 4 : 2;
   KvPlan p{};
   const int64_t rows = (int64_t)max_new * (H / KVH);
+  // what the rows of a workgroup see at most: in a window whole steps of the first tokens, and
+  // from its first row's window, rounded to a step, to its last row
+  const auto keys = [&](int rows_wg) {
+    const int64_t len = std::min(std::max(a.c.max_len, 1), KV_MAX_TOKENS);  // no table holds more
+    if (a.view != KV_WINDOW) return len;
+    const int64_t tokens = std::min<int64_t>(max_new, (rows_wg - 1) / a.G + 2);
+    return std::min(len, ((int64_t)a.sinks + 63) / 64 * 64 + a.window + tokens + 63);
+  };
   // up to one tile of rows the waves share it and split the keys; beyond, every further
   // tile would read all keys again, which windows and trees often still gain by
-  p.by_rows = by_rows(a.view, (int64_t)B * KVH, rows, R, bytes);
+  p.by_rows = by_rows(a.view, (int64_t)B * KVH, rows, keys(16), R, bytes);
   // two tiles a wave use a K or V operand twice: 310 us for two prompts of 2048 tokens
   // behind 2048, one tile 376; larger heads and float32's parts leave no registers
   p.rt = p.by_rows && rows > 64 && R <= kv_two_tiles(bytes) ? 2 : 1;
   p.rows_wg = 16 * p.rt * (p.by_rows ? 4 : 1);
   p.tiles = (int)((rows + p.rows_wg - 1) / p.rows_wg);
   const int64_t items = (int64_t)B * KVH * p.tiles, unit = p.by_rows ? 64 : 256;
-  int64_t len = std::min(std::max(a.c.max_len, 1), KV_MAX_TOKENS);  // no table holds more
-  if (a.view == KV_WINDOW) {
-    // what the rows of a workgroup see at most: whole steps of the first tokens, and from
-    // its first row's window, rounded to a step, to its last row
-    const int64_t tokens = std::min<int64_t>(max_new, (p.rows_wg - 1) / a.G + 2);
-    len = std::min(len, ((int64_t)a.sinks + 63) / 64 * 64 + a.window + tokens + 63);
-  }
+  const int64_t len = keys(p.rows_wg);
   const int64_t splits = kv_splits(p.by_rows, a.view, items, len), chunk = (len + splits - 1) / splits;
   p.chunk = (int)((chunk + unit - 1) / unit * unit);
   p.splits = (int)((len + p.chunk - 1) / p.chunk);  // no more than kv_splits: chunks only grow
