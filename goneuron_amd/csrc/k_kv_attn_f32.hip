@@ -119,13 +119,16 @@ int64_t kv_attn_work_floats(int B, int max_new, int max_len, int H, int KVH, int
   const int R = kv_row(hd), G = H / KVH;
   const int64_t len = std::min(max_len, KV_MAX_TOKENS);
   int64_t most = 0;
-  const auto look = [&](bool by_rows, int64_t tiles, int64_t rows) {  // rows: of a key head
+  const auto look = [&](bool own, int64_t tiles, int64_t rows) {  // own: rows of a wave's own; rows: of a key head
     const int64_t n = std::min<int64_t>(max_new, rows / G);
-    if (n == 0 || (by_rows && n * G <= 16)) return;
-    for (int64_t b = 1; b <= B && b * KVH * tiles <= (by_rows ? 1024 : 2048); ++b) {
+    if (n == 0 || (own && n * G <= 16)) return;
+    const int first = !own && tiles > 1 ? KV_WINDOW : KV_PREFIX;  // prefixes share one tile alone
+    for (int64_t b = 1; b <= B && b * KVH * tiles <= (own ? 1024 : 2048); ++b) {
+      // heads of up to 96 go by rows and sequences alone
+      const bool views = every_view && (!own || R > 96 || by_rows(KV_TREE, b * KVH, n * G, len, R, 4));
       int64_t s = 0;
-      for (int view = KV_PREFIX; view <= (every_view ? KV_TREE : KV_PREFIX); ++view)
-        s = std::max(s, kv_splits(by_rows, view, b * KVH * tiles, len));
+      for (int view = first; view <= (views ? KV_TREE : KV_PREFIX); ++view)
+        s = std::max(s, kv_splits(own, view, b * KVH * tiles, len));
       if (s > 1) most = std::max(most, s * b * n * H);
     }
   };

@@ -76,6 +76,14 @@ def test_sizes_at_random(L, heads):
             assert need <= min(have), (more, have, need, what)
 
 
+@pytest.mark.parametrize("B,new,length,heads,rows", [(8, 128, 8192, (32, 8, 64), 65536), (2, 2000, 4000, (8, 8, 96), 65536),
+                                                     (1, 64, 32768, (16, 2, 32), 65536), (3, 300, 9000, (12, 3, 80), 65280)])
+def test_heads_that_share_their_rows_take_no_more_than_prefixes(L, B, new, length, heads, rows):
+    """As many (split, token, head) rows as prefixes are split into, each with a maximum and a sum."""
+    R = next(r for r in (32, 64, 96) if r >= heads[2])
+    assert grant(L, B, new, length, heads) == rows * (R + 2)
+
+
 # ---------------------------------------------------------------- the layer, which sees prefixes alone
 def layer(L, B, rows, new, length, D, heads):
     """Floats that it asks for beside its own rows."""
