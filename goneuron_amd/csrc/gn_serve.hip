@@ -260,9 +260,13 @@ extern "C" int gn_kv_attention_workspace(int32_t B, int32_t max_new, int32_t max
 }
 
 // Not of the public interface: what a call of these sizes would take of its workspace
-// (view: KvView), for the test that holds it against gn_kv_attention_workspace.
+// (view: KvView; -1 for sizes that no call has), for the test that holds it against
+// gn_kv_attention_workspace.
 extern "C" int64_t gn_kv_attention_need(int32_t view, int32_t B, int32_t max_new, int32_t max_len, int32_t heads,
                                         int32_t kv_heads, int32_t head_dim, int32_t sinks, int32_t window, int32_t dtype) {
+  if (view < KV_PREFIX || view > KV_TREE || B < 1 || max_new < 1 || max_len < 0 || heads < 1 || kv_heads < 1 ||
+      heads % kv_heads || head_dim < 1 || head_dim > KV_MAX_HEAD || sinks < 0 || window < 0 || too_many_rows(B, max_new, heads))
+    return -1;
   KvAttnArgs a{};
   a.c.B = B;
   a.c.max_new = max_new;

@@ -46,6 +46,14 @@ def test_long_windows_of_few_sequences(L, B, heads, length, window):
     assert 0 < need <= grant(L, B, 1, length, heads)
 
 
+def test_sizes_that_no_call_has(L):
+    good = dict(view=WINDOW, B=1, new=1, length=9000, heads=8, kvh=1, hd=64, sinks=0, window=9000, dtype=0)
+    assert L.gn_kv_attention_need(*good.values()) > 0
+    for kw in (dict(view=-1), dict(view=3), dict(B=0), dict(new=0), dict(length=-1), dict(heads=0), dict(kvh=0), dict(kvh=3), dict(hd=0),
+               dict(hd=257), dict(sinks=-1), dict(window=-1), dict(B=ALL, new=ALL)):
+        assert L.gn_kv_attention_need(*{**good, **kw}.values()) == -1, kw
+
+
 @pytest.mark.parametrize("heads", HEADS)
 def test_few_sequences_of_every_view(L, heads):
     windows = [(s, w) for s in (0, 4, 70000, ALL) for w in (1, 4096, 32768, 33333, 40000, 65536, 131072, ALL)]
